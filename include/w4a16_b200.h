@@ -425,6 +425,97 @@ W4A16_API int w4a16_gemm_prefill_dual_gate_up_swiglu_w4a16(const uint32_t* gate_
                                                            w4a16_stream_t stream, int hidden_size,
                                                            int intermediate_size);
 
+/* ---- 4-bit key/value cache: append, attention, eviction --------------------------- */
+/*
+ * What lies between the QKV projection and the O projection, on a cache of 136 bytes per position and key/value head
+ * instead of 512 (no reference counterpart: its cache is fp16, src/kernels/rmsnorm_rope.cu:320-423 and
+ * src/kernels/attention_gqa.cu).  head_dim is 128.
+ *
+ * A cached row (one position of one head) is one quantisation group with a zero point:
+ *   scale = fp16((max - min) / 15), zero = fp16(min + 8 scale), code = clamp(rn((x - zero) / scale) + 8, 0, 15),
+ *   value = (code - 8) * scale + zero;  a row that holds an infinity or a NaN reads back as NaN.
+ * The pool is uint32 [num_pages][num_kv_heads][34 * page_size]; a record is
+ *   key codes [page_size][16] | value codes [page_size][16] | key (scale, zero) [page_size] | value (scale, zero) [page_size]
+ * with code words packed as the weight words above and (scale, zero) an fp16 pair, scale in the low half.
+ * page_size is a power of two from 16 to 4096.
+ */
+typedef struct w4a16_kv4_cache {
+    void* pages;               /* the pool, 16-byte aligned */
+    float* key_weight;         /* fp32 [num_pages][num_kv_heads][page_size]: attention weight a position has got; may be
+                                  NULL where nothing is evicted */
+    int num_pages, num_kv_heads, page_size;
+} w4a16_kv4_cache;
+/*
+ * The sequences of a call.  seq_lens counts a sequence's cached positions WITH the call's new tokens; new token i of n
+ * is position seq_lens - n + i, and sees the positions up to its own.  The arrays live in device memory and are read
+ * when the kernels run, so a captured graph follows them.  Positions beyond the block table do not exist; those on a
+ * page number outside the pool are dropped by append, read back as zero and are not seen by attention.  Rows of the
+ * batch behind the last sequence are left as they are.
+ */
+typedef struct w4a16_kv4_batch {
+    const int32_t* block_table;   /* [num_seqs][max_pages_per_seq] page numbers */
+    const int32_t* seq_lens;      /* [num_seqs] */
+    const int32_t* query_start;   /* [num_seqs + 1] first new token of each sequence, ascending from 0; NULL: one token each
+                                     (num_tokens == num_seqs) */
+    int num_seqs, max_pages_per_seq, num_tokens;
+} w4a16_kv4_batch;
+
+/* Bytes of one page of the pool (all heads), or a status below 0. */
+W4A16_API int64_t w4a16_kv4_page_bytes(int page_size, int num_kv_heads);
+
+/*
+ * Bias, rotary position, quantisation and store of the batch's new tokens in one launch:
+ *   q_out = fp16(rot(q + q_bias)), cached key = Q4(fp16(rot(k + k_bias))), cached value = Q4(fp16(v + v_bias)),
+ * sums and rotation in fp32.  rot turns the pairs (d, d + 64) by positions[token] * rope_inv_freq[d], the angle taken in
+ * 64 bits.  q: fp16 [num_tokens] rows of num_q_heads * 128 (q_stride elements apart, 0: packed), q_out the same, may be q;
+ * both may be NULL.  k, v: rows of num_kv_heads * 128, kv_stride apart.  Biases may be NULL; positions NULL: the cached
+ * position; rope_inv_freq fp32 [64], NULL: no rotation.  New positions start with key_weight 0.  Tensors 16-byte aligned,
+ * strides multiples of 8.  No two tokens of a call may share a cached position.
+ */
+W4A16_API int w4a16_kv4_append(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, const void* q, const void* k,
+                               const void* v, const void* q_bias, const void* k_bias, const void* v_bias,
+                               const int32_t* positions, const float* rope_inv_freq, void* q_out, int num_q_heads, int q_stride,
+                               int kv_stride, w4a16_stream_t stream);
+
+/* The rows of the batch's new tokens as fp16 [num_tokens][num_kv_heads][128], cut at +-65504; either output may be NULL. */
+W4A16_API int w4a16_kv4_read(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, void* k_out, void* v_out,
+                             w4a16_stream_t stream);
+
+/*
+ * out[token][head] = sum over the positions j that the token sees of softmax_j(softmax_scale * q . key_j) * value_j;
+ * query heads share key/value heads in consecutive groups.  out: fp16, or fp32 with out_fp32 (what
+ * w4a16_gemv_attn_heads_f32_w4a16 takes), [num_tokens][num_q_heads][128]; lse (may be NULL): fp32
+ * [num_tokens][num_q_heads], the logarithm of the sum of exp(softmax_scale * q . key_j).  A token that sees nothing
+ * gives zeros and -infinity.  workspace: w4a16_attention_kv4_workspace_bytes() of device memory that no other call in
+ * flight uses (nothing is kept in it between calls); NULL where that is 0.
+ */
+W4A16_API int64_t w4a16_attention_kv4_workspace_bytes(int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads);
+W4A16_API int w4a16_attention_kv4(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, const void* q, void* out,
+                                  float* lse, void* workspace, int num_q_heads, int64_t workspace_bytes, int out_fp32,
+                                  float softmax_scale, int q_stride, w4a16_stream_t stream);
+
+/*
+ * key_weight[position] += sum over the batch's tokens that see it and over the query heads of its group of
+ * exp(softmax_scale * q . key - lse): how much attention each cached position got from these tokens.  q and lse are those
+ * of the attention call; passing only the last tokens of each sequence adds up an observation window.
+ */
+W4A16_API int w4a16_kv4_add_key_weights(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, const void* q,
+                                        const float* lse, int num_q_heads, float softmax_scale, int q_stride,
+                                        w4a16_stream_t stream);
+
+/*
+ * Cuts every sequence down to `budget` positions, each head by itself: its first num_sink, its last num_recent, and of
+ * the rest those with the largest key_weight (the earlier of equal ones; a NaN is the smallest).  What stays keeps its
+ * order and is copied, rows and weights, to the pages of dst_block_table [num_seqs][dst_max_pages_per_seq], which must not
+ * hold pages of the sequences being cut; the old pages are left as they are, so pages shared with other sequences are
+ * safe.  Sequences that fit are copied whole.  new_seq_lens [num_seqs] = min(length, budget);
+ * kept int32 [num_seqs][num_kv_heads][budget]: the old positions in order, -1 behind the last.  num_tokens and query_start
+ * of the batch are not used.
+ */
+W4A16_API int w4a16_kv4_evict(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, const int32_t* dst_block_table,
+                              int32_t* new_seq_lens, int32_t* kept, int dst_max_pages_per_seq, int budget, int num_sink,
+                              int num_recent, w4a16_stream_t stream);
+
 /* ---- decode projection sweep -------------------------------------------------------- */
 
 /*

@@ -44,6 +44,17 @@ class QwenBinBiases(ctypes.Structure):
     _fields_ = [(n, c_void_p) for n in ("q_bias", "k_bias", "v_bias")]
 
 
+class KV4CacheView(ctypes.Structure):
+    """Mirror of w4a16_kv4_cache."""
+    _fields_ = [("pages", c_void_p), ("key_weight", c_void_p)] + [(n, c_int) for n in ("num_pages", "num_kv_heads", "page_size")]
+
+
+class KV4BatchView(ctypes.Structure):
+    """Mirror of w4a16_kv4_batch."""
+    _fields_ = [(n, c_void_p) for n in ("block_table", "seq_lens", "query_start")] + [
+        (n, c_int) for n in ("num_seqs", "max_pages_per_seq", "num_tokens")]
+
+
 class SweepDesc(ctypes.Structure):
     """Mirror of w4a16_sweep_desc."""
     _fields_ = [("num_layers", c_int), ("hidden_size", c_int), ("intermediate_size", c_int),
@@ -110,6 +121,16 @@ SIGNATURES = {
     "w4a16_gemm_prefill_dual_gate_up_swiglu_w4a16": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                                                      c_int, c_int],
     "w4a16_gemv_group_dots": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
+    "w4a16_kv4_page_bytes": [c_int, c_int],
+    "w4a16_kv4_append": [POINTER(KV4CacheView), POINTER(KV4BatchView), *[c_void_p] * 9, c_int, c_int, c_int, c_void_p],
+    "w4a16_kv4_read": [POINTER(KV4CacheView), POINTER(KV4BatchView), c_void_p, c_void_p, c_void_p],
+    "w4a16_attention_kv4_workspace_bytes": [c_int, c_int, c_int, c_int],
+    "w4a16_attention_kv4": [POINTER(KV4CacheView), POINTER(KV4BatchView), c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                            ctypes.c_int64, c_int, ctypes.c_float, c_int, c_void_p],
+    "w4a16_kv4_add_key_weights": [POINTER(KV4CacheView), POINTER(KV4BatchView), c_void_p, c_void_p, c_int, ctypes.c_float, c_int,
+                                  c_void_p],
+    "w4a16_kv4_evict": [POINTER(KV4CacheView), POINTER(KV4BatchView), c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                        c_void_p],
     "w4a16_debug_counter": [c_int, POINTER(ctypes.c_uint)],
     "w4a16_sweep_workspace_bytes": [c_int, c_int, c_int, c_int, c_int],
     "w4a16_sweep_create": [POINTER(SweepDesc), c_void_p, POINTER(c_void_p)],
@@ -120,7 +141,8 @@ SIGNATURES = {
     "w4a16_sweep_buffer": [c_void_p, c_int],
     "w4a16_sweep_status": [c_void_p, POINTER(c_int)],
 }
-RESTYPES = {"w4a16_sweep_workspace_bytes": ctypes.c_int64, "w4a16_sweep_buffer": c_void_p}
+RESTYPES = {"w4a16_sweep_workspace_bytes": ctypes.c_int64, "w4a16_kv4_page_bytes": ctypes.c_int64,
+            "w4a16_attention_kv4_workspace_bytes": ctypes.c_int64, "w4a16_sweep_buffer": c_void_p}
 
 _lib = None
 

@@ -1,9 +1,11 @@
 // extern "C" boundary of the library: argument checks, then the kernel launchers.
 // Declarations and the reference functions they replace: include/w4a16_b200.h.
 #include <atomic>
+#include <cmath>
 #include <cstdlib>
 #include <mutex>
 
+#include "kv4_attention.hpp"
 #include "w4a16_internal.hpp"
 
 namespace w4 {
@@ -82,6 +84,35 @@ inline const __half* H(const void* p) { return static_cast<const __half*>(p); }
 inline __half* H(void* p) { return static_cast<__half*>(p); }
 inline cudaStream_t S(w4a16_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
 inline bool misaligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
+
+// The 4-bit key/value cache and the batch that a call works on: argument checks, then the kernels' view of both.
+int kv4_view(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, Kv4View* v) {
+    if (!cache || !batch || !cache->pages || !batch->block_table || !batch->seq_lens) return W4A16_ERR_INVALID_ARG;
+    if (cache->num_pages <= 0 || cache->num_kv_heads <= 0 || batch->num_seqs <= 0 || batch->max_pages_per_seq <= 0 || batch->num_tokens <= 0)
+        return W4A16_ERR_INVALID_ARG;
+    if (!batch->query_start && batch->num_tokens != batch->num_seqs) return W4A16_ERR_INVALID_ARG;
+    const int ps = cache->page_size;
+    if (ps < 16 || ps > 4096 || (ps & (ps - 1)) != 0) return W4A16_ERR_SHAPE;
+    if (misaligned(cache->pages, 16) || misaligned(cache->key_weight, 4) || misaligned(batch->block_table, 4) || misaligned(batch->seq_lens, 4) ||
+        misaligned(batch->query_start, 4))
+        return W4A16_ERR_ALIGNMENT;
+    if (cache->num_kv_heads > 65535 || batch->num_seqs > 65535 || batch->num_tokens > (1 << 24)) return W4A16_ERR_TOO_LARGE;
+    int shift = 4;
+    while ((1 << shift) < ps) ++shift;
+    *v = Kv4View{static_cast<uint32_t*>(cache->pages), cache->key_weight, batch->block_table, batch->seq_lens, batch->query_start,
+                 cache->num_pages, cache->num_kv_heads, shift, batch->num_seqs, batch->max_pages_per_seq, batch->num_tokens};
+    return 0;
+}
+// Query heads over key/value heads, and the row stride of q (0: the heads packed).
+int kv4_heads(const Kv4View& v, int num_q_heads, int* stride, int heads) {
+    if (num_q_heads <= 0) return W4A16_ERR_INVALID_ARG;
+    if (num_q_heads % v.kv_heads != 0) return W4A16_ERR_SHAPE;
+    if (num_q_heads > 65535 || static_cast<long long>(v.num_tokens) * num_q_heads > (1ll << 30)) return W4A16_ERR_TOO_LARGE;
+    if (*stride < 0) return W4A16_ERR_INVALID_ARG;
+    if (*stride == 0) *stride = heads * kKvDim;
+    if (*stride < heads * kKvDim) return W4A16_ERR_SHAPE;
+    return *stride % 8 == 0 ? 0 : W4A16_ERR_ALIGNMENT;
+}
 
 int check_k(int K) { return (K > 0 && K % 256 == 0) ? 0 : W4A16_ERR_SHAPE; }
 
@@ -619,6 +650,88 @@ int w4a16_gemv_group_dots(const uint32_t* qweight, const int8_t* input_q8, const
     if (int st = check_k(in_features)) return st;
     if (misaligned(qweight, 4) || misaligned(input_sum8, 4) || misaligned(out_dots, 4)) return W4A16_ERR_ALIGNMENT;
     return gemv_group_dots(qweight, input_q8, input_sum8, out_dots, out_features, in_features, S(stream));
+}
+
+// ---- 4-bit key/value cache ---------------------------------------------------------------------------------------
+
+int64_t w4a16_kv4_page_bytes(int page_size, int num_kv_heads) {
+    if (page_size < 16 || page_size > 4096 || (page_size & (page_size - 1)) != 0) return W4A16_ERR_SHAPE;
+    if (num_kv_heads <= 0) return W4A16_ERR_INVALID_ARG;
+    return static_cast<int64_t>(page_size) * num_kv_heads * kKvSlotWords * 4;
+}
+
+int w4a16_kv4_append(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, const void* q, const void* k, const void* v,
+                     const void* q_bias, const void* k_bias, const void* v_bias, const int32_t* positions,
+                     const float* rope_inv_freq, void* q_out, int num_q_heads, int q_stride, int kv_stride, w4a16_stream_t stream) {
+    Kv4View c;
+    if (int st = kv4_view(cache, batch, &c)) return st;
+    if (!k || !v || (q == nullptr) != (q_out == nullptr) || (q_bias && !q)) return W4A16_ERR_INVALID_ARG;
+    if (int st = kv4_heads(c, num_q_heads, &q_stride, num_q_heads)) return st;
+    if (int st = kv4_heads(c, num_q_heads, &kv_stride, c.kv_heads)) return st;
+    if (misaligned(q, 16) || misaligned(k, 16) || misaligned(v, 16) || misaligned(q_out, 16) || misaligned(q_bias, 16) || misaligned(k_bias, 16) ||
+        misaligned(v_bias, 16) || misaligned(positions, 4) || misaligned(rope_inv_freq, 4))
+        return W4A16_ERR_ALIGNMENT;
+    if (int st = ensure_device_ready(nullptr)) return st;
+    return kv4_append(c, Kv4AppendArgs{H(q), H(k), H(v), H(q_bias), H(k_bias), H(v_bias), H(q_out), positions, rope_inv_freq, num_q_heads, q_stride, kv_stride},
+                      S(stream));
+}
+
+int w4a16_kv4_read(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, void* k_out, void* v_out, w4a16_stream_t stream) {
+    Kv4View c;
+    if (int st = kv4_view(cache, batch, &c)) return st;
+    if (!k_out && !v_out) return W4A16_ERR_INVALID_ARG;
+    if (misaligned(k_out, 16) || misaligned(v_out, 16)) return W4A16_ERR_ALIGNMENT;
+    if (int st = ensure_device_ready(nullptr)) return st;
+    return kv4_read(c, H(k_out), H(v_out), S(stream));
+}
+
+int64_t w4a16_attention_kv4_workspace_bytes(int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads) {
+    if (num_tokens <= 0 || num_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0) return W4A16_ERR_INVALID_ARG;
+    if (num_q_heads % num_kv_heads != 0) return W4A16_ERR_SHAPE;
+    if (num_tokens > (1 << 24) || num_seqs > 65535 || num_q_heads > 65535 || static_cast<long long>(num_tokens) * num_q_heads > (1ll << 30))
+        return W4A16_ERR_TOO_LARGE;
+    return kv4_attention_plan(num_tokens, num_seqs, num_q_heads, num_kv_heads).bytes;
+}
+
+int w4a16_attention_kv4(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, const void* q, void* out, float* lse,
+                        void* workspace, int num_q_heads, int64_t workspace_bytes, int out_fp32, float softmax_scale, int q_stride,
+                        w4a16_stream_t stream) {
+    Kv4View c;
+    if (int st = kv4_view(cache, batch, &c)) return st;
+    if (!q || !out || !std::isfinite(softmax_scale) || softmax_scale <= 0.0f) return W4A16_ERR_INVALID_ARG;
+    if (int st = kv4_heads(c, num_q_heads, &q_stride, num_q_heads)) return st;
+    if (misaligned(q, 16) || misaligned(out, 16) || misaligned(lse, 4) || misaligned(workspace, 16)) return W4A16_ERR_ALIGNMENT;
+    const int64_t need = kv4_attention_plan(c.num_tokens, c.num_seqs, num_q_heads, c.kv_heads).bytes;
+    if (need > 0 && (!workspace || workspace_bytes < need)) return W4A16_ERR_INVALID_ARG;
+    if (int st = ensure_device_ready(nullptr)) return st;
+    Kv4AttentionArgs a{};
+    a.c = c; a.q = H(q); a.out = out; a.lse = lse; a.scale = softmax_scale; a.group = num_q_heads / c.kv_heads; a.q_stride = q_stride;
+    return kv4_attention(a, num_q_heads, out_fp32 != 0, workspace, S(stream));
+}
+
+int w4a16_kv4_add_key_weights(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, const void* q, const float* lse, int num_q_heads,
+                              float softmax_scale, int q_stride, w4a16_stream_t stream) {
+    Kv4View c;
+    if (int st = kv4_view(cache, batch, &c)) return st;
+    if (!q || !lse || !c.key_weight || !std::isfinite(softmax_scale) || softmax_scale <= 0.0f) return W4A16_ERR_INVALID_ARG;
+    if (int st = kv4_heads(c, num_q_heads, &q_stride, num_q_heads)) return st;
+    if (misaligned(q, 16) || misaligned(lse, 4)) return W4A16_ERR_ALIGNMENT;
+    if (int st = ensure_device_ready(nullptr)) return st;
+    return kv4_add_key_weights(Kv4WeightArgs{c, H(q), lse, softmax_scale, num_q_heads / c.kv_heads, q_stride}, S(stream));
+}
+
+int w4a16_kv4_evict(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, const int32_t* dst_block_table, int32_t* new_seq_lens,
+                    int32_t* kept, int dst_max_pages_per_seq, int budget, int num_sink, int num_recent, w4a16_stream_t stream) {
+    Kv4View c;
+    if (int st = kv4_view(cache, batch, &c)) return st;
+    if (!c.key_weight || !dst_block_table || !new_seq_lens || !kept || dst_max_pages_per_seq <= 0 || budget <= 0 || num_sink < 0 || num_recent < 0)
+        return W4A16_ERR_INVALID_ARG;
+    if (dst_block_table == batch->block_table) return W4A16_ERR_INVALID_ARG;
+    if (static_cast<long long>(num_sink) + num_recent > budget) return W4A16_ERR_SHAPE;
+    if (static_cast<long long>(dst_max_pages_per_seq) * cache->page_size < budget) return W4A16_ERR_SHAPE;
+    if (misaligned(dst_block_table, 4) || misaligned(new_seq_lens, 4) || misaligned(kept, 4)) return W4A16_ERR_ALIGNMENT;
+    if (int st = ensure_device_ready(nullptr)) return st;
+    return kv4_evict(c, Kv4EvictArgs{dst_block_table, new_seq_lens, kept, dst_max_pages_per_seq, budget, num_sink, num_recent}, S(stream));
 }
 
 int w4a16_debug_counter(int which, unsigned int* out) {

@@ -1,0 +1,99 @@
+// The 4-bit key/value cache: layout, index arithmetic and conversions shared by its kernels (sm_100a).
+//
+// A page record holds page_size rows of one key/value head, 34 words a position:
+//   key codes [page_size][16] | value codes [page_size][16] | key (scale, zero) [page_size] | value (scale, zero) [page_size]
+// A row is 128 values quantised as one group with a zero point: value = (code - 8) * scale + zero; its 16 words are packed as
+// the library's weight words are (element j of a word at bit {0, 8, 16, 24, 4, 12, 20, 28}[j]); (scale, zero) is an fp16 pair
+// with the scale in the low half.  8 is subtracted for the same reason as in the weights: the products of a long sum then
+// have both signs, and the 32-bit accumulators of the tensor cores do not grow with its length.
+//
+// Every index that comes from device memory is checked before it forms an address: lengths are cut at what the block table
+// can hold, a page number outside the pool makes its positions unreadable (append drops them, read gives zero, attention does
+// not see them).
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "w4a16_common.cuh"
+
+namespace w4 {
+
+constexpr int kKvDim = 128;              // values of a head
+constexpr int kKvRowWords = 16;          // words of codes of a row
+constexpr int kKvSlotWords = 34;         // words of a position in a record
+constexpr int kKvTile = 16;              // positions that lie in one page for certain
+
+struct Kv4View {
+    uint32_t* pages;
+    float* key_weight;                   // [num_pages][kv_heads][page_size] or null
+    const int32_t* table;                // [num_seqs][max_pages]
+    const int32_t* lens;                 // [num_seqs]
+    const int32_t* qstart;               // [num_seqs + 1] or null: one token a sequence
+    int num_pages, kv_heads, page_shift, num_seqs, max_pages, num_tokens;
+};
+
+// New tokens of sequence b: first row of the batch and count, both inside the batch whatever the array holds.
+__device__ __forceinline__ int2 kv4_new_tokens(const Kv4View& c, int b) {
+    if (c.qstart == nullptr) return make_int2(b, b < c.num_tokens ? 1 : 0);
+    const int first = min(max(__ldcg(c.qstart + b), 0), c.num_tokens);
+    const int end = min(max(__ldcg(c.qstart + b + 1), first), c.num_tokens);
+    return make_int2(first, end - first);
+}
+__device__ __forceinline__ int kv4_capacity(const Kv4View& c) {
+    return static_cast<int>(min(static_cast<long long>(c.max_pages) << c.page_shift, 0x7FFFFFF0ll));
+}
+// The record of position `at` of a sequence and head; null where the table has no page of the pool there.
+__device__ __forceinline__ uint32_t* kv4_record_of_page(const Kv4View& c, int page, int head) {
+    if (static_cast<unsigned>(page) >= static_cast<unsigned>(c.num_pages)) return nullptr;
+    const size_t record = static_cast<size_t>(page) * c.kv_heads + head;
+    return c.pages + ((record * kKvSlotWords) << c.page_shift);
+}
+__device__ __forceinline__ int kv4_page(const Kv4View& c, int b, int at) {
+    return __ldcg(c.table + static_cast<size_t>(b) * c.max_pages + (at >> c.page_shift));
+}
+__device__ __forceinline__ size_t kv4_weight_index(const Kv4View& c, int page, int head, int at) {
+    return (((static_cast<size_t>(page) * c.kv_heads + head) << c.page_shift) | (at & ((1 << c.page_shift) - 1)));
+}
+
+// Sequence of a token: how many sequences end at or before it.  A whole warp calls it; one round trip for up to 32 sequences.
+__device__ __forceinline__ int kv4_seq_of_token(const Kv4View& c, int token) {
+    if (c.qstart == nullptr) return token;
+    int before = 0;
+    for (int i = threadIdx.x & 31; i < c.num_seqs; i += 32) before += __ldcg(c.qstart + i + 1) <= token;
+    return __reduce_add_sync(0xFFFFFFFFu, before);
+}
+
+__device__ __forceinline__ float kv4_scale(uint32_t params) { return __half2float(__ushort_as_half(static_cast<unsigned short>(params))); }
+__device__ __forceinline__ float kv4_zero(uint32_t params) { return __half2float(__ushort_as_half(static_cast<unsigned short>(params >> 16))); }
+
+// Four pairs (code - 8) as fp16 out of a word whose nibbles are a pair in each byte column: pair n holds the nibbles at bits
+// 4 n and 16 + 4 n.  0x6400 | c is 1024 + c and 0x6400 | c << 4 is 1024 + 16 c, so one addition or one fma gives c - 8, exactly.
+__device__ __forceinline__ void kv4_codes_to_half2(uint32_t w, uint32_t (&out)[4]) {
+    const __half2 a = __float2half2_rn(-1032.0f), m = __float2half2_rn(0.0625f), b = __float2half2_rn(-72.0f);
+    const uint32_t u = w >> 8;
+    uint32_t r[4];
+    asm("lop3.b32 %0, %1, 0x000F000F, 0x64006400, 0xEA;" : "=r"(r[0]) : "r"(w));
+    asm("lop3.b32 %0, %1, 0x00F000F0, 0x64006400, 0xEA;" : "=r"(r[1]) : "r"(w));
+    asm("lop3.b32 %0, %1, 0x000F000F, 0x64006400, 0xEA;" : "=r"(r[2]) : "r"(u));
+    asm("lop3.b32 %0, %1, 0x00F000F0, 0x64006400, 0xEA;" : "=r"(r[3]) : "r"(u));
+    __half2 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<const __half2*>(&r[i]);
+    h[0] = __hadd2(h[0], a);
+    h[1] = __hfma2(h[1], m, b);
+    h[2] = __hadd2(h[2], a);
+    h[3] = __hfma2(h[3], m, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = *reinterpret_cast<const uint32_t*>(&h[i]);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+}  // namespace w4

@@ -1,0 +1,554 @@
+// Attention over the 4-bit key/value cache for single tokens and small groups of them, and the attention weight of every
+// cached position.
+//
+// Both contract small sets of query rows with the cached rows on mma.sync.m16n8k16, the cached positions (or the values'
+// dimensions) as the 16 rows of A and the queries as the 8 columns of B: a decode step has as many query rows as a key/value
+// head has query heads, and these, not the positions, are what is padded.  The rows of a head (token major) are cut into tiles
+// of 8 or 16; a tile's positions are split over CTAs, a CTA's over its four warps, 16 positions at a time.
+//
+//   scores^T [16 positions x 8 queries] = codes [16 x 128] . q^T;  then scale * score + zero * (sum of q), because a row is
+//       (code - 8) * scale + zero: the codes are exact in fp16 and no key is ever rounded.
+//   out^T [128 x 8] += codes^T [128 x 16] . (p * value scale)^T: the weight enters as two fp16 numbers whose sum has 22
+//       bits (one would leave 2^-11 in a 32-bit result), zeros as one 32-bit sum a query.
+//   running maximum: renewed only where a score exceeds it by 2^8, which a vote finds; p <= 2^8 fits.
+#include "kv4.cuh"
+#include "kv4_attention.hpp"
+#include "w4a16_internal.hpp"
+
+namespace w4 {
+namespace {
+
+constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Query rows of a tile and the positions they see.
+struct QTile {
+    int seq, first_token, n;      // the sequence, its first row in the batch, its new tokens
+    int row0, rows;               // rows of (token, query head of the group) in the sequence, token major
+    int past;                     // positions in front of the first new token (negative where the batch has more tokens than positions)
+    int seen;                     // positions that the tile's last row sees
+};
+
+// The tile with number `index`, in order of the sequences; false past the last one.  A whole warp calls it.
+__device__ __forceinline__ bool find_qtile(const Kv4View& c, int group, int tile_rows, int index, QTile* out) {
+    const int lane = threadIdx.x & 31;
+    int b = -1, t = 0;
+    if (c.qstart == nullptr) {
+        const int per = (group + tile_rows - 1) / tile_rows;
+        b = index / per;
+        t = index - b * per;
+        if (b >= c.num_seqs) return false;
+    } else {
+        int before = 0;
+        for (int b0 = 0; b0 < c.num_seqs; b0 += 32) {
+            int mine = 0;
+            if (b0 + lane < c.num_seqs) mine = (kv4_new_tokens(c, b0 + lane).y * group + tile_rows - 1) / tile_rows;
+            int upto = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+                if (lane >= d) upto += o;
+            }
+            const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + upto > index);
+            if (past != 0) {
+                const int l = __ffs(past) - 1;
+                b = b0 + l;
+                t = index - before - __shfl_sync(0xFFFFFFFFu, upto - mine, l);
+                break;
+            }
+            before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+        }
+        if (b < 0) return false;
+    }
+    const int2 mine = kv4_new_tokens(c, b);
+    const int len = max(__ldcg(c.lens + b), 0);
+    out->seq = b;
+    out->first_token = mine.x;
+    out->n = mine.y;
+    out->row0 = t * tile_rows;
+    out->rows = min(tile_rows, mine.y * group - out->row0);
+    out->past = len - mine.y;
+    out->seen = min(max(out->past + (out->row0 + out->rows - 1) / group + 1, 0), kv4_capacity(c));
+    return out->rows > 0;
+}
+
+// Positions of one split of `seen`; a multiple of what a CTA takes in one go.
+__device__ __forceinline__ int split_positions(int seen, int splits, int least) {
+    const int n = min(splits, max(1, (seen + least - 1) / least));
+    const int per = (seen + n - 1) / n;
+    constexpr int kStep = kKvTile * kAttnWarps;
+    return max(kStep, (per + kStep - 1) / kStep * kStep);
+}
+
+// What a lane holds of 16 positions: rows g and g + 8 of the keys, four positions' share of the values.
+struct KvRegs {
+    uint4 k[2];
+    uint2 v[4];
+    uint32_t kp[2], vp[2];
+    bool ok;
+};
+__device__ __forceinline__ void load_tile(const Kv4View& c, int page, int head, int at, int g, int t, KvRegs& r) {
+    const uint32_t* record = kv4_record_of_page(c, page, head);
+    r.ok = record != nullptr;
+    if (!r.ok) return;
+    const int ps = 1 << c.page_shift, s = at & (ps - 1);
+    const uint32_t* keys = record + s * kKvRowWords;
+    const uint32_t* values = keys + ps * kKvRowWords;
+    const uint32_t* params = record + 32 * ps + s;
+    r.k[0] = __ldcg(reinterpret_cast<const uint4*>(keys + g * kKvRowWords + 4 * t));
+    r.k[1] = __ldcg(reinterpret_cast<const uint4*>(keys + (g + 8) * kKvRowWords + 4 * t));
+    r.kp[0] = __ldcg(params + g);
+    r.kp[1] = __ldcg(params + g + 8);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        r.v[i] = __ldcg(reinterpret_cast<const uint2*>(values + (2 * t + (i & 1) + 8 * (i >> 1)) * kKvRowWords + 2 * g));
+    r.vp[0] = __ldcg(params + ps + g);
+    r.vp[1] = __ldcg(params + ps + g + 8);
+}
+
+// B fragments of eight query rows for the eight k steps: step 2 j and 2 j + 1 take the elements of word 4 t + j in the order in
+// which the code conversion gives them.
+__device__ __forceinline__ void query_words(const uint4& w, uint32_t* b) {
+    b[0] = __byte_perm(w.x, w.y, 0x5410);
+    b[1] = __byte_perm(w.z, w.w, 0x5410);
+    b[2] = __byte_perm(w.x, w.y, 0x7632);
+    b[3] = __byte_perm(w.z, w.w, 0x7632);
+}
+__device__ __forceinline__ float sum_half8(const uint4& w) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        s += f.x + f.y;
+    }
+    return s;
+}
+
+template <bool F32>
+__device__ __forceinline__ void store_out(void* out, size_t at, float x) {
+    if constexpr (F32) static_cast<float*>(out)[at] = x;
+    else static_cast<__half*>(out)[at] = __float2half_rn(x);
+}
+
+template <int NT, bool F32>
+__global__ void __launch_bounds__(kAttnThreads) kv4_attention_kernel(const __grid_constant__ Kv4AttentionArgs a) {
+    constexpr int R = 8 * NT, kPitch = kKvDim + 4;
+    __shared__ float s_o[kAttnWarps][R][kPitch];
+    __shared__ float2 s_ml[kAttnWarps][R];
+    pdl_wait_prior_grids();
+    pdl_release_dependents();
+    const Kv4View& c = a.c;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int tile_index = blockIdx.x / a.splits, split = blockIdx.x - tile_index * a.splits, head = blockIdx.y;
+    QTile q;
+    if (!find_qtile(c, a.group, R, tile_index, &q)) return;
+    const int per = split_positions(q.seen, a.splits, a.least);
+    const int used = max(1, (q.seen + per - 1) / per);
+    if (split >= used) return;
+    const int k0 = split * per, k1 = min(k0 + per, q.seen);
+
+    // queries: B fragments of rows g (+ 8), and for the lane's columns 2 t, 2 t + 1 the sum of q and how far the row sees
+    uint32_t qb[NT][16];
+    float qsum[NT][2];
+    int limit[NT][2];
+    const float to_log2 = a.scale * kLog2e;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int r = n * 8 + g, row = q.row0 + r;
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (r < q.rows) {
+                const int token = q.first_token + row / a.group, h = head * a.group + row % a.group;
+                w = __ldcg(reinterpret_cast<const uint4*>(a.q + static_cast<size_t>(token) * a.q_stride + h * kKvDim + 32 * t + 8 * j));
+            }
+            s += sum_half8(w);
+            query_words(w, &qb[n][4 * j]);
+        }
+        s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
+        s += __shfl_xor_sync(0xFFFFFFFFu, s, 2);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            qsum[n][e] = __shfl_sync(0xFFFFFFFFu, s, 4 * (2 * t + e)) * to_log2;
+            limit[n][e] = q.past + (q.row0 + min(n * 8 + 2 * t + e, q.rows - 1)) / a.group + 1;
+        }
+    }
+    const int all_see = q.past + q.row0 / a.group + 1;      // positions that every row of the tile sees
+
+    float o[NT][8][4] = {}, m[NT][2], l[NT][2] = {}, zacc[NT][2] = {};
+#pragma unroll
+    for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY;
+    float pw = 0.0f;                                        // power of two on the value scales; 0: not chosen yet
+
+    constexpr int kStep = kKvTile * kAttnWarps;
+    int at = k0 + warp * kKvTile;
+    KvRegs cur;
+    int next_page = -1;
+    if (at < k1) load_tile(c, kv4_page(c, q.seq, at), head, at, g, t, cur);
+    if (at + kStep < k1) next_page = kv4_page(c, q.seq, at + kStep);
+    for (; at < k1; at += kStep) {
+        KvRegs nxt;
+        nxt.ok = false;
+        if (at + kStep < k1) load_tile(c, next_page, head, at + kStep, g, t, nxt);
+        if (at + 2 * kStep < k1) next_page = kv4_page(c, q.seq, at + 2 * kStep);
+        if (cur.ok) {
+            float s[NT][4] = {};
+            const uint32_t kw0[4] = {cur.k[0].x, cur.k[0].y, cur.k[0].z, cur.k[0].w}, kw1[4] = {cur.k[1].x, cur.k[1].y, cur.k[1].z, cur.k[1].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t lo[4], hi[4];
+                kv4_codes_to_half2(kw0[j], lo);
+                kv4_codes_to_half2(kw1[j], hi);
+                const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]}, a1[4] = {lo[2], hi[2], lo[3], hi[3]};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    mma_16816(s[n], a0, qb[n][4 * j], qb[n][4 * j + 1]);
+                    mma_16816(s[n], a1, qb[n][4 * j + 2], qb[n][4 * j + 3]);
+                }
+            }
+            const float ks[2] = {kv4_scale(cur.kp[0]) * to_log2, kv4_scale(cur.kp[1]) * to_log2};
+            const float kz[2] = {kv4_zero(cur.kp[0]), kv4_zero(cur.kp[1])};
+            float vs[2] = {kv4_scale(cur.vp[0]), kv4_scale(cur.vp[1])}, vz[2] = {kv4_zero(cur.vp[0]), kv4_zero(cur.vp[1])};
+            const bool cut = at + kKvTile > all_see;        // some row does not see some of these positions
+            bool above = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[n][e] = fmaf(s[n][e], ks[e >> 1], kz[e >> 1] * qsum[n][e & 1]);
+                    if (cut && at + g + 8 * (e >> 1) >= limit[n][e & 1]) s[n][e] = -INFINITY;
+                    above = above || s[n][e] > m[n][e & 1] + 8.0f;
+                }
+            if (cut) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (at + g + 8 * i >= k1) vs[i] = vz[i] = 0.0f;
+            }
+            const bool far = pw == 0.0f || vs[0] * pw > 64.0f || vs[1] * pw > 64.0f;
+            if (__any_sync(0xFFFFFFFFu, above || far)) {
+                float big = fmaxf(vs[0], vs[1]);
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, d));
+                float ratio = 1.0f;
+                if (pw == 0.0f || big * pw > 64.0f) {       // the largest value scale times pw into [8, 16)
+                    const float fresh = big > 0.0f ? __uint_as_float((130u + 127u - (__float_as_uint(big) >> 23)) << 23) : 1.0f;
+                    ratio = pw == 0.0f ? 1.0f : fresh / pw;
+                    pw = fresh;
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float x = fmaxf(s[n][e], s[n][e + 2]);
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
+                        const float fresh = fmaxf(m[n][e], x);
+                        const float f = fresh == m[n][e] ? 1.0f : ex2(m[n][e] - fresh);
+                        m[n][e] = fresh;
+                        l[n][e] *= f;
+                        zacc[n][e] *= f;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            o[n][i][e] *= f * ratio;
+                            o[n][i][e + 2] *= f * ratio;
+                        }
+                    }
+            }
+            vs[0] *= pw;
+            vs[1] *= pw;
+            uint32_t ph[NT][2], pl[NT][2];                  // p * value scale in two fp16 parts, columns = positions
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float top = m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1];
+                    const float p = ex2(s[n][e] - top);
+                    l[n][e & 1] += p;
+                    x[e] = p * vs[e >> 1];
+                    float z = p * vz[e >> 1];
+                    if (cut && at + g + 8 * (e >> 1) >= limit[n][e & 1]) x[e] = z = 0.0f;   // whatever the row holds
+                    zacc[n][e & 1] += z;
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+                    const float2 f = __half22float2(h);
+                    ph[n][i] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&h));
+                    pl[n][i] = transpose_8x8(pack_half2(x[2 * i] - f.x, x[2 * i + 1] - f.y));
+                }
+            }
+            // values: pair two positions' words by 16-bit halves, then each nibble place is one dimension of both
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t sel = half ? 0x7632u : 0x5410u;
+                uint32_t f[4][4];
+                kv4_codes_to_half2(__byte_perm(cur.v[0].x, cur.v[1].x, sel), f[0]);
+                kv4_codes_to_half2(__byte_perm(cur.v[0].y, cur.v[1].y, sel), f[1]);
+                kv4_codes_to_half2(__byte_perm(cur.v[2].x, cur.v[3].x, sel), f[2]);
+                kv4_codes_to_half2(__byte_perm(cur.v[2].y, cur.v[3].y, sel), f[3]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t av[4] = {f[0][i], f[1][i], f[2][i], f[3][i]};
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma_16816(o[n][half * 4 + i], av, ph[n][0], ph[n][1]);
+                        mma_16816(o[n][half * 4 + i], av, pl[n][0], pl[n][1]);
+                    }
+                }
+            }
+        }
+        cur = nxt;
+    }
+
+    // the warps' parts into shared memory: a lane has dimensions 16 g .. 16 g + 15 of queries 2 t and 2 t + 1
+    const float undo = pw == 0.0f ? 1.0f : 1.0f / pw;
+    constexpr int kElement[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float ls = l[n][e], zs = zacc[n][e];
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) {
+                ls += __shfl_xor_sync(0xFFFFFFFFu, ls, d);
+                zs += __shfl_xor_sync(0xFFFFFFFFu, zs, d);
+            }
+            const int r = n * 8 + 2 * t + e;
+            if (g == 0) s_ml[warp][r] = make_float2(m[n][e], ls);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                s_o[warp][r][16 * g + kElement[i]] = fmaf(o[n][i][e], undo, zs);
+                s_o[warp][r][16 * g + 8 + kElement[i]] = fmaf(o[n][i][e + 2], undo, zs);
+            }
+        }
+    __syncthreads();
+    const size_t part = (static_cast<size_t>(tile_index) * c.kv_heads + head) * a.splits + split;
+    for (int r = 0; r < q.rows; ++r) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kAttnWarps; ++w) top = fmaxf(top, s_ml[w][r].x);
+        float sum = 0.0f, x = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kAttnWarps; ++w) {
+            const float2 ml = s_ml[w][r];
+            const float f = ml.x == top ? 1.0f : ex2(ml.x - top);
+            sum = fmaf(ml.y, f, sum);
+            x = fmaf(s_o[w][r][threadIdx.x], f, x);
+        }
+        if (used > 1) {
+            a.part_o[(part * R + r) * kKvDim + threadIdx.x] = x;
+            if (threadIdx.x == 0) a.part_ml[part * R + r] = make_float2(top, sum);
+            continue;
+        }
+        const int row = q.row0 + r, token = q.first_token + row / a.group, h = head * a.group + row % a.group;
+        const size_t at_row = static_cast<size_t>(token) * c.kv_heads * a.group + h;
+        store_out<F32>(a.out, at_row * kKvDim + threadIdx.x, sum == 0.0f ? 0.0f : x / sum);
+        if (threadIdx.x == 0 && a.lse != nullptr) a.lse[at_row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+    }
+}
+
+// The splits of a tile joined; a CTA a tile and head.
+template <bool F32>
+__global__ void __launch_bounds__(kKvDim) kv4_attention_join_kernel(const __grid_constant__ Kv4AttentionArgs a, int tile_rows) {
+    pdl_wait_prior_grids();
+    pdl_release_dependents();
+    const Kv4View& c = a.c;
+    const int head = blockIdx.y;
+    QTile q;
+    if (!find_qtile(c, a.group, tile_rows, blockIdx.x, &q)) return;
+    const int per = split_positions(q.seen, a.splits, a.least);
+    const int used = max(1, (q.seen + per - 1) / per);
+    if (used == 1) return;
+    const size_t part = (static_cast<size_t>(blockIdx.x) * c.kv_heads + head) * a.splits;
+    for (int r = 0; r < q.rows; ++r) {
+        float top = -INFINITY;
+        for (int s = 0; s < used; ++s) top = fmaxf(top, __ldcg(&a.part_ml[(part + s) * tile_rows + r].x));
+        float sum = 0.0f, x = 0.0f;
+        for (int s = 0; s < used; ++s) {
+            const float2 ml = __ldcg(&a.part_ml[(part + s) * tile_rows + r]);
+            const float f = ml.x == top ? 1.0f : ex2(ml.x - top);
+            sum = fmaf(ml.y, f, sum);
+            x = fmaf(__ldcg(a.part_o + ((part + s) * tile_rows + r) * kKvDim + threadIdx.x), f, x);
+        }
+        const int row = q.row0 + r, token = q.first_token + row / a.group, h = head * a.group + row % a.group;
+        const size_t at_row = static_cast<size_t>(token) * c.kv_heads * a.group + h;
+        store_out<F32>(a.out, at_row * kKvDim + threadIdx.x, sum == 0.0f ? 0.0f : x / sum);
+        if (threadIdx.x == 0 && a.lse != nullptr) a.lse[at_row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+    }
+}
+
+// ---- attention weight of the cached positions ------------------------------------------------------------------
+
+// A warp owns 32 positions of a head and adds up, over all query rows of the sequence, exp(score - lse): no position is
+// another warp's, so nothing is atomic and the order of the sum is fixed.  The keys' codes are converted once and stay in
+// registers; the queries pass through shared memory in blocks of 64 rows, already in fragment order.
+constexpr int kWeightRows = 64, kWeightPositions = 32 * kAttnWarps;
+
+__global__ void __launch_bounds__(kAttnThreads) kv4_key_weight_kernel(const __grid_constant__ Kv4WeightArgs a) {
+    __shared__ uint4 s_q[kWeightRows / 8][4][32];
+    __shared__ float s_qsum[kWeightRows], s_lse[kWeightRows];
+    pdl_wait_prior_grids();
+    pdl_release_dependents();
+    const Kv4View& c = a.c;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int head = blockIdx.y, b = blockIdx.z;
+    const int2 mine = kv4_new_tokens(c, b);
+    const int len = max(__ldcg(c.lens + b), 0), seen = min(len, kv4_capacity(c)), past = len - mine.y;
+    const int rows = mine.y * a.group;
+    const float to_log2 = a.scale * kLog2e;
+    for (int base = blockIdx.x * kWeightPositions; base < seen && rows > 0; base += gridDim.x * kWeightPositions) {
+        const int at = base + warp * 32;
+        // codes of positions at + g + {0, 8, 16, 24}
+        uint32_t codes[2][4][2][4];
+        float ks[4], kz[4], got[4] = {};
+        bool ok[2];
+        int pages[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int p = at + 16 * u;
+            pages[u] = p < seen ? kv4_page(c, b, p) : -1;
+            const uint32_t* record = kv4_record_of_page(c, pages[u], head);
+            ok[u] = record != nullptr;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint4 w = make_uint4(0, 0, 0, 0);
+                uint32_t params = 0;
+                if (ok[u]) {
+                    const int ps = 1 << c.page_shift, s = (p & (ps - 1)) + g + 8 * i;
+                    w = __ldcg(reinterpret_cast<const uint4*>(record + s * kKvRowWords + 4 * t));
+                    params = __ldcg(record + 32 * ps + s);
+                }
+                ks[2 * u + i] = kv4_scale(params) * to_log2;
+                kz[2 * u + i] = kv4_zero(params);
+                kv4_codes_to_half2(w.x, codes[u][0][i]);
+                kv4_codes_to_half2(w.y, codes[u][1][i]);
+                kv4_codes_to_half2(w.z, codes[u][2][i]);
+                kv4_codes_to_half2(w.w, codes[u][3][i]);
+            }
+        }
+        for (int r0 = 0; r0 < rows; r0 += kWeightRows) {
+            __syncthreads();
+            // a row is 16 pieces of 16 bytes; half-warps take rows
+            for (int r = threadIdx.x >> 4; r < kWeightRows; r += kAttnThreads / 16) {
+                const int piece = threadIdx.x & 15, row = r0 + r;
+                uint4 w = make_uint4(0, 0, 0, 0);
+                float lse = INFINITY;
+                if (row < rows) {
+                    const int token = mine.x + row / a.group, h = head * a.group + row % a.group;
+                    w = __ldcg(reinterpret_cast<const uint4*>(a.q + static_cast<size_t>(token) * a.q_stride + h * kKvDim + 8 * piece));
+                    lse = __ldcg(a.lse + static_cast<size_t>(token) * c.kv_heads * a.group + h);
+                }
+                float s = sum_half8(w);
+#pragma unroll
+                for (int d = 8; d > 0; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
+                uint32_t f[4];
+                query_words(w, f);
+                s_q[r >> 3][piece & 3][(r & 7) * 4 + (piece >> 2)] = make_uint4(f[0], f[1], f[2], f[3]);
+                if (piece == 0) { s_qsum[r] = s * to_log2; s_lse[r] = lse * kLog2e; }
+            }
+            __syncthreads();
+            const int blocks = (min(rows - r0, kWeightRows) + 7) / 8;
+            for (int n = 0; n < blocks; ++n) {
+                float s[2][4] = {};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint4 f = s_q[n][j][lane];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t a0[4] = {codes[u][j][0][0], codes[u][j][1][0], codes[u][j][0][1], codes[u][j][1][1]};
+                        const uint32_t a1[4] = {codes[u][j][0][2], codes[u][j][1][2], codes[u][j][0][3], codes[u][j][1][3]};
+                        mma_16816(s[u], a0, f.x, f.y);
+                        mma_16816(s[u], a1, f.z, f.w);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int r = n * 8 + 2 * t + e;
+                    const float qs = s_qsum[r], lse = s_lse[r];
+                    const int limit = r0 + r < rows ? past + (r0 + r) / a.group + 1 : 0;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float x = fmaf(s[u][2 * i + e], ks[2 * u + i], kz[2 * u + i] * qs) - lse;
+                            if (at + 16 * u + 8 * i + g < limit) got[2 * u + i] += ex2(x);
+                        }
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            got[i] += __shfl_xor_sync(0xFFFFFFFFu, got[i], 1);
+            got[i] += __shfl_xor_sync(0xFFFFFFFFu, got[i], 2);
+            const int p = at + 8 * i + g;
+            if (t == 0 && p < seen && ok[i >> 1]) {
+                float* w = c.key_weight + kv4_weight_index(c, pages[i >> 1], head, p);
+                *w = __ldcg(w) + got[i];
+            }
+        }
+    }
+}
+
+}  // namespace
+
+Kv4AttentionPlan kv4_attention_plan(int num_tokens, int num_seqs, int q_heads, int kv_heads) {
+    Kv4AttentionPlan p;
+    const long long group = q_heads / kv_heads, rows = group * num_tokens;
+    p.nt = rows > 8ll * num_seqs ? 2 : 1;
+    const long long R = 8 * p.nt;
+    const long long by_token = num_tokens * ((group + R - 1) / R), by_rows = rows / R + num_seqs;
+    p.tiles = by_token < by_rows ? by_token : by_rows;
+    const long long ctas = p.tiles * kv_heads, want = 148 * 8;
+    p.splits = static_cast<int>(ctas >= want ? 1 : (want + ctas - 1) / ctas);
+    if (p.splits > 128) p.splits = 128;
+    p.least = 128;
+    const long long parts = p.splits > 1 ? ctas * p.splits * R : 0;
+    p.ml_offset = parts * kKvDim * 4;
+    p.bytes = p.ml_offset + parts * 8;
+    return p;
+}
+
+int kv4_attention(Kv4AttentionArgs a, int q_heads, bool f32, void* workspace, cudaStream_t stream) {
+    const Kv4View& c = a.c;
+    const Kv4AttentionPlan p = kv4_attention_plan(c.num_tokens, c.num_seqs, q_heads, c.kv_heads);
+    if (p.tiles * p.splits > 0x7FFFFFFFll) return W4A16_ERR_TOO_LARGE;
+    a.splits = p.splits;
+    a.least = p.least;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.ml_offset);
+    const dim3 grid(static_cast<unsigned>(p.tiles * p.splits), c.kv_heads);
+    auto kernel = p.nt == 1 ? (f32 ? kv4_attention_kernel<1, true> : kv4_attention_kernel<1, false>)
+                            : (f32 ? kv4_attention_kernel<2, true> : kv4_attention_kernel<2, false>);
+    cudaError_t e = launch_kernel(kernel, grid, dim3(kAttnThreads), 0, stream, pdl_enabled(), a);
+    if (e != cudaSuccess || p.splits == 1) return static_cast<int>(e);
+    const dim3 join(static_cast<unsigned>(p.tiles), c.kv_heads);
+    return static_cast<int>(launch_kernel(f32 ? kv4_attention_join_kernel<true> : kv4_attention_join_kernel<false>, join, dim3(kKvDim), 0, stream,
+                                          pdl_enabled(), a, 8 * p.nt));
+}
+
+int kv4_add_key_weights(const Kv4WeightArgs& a, cudaStream_t stream) {
+    const Kv4View& c = a.c;
+    const long long blocks = ((static_cast<long long>(c.max_pages) << c.page_shift) + kWeightPositions - 1) / kWeightPositions;
+    const dim3 grid(static_cast<unsigned>(blocks < 4096 ? blocks : 4096), c.kv_heads, c.num_seqs);
+    return static_cast<int>(launch_kernel(kv4_key_weight_kernel, grid, dim3(kAttnThreads), 0, stream, pdl_enabled(), a));
+}
+
+}  // namespace w4

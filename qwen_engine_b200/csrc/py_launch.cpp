@@ -29,7 +29,7 @@ struct Arg {
     bool optional = false;
     int def = 0;
 };
-constexpr int kMaxArgs = 14;
+constexpr int kMaxArgs = 15;
 struct Spec {
     const char* name;         // Python name
     const char* c_name;       // C ABI name, for error messages
@@ -43,6 +43,8 @@ constexpr int kHidden = 1536, kInter = 8960, kQHeads = 12, kKvHeads = 2, kHeadDi
 PyObject* g_str_cuda_stream = nullptr;
 PyObject* g_check = nullptr;                                  // qwen_engine_b200._lib.check
 PyObject* g_view_names[9] = {};                               // attributes of QKVProjectionView, in the C struct's order
+PyObject* g_kv4_cache_names[5] = {};                          // the same of KV4Cache and KV4Batch
+PyObject* g_kv4_batch_names[6] = {};
 
 // A torch call that may throw (a tensor without storage, as under vmap; the current stream where CUDA cannot start): a C++
 // exception must not leave through the interpreter's C frames, which ends the process.
@@ -115,6 +117,32 @@ bool to_stream(PyObject* o, w4a16_stream_t* out) {
     *out = reinterpret_cast<w4a16_stream_t>(p);
     return true;
 }
+bool to_int64(PyObject* o, int64_t* out) {
+    PyObject* i = PyNumber_Index(o);
+    if (i == nullptr) return false;
+    const long long v = PyLong_AsLongLong(i);
+    Py_DECREF(i);
+    if (v == -1 && PyErr_Occurred()) return false;
+    *out = v;
+    return true;
+}
+bool to_float(PyObject* o, float* out) {
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) return false;
+    *out = static_cast<float>(v);
+    return true;
+}
+// `n` attributes of an object, of which the first `pointers` are tensors and the rest integers.
+bool to_fields(PyObject* o, PyObject* const* names, int pointers, int n, void** p, int* v) {
+    for (int i = 0; i < n; ++i) {
+        PyObject* t = PyObject_GetAttr(o, names[i]);
+        if (t == nullptr) return false;
+        const bool ok = i < pointers ? to_pointer(t, &p[i]) : to_int(t, &v[i - pointers]);
+        Py_DECREF(t);               // the object holds the tensor
+        if (!ok) return false;
+    }
+    return true;
+}
 bool to_view(PyObject* o, w4a16_qkv_view* v) {
     void* p[9];
     for (int i = 0; i < 9; ++i) {
@@ -157,6 +185,43 @@ struct Slot<const w4a16_qkv_view*> {
     w4a16_qkv_view v{};
     bool take(PyObject* o, const Arg&) { return to_view(o, &v); }
     const w4a16_qkv_view* get() { return &v; }
+};
+
+template <>
+struct Slot<int64_t> {
+    int64_t v = 0;
+    bool take(PyObject* o, const Arg&) { return to_int64(o, &v); }
+    int64_t get() { return v; }
+};
+template <>
+struct Slot<float> {
+    float v = 0.0f;
+    bool take(PyObject* o, const Arg&) { return to_float(o, &v); }
+    float get() { return v; }
+};
+template <>
+struct Slot<const w4a16_kv4_cache*> {
+    w4a16_kv4_cache c{};
+    bool take(PyObject* o, const Arg&) {
+        void* p[2];
+        int v[3];
+        if (!to_fields(o, g_kv4_cache_names, 2, 5, p, v)) return false;
+        c = {p[0], static_cast<float*>(p[1]), v[0], v[1], v[2]};
+        return true;
+    }
+    const w4a16_kv4_cache* get() { return &c; }
+};
+template <>
+struct Slot<const w4a16_kv4_batch*> {
+    w4a16_kv4_batch b{};
+    bool take(PyObject* o, const Arg&) {
+        void* p[3];
+        int v[3];
+        if (!to_fields(o, g_kv4_batch_names, 3, 6, p, v)) return false;
+        b = {static_cast<const int32_t*>(p[0]), static_cast<const int32_t*>(p[1]), static_cast<const int32_t*>(p[2]), v[0], v[1], v[2]};
+        return true;
+    }
+    const w4a16_kv4_batch* get() { return &b; }
 };
 
 // Positional and keyword arguments into `got` (borrowed, null where left out).
@@ -315,6 +380,24 @@ W4_SPEC(gemv_group_dots, w4a16_gemv_group_dots,
         "Diagnostic: int32 per-group partial sums of the decode GEMV (no reference launcher).",
         {"qweight"}, {"input_q8"}, {"input_sum8"}, {"out_dots"}, {"out_features"}, {"in_features"}, kStream)
 
+W4_SPEC(kv4_append, w4a16_kv4_append,
+        "New tokens into a 4-bit key/value cache: bias, rotary position, quantisation and store; the rotated q beside it.",
+        {"cache"}, {"batch"}, {"q"}, {"k"}, {"v"}, {"q_bias"}, {"k_bias"}, {"v_bias"}, {"positions"}, {"rope_inv_freq"}, {"q_out"},
+        opt("num_q_heads", kQHeads), opt("q_stride", 0), opt("kv_stride", 0), kStream)
+W4_SPEC(kv4_read, w4a16_kv4_read, "Cached rows of the batch's new tokens as fp16.", {"cache"}, {"batch"}, {"k_out"}, {"v_out"}, kStream)
+W4_SPEC(attention_kv4, w4a16_attention_kv4,
+        "Causal attention of the batch's new tokens over their sequences' cached rows; out in fp16 or fp32, lse optional.\n"
+        "workspace: attention_kv4_workspace_bytes() bytes.",
+        {"cache"}, {"batch"}, {"q"}, {"out"}, {"lse"}, {"workspace"}, {"num_q_heads"}, {"workspace_bytes"}, {"out_fp32"},
+        {"softmax_scale"}, opt("q_stride", 0), kStream)
+W4_SPEC(kv4_add_key_weights, w4a16_kv4_add_key_weights,
+        "Adds the attention that each cached position got from the batch's tokens to the cache's key_weight.",
+        {"cache"}, {"batch"}, {"q"}, {"lse"}, {"num_q_heads"}, {"softmax_scale"}, opt("q_stride", 0), kStream)
+W4_SPEC(kv4_evict, w4a16_kv4_evict,
+        "Copies, of every sequence and head, the first, the last and the most attended positions to fresh pages.",
+        {"cache"}, {"batch"}, {"dst_block_table"}, {"new_seq_lens"}, {"kept"}, {"dst_max_pages_per_seq"}, {"budget"},
+        opt("num_sink", 0), opt("num_recent", 0), kStream)
+
 // sweep_run_device(handle, h_in, h_out, stream)
 PyObject* sweep_run_device(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (nargs != 4) {
@@ -358,6 +441,11 @@ PyMethodDef g_methods[] = {
     W4_ENTRY(launch_gemm_prefill_qkv_w4a16, w4a16_gemm_prefill_qkv_w4a16),
     W4_ENTRY(launch_gemm_prefill_dual_gate_up_swiglu_w4a16, w4a16_gemm_prefill_dual_gate_up_swiglu_w4a16),
     W4_ENTRY(gemv_group_dots, w4a16_gemv_group_dots),
+    W4_ENTRY(kv4_append, w4a16_kv4_append),
+    W4_ENTRY(kv4_read, w4a16_kv4_read),
+    W4_ENTRY(attention_kv4, w4a16_attention_kv4),
+    W4_ENTRY(kv4_add_key_weights, w4a16_kv4_add_key_weights),
+    W4_ENTRY(kv4_evict, w4a16_kv4_evict),
     {"sweep_run_device", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&sweep_run_device)), METH_FASTCALL,
      "One pass of a decode sweep (handle of w4a16_sweep_create) on device buffers."},
     {nullptr, nullptr, 0, nullptr}};
@@ -377,5 +465,9 @@ PyMODINIT_FUNC PyInit__launch(void) {
     g_str_cuda_stream = PyUnicode_InternFromString("cuda_stream");
     const char* names[9] = {"q_weight", "q_scale", "d_q", "k_weight", "k_scale", "d_k", "v_weight", "v_scale", "d_v"};
     for (int i = 0; i < 9; ++i) g_view_names[i] = PyUnicode_InternFromString(names[i]);
+    const char* cache[5] = {"pages", "key_weight", "num_pages", "num_kv_heads", "page_size"};
+    for (int i = 0; i < 5; ++i) g_kv4_cache_names[i] = PyUnicode_InternFromString(cache[i]);
+    const char* batch[6] = {"block_table", "seq_lens", "query_start", "num_seqs", "max_pages_per_seq", "num_tokens"};
+    for (int i = 0; i < 6; ++i) g_kv4_batch_names[i] = PyUnicode_InternFromString(batch[i]);
     return PyModule_Create(&g_module);
 }

@@ -26,6 +26,7 @@ __all__ = [
     "launch_gemm_prefill_dual_gate_up_swiglu_w4a16", "gemv_group_dots", "DecodeSweep",
     "launch_gemv_rmsnorm_w4a16", "launch_gemv_qkv_rmsnorm_w4a16", "launch_gemv_dual_gate_up_swiglu_rmsnorm_w4a16", "launch_gemv_dual_gate_up_swiglu_rmsnorm_w4a16_q8_1",
     "gemv_w4a8_peers", "gemm_prefill_w4a16_block", "make_sample_control", "launch_embed_lookup_w4a16", "read_sample_control", "launch_sample_and_advance", "sample_slots", "launch_gemv_w4a8_sample_candidates", "launch_sample_finish", "launch_gemv_w4a8_sample_one_launch", "gemv_w4a8_sample_candidates_peers", "gemv_w4a8_sample_candidates_signal", "sample_finish_after_signals", "gemv_w4a8_peers_signal", "gather_after_signals", "launch_gemv_w4a8_sample_and_advance", "SWEEP_SEPARATE", "SWEEP_FUSE_ALL", "SWEEP_PERSISTENT", "SWEEP_QUANT_IN_GATE_UP", "SWEEP_PUBLISH_SUMSQ", "SWEEP_PUBLISH_AMAX", "SWEEP_DEFAULT", "gemv_w4a16_static_scratch", "debug_counter",
+    "KV4Cache", "KV4Batch", "kv4_append", "kv4_read", "attention_kv4", "attention_kv4_workspace_bytes", "kv4_add_key_weights", "kv4_evict",
 ]
 
 # Qwen2.5-1.5B defaults of the reference's launchers (include/config.cuh:10-22)
@@ -58,6 +59,7 @@ _NATIVE = (
     "launch_gemv_rmsnorm_w4a16", "launch_gemv_qkv_rmsnorm_w4a16", "launch_gemv_dual_gate_up_swiglu_rmsnorm_w4a16",
     "launch_gemv_dual_gate_up_swiglu_rmsnorm_w4a16_q8_1", "launch_gemm_prefill_w4a16",
     "launch_gemm_prefill_qkv_w4a16", "launch_gemm_prefill_dual_gate_up_swiglu_w4a16", "gemv_group_dots",
+    "kv4_append", "kv4_read", "attention_kv4", "kv4_add_key_weights", "kv4_evict",
 )
 
 
@@ -100,6 +102,59 @@ class QKVProjectionView:
     def pod(self) -> QKVView:
         """The C struct, for hosts that call the C functions through load()."""
         return QKVView(*[_ptr(getattr(self, n)) for n, _ in QKVView._fields_])
+
+
+@dataclass
+class KV4Cache:
+    """A layer's 4-bit key/value pool (w4a16_kv4_cache): int32 [num_pages][num_kv_heads][34 * page_size], and the attention
+    weight of its positions, fp32 [num_pages][num_kv_heads][page_size] or None where nothing is evicted."""
+    pages: torch.Tensor
+    key_weight: torch.Tensor | None
+    num_pages: int
+    num_kv_heads: int
+    page_size: int
+
+    @classmethod
+    def allocate(cls, num_pages: int, page_size: int = 16, num_kv_heads: int = NUM_KV_HEADS, key_weight: bool = False, device="cuda"):
+        nbytes = load().w4a16_kv4_page_bytes(page_size, num_kv_heads)
+        if nbytes < 0:
+            check("w4a16_kv4_page_bytes", int(nbytes))
+        pages = torch.zeros(num_pages, num_kv_heads, nbytes // (4 * num_kv_heads), dtype=torch.int32, device=device)
+        weight = torch.zeros(num_pages, num_kv_heads, page_size, device=device) if key_weight else None
+        return cls(pages, weight, num_pages, num_kv_heads, page_size)
+
+
+@dataclass
+class KV4Batch:
+    """The sequences of a call on a KV4Cache (w4a16_kv4_batch): int32 tensors on the device; query_start None is one new
+    token a sequence."""
+    block_table: torch.Tensor
+    seq_lens: torch.Tensor
+    query_start: torch.Tensor | None
+    num_seqs: int
+    max_pages_per_seq: int
+    num_tokens: int
+
+    @classmethod
+    def of(cls, block_table: torch.Tensor, seq_lens: torch.Tensor, query_start: torch.Tensor | None = None, num_tokens: int | None = None):
+        """Sizes taken from the tensors; num_tokens (the rows of q) has to be given with query_start."""
+        for name, t in (("block_table", block_table), ("seq_lens", seq_lens), ("query_start", query_start)):
+            if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+                raise ValueError(f"{name}: a contiguous int32 tensor expected")
+        seqs, pages = block_table.shape
+        if seq_lens.numel() != seqs or (query_start is not None and query_start.numel() != seqs + 1):
+            raise ValueError("block_table, seq_lens and query_start disagree on the number of sequences")
+        if query_start is not None and num_tokens is None:
+            raise ValueError("num_tokens has to be given with query_start")
+        return cls(block_table, seq_lens, query_start, seqs, pages, seqs if num_tokens is None else num_tokens)
+
+
+def attention_kv4_workspace_bytes(num_tokens: int, num_seqs: int, num_q_heads: int = NUM_Q_HEADS, num_kv_heads: int = NUM_KV_HEADS) -> int:
+    """Bytes of device memory that attention_kv4 wants as `workspace` for a batch of that size."""
+    n = load().w4a16_attention_kv4_workspace_bytes(num_tokens, num_seqs, num_q_heads, num_kv_heads)
+    if n < 0:
+        check("w4a16_attention_kv4_workspace_bytes", int(n))
+    return int(n)
 
 
 def debug_counter(which: int = 0) -> int:

@@ -1,0 +1,407 @@
+"""The 4-bit key/value cache against its restatement in 64 bits (tests/kv4_reference.py): append, read, attention, attention
+weights, eviction, and a run of them between the QKV and the O projection."""
+import math
+
+import numpy as np
+import pytest
+
+from tests import kv4_reference as ref
+from tests import util
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+SCALE = 1 / math.sqrt(128)
+BF = np.float16
+
+
+@pytest.fixture(scope="module")
+def ops():
+    import qwen_engine_b200 as q
+    q.init()
+    return q
+
+
+def i32(a):
+    return torch.tensor(np.asarray(a, dtype=np.int32), device="cuda")
+
+
+def make(ops, seed, lens, new, kv, page, extra_pages=3, seqs_pages=None, fill=0x7FFF7FFF, bad=()):
+    """A pool whose unused positions hold NaN, its twin on the device, and the batch.  bad: (sequence, page of it, number)."""
+    rng = np.random.default_rng(seed)
+    per = max(1, seqs_pages or -(-max(max(lens), 1) // page))
+    n = len(lens) * per + extra_pages
+    pool = ref.Pool(n, kv, page).fill_random(rng, 1.5, 0.7)
+    table = rng.permutation(n)[:len(lens) * per].reshape(len(lens), per).astype(np.int32)
+    for b, p, number in bad:
+        table[b, p] = number
+    used = np.zeros((n, page), bool)
+    for b, L in enumerate(lens):
+        for j in range(min(L, per * page)):
+            if 0 <= table[b, j // page] < n:
+                used[table[b, j // page], j % page] = True
+    for p, s in zip(*np.nonzero(~used)):
+        pool.words[p, :, 32 * page + s] = fill
+        pool.words[p, :, 33 * page + s] = fill
+    pool.weight[:] = rng.random(pool.weight.shape, dtype=np.float32)
+    start = np.concatenate([[0], np.cumsum(new)])
+    one = all(x == 1 for x in new)
+    cache = ops.KV4Cache(util.to_dev(pool.words), util.to_dev(pool.weight), n, kv, page)
+    batch = ops.KV4Batch.of(i32(table), i32(lens), None if one else i32(start), num_tokens=int(start[-1]))
+    return rng, pool, table, cache, batch
+
+
+def words_of(cache):
+    return util.to_np(cache.pages, np.uint32)
+
+
+# ---- append and read -----------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("lens,new,kv,heads,page", [
+    ([1], [1], 2, 12, 16), ([1000], [1], 2, 12, 16), ([17, 1, 33, 16], [1, 1, 1, 1], 8, 32, 16),
+    ([40, 5, 0, 70], [20, 5, 0, 1], 3, 9, 32), ([129], [129], 1, 1, 64), ([5] * 70, [1] * 70, 2, 2, 16), ([300, 200], [7, 190], 8, 8, 128)])
+def test_append_stores_the_formula_bit_for_bit(ops, lens, new, kv, heads, page):
+    """Without rotation and bias the rows are the inputs', so codes, scales and zeros are those of the formula, whole."""
+    rng, pool, table, cache, batch = make(ops, 1, lens, new, kv, page)
+    T = sum(new)
+    k, v = (rng.standard_normal((T, kv, 128)).astype(BF) for _ in range(2))
+    k[0, 0] = 0.25                                   # a row of one value: scale 0
+    v[0, 0] = np.linspace(-3e-7, 3e-7, 128)          # a scale below fp16's normal numbers
+    v[-1, -1] = np.where(np.arange(128) % 2, 65504, -65504)
+    want = pool.words.copy()
+    for b, first, L, n in ref.spans(lens, new):
+        for i in range(n):
+            at = L - n + i
+            for h in range(kv):
+                for part, x in enumerate((k, v)):
+                    w, s, z = ref.quantise(x[first + i, h])
+                    pool.put(table[b, at // page], h, at % page, part, w, s, z)
+                pool.weight[table[b, at // page], h, at % page] = 0
+    q = rng.standard_normal((T, heads * 128)).astype(BF)
+    q_out = torch.full((T, heads * 128), 7.0, dtype=torch.float16, device="cuda")
+    ops.kv4_append(cache, batch, util.to_dev(q), util.to_dev(k), util.to_dev(v), None, None, None, None, None, q_out, heads)
+    assert np.array_equal(words_of(cache), pool.words) and (T == 0 or not np.array_equal(want, pool.words))
+    assert np.array_equal(util.to_np(cache.key_weight), pool.weight)
+    assert np.array_equal(util.to_np(q_out), q)
+    kr, vr = (torch.full((T + 1, kv, 128), 7.0, dtype=torch.float16, device="cuda") for _ in range(2))
+    ops.kv4_read(cache, batch, kr, vr)
+    for part, got in enumerate((kr, vr)):
+        got = util.to_np(got)
+        assert (got[T] == 7).all()
+        for b, first, L, n in ref.spans(lens, new):
+            for i in range(n):
+                at = L - n + i
+                for h in range(kv):
+                    exact = pool.row(table[b, at // page], h, at % page, part)
+                    # product exact in 32 bits, one rounding of the sum and one to fp16 (a subnormal's half step besides)
+                    assert np.all(np.abs(got[first + i, h] - exact) <= np.abs(exact) * (2.0 ** -11 + 2.0 ** -23) + 2.0 ** -25), (part, first + i, h)
+
+
+@pytest.mark.parametrize("theta,past", [(1e4, 0), (1e6, 0), (1e6, 130000)])
+@pytest.mark.parametrize("strided", [False, True])
+def test_append_rotates_and_adds_biases(ops, theta, past, strided):
+    lens, new, kv, heads, page = [30, 9], [30, 4], 2, 6, 16
+    rng, pool, table, cache, batch = make(ops, 2, lens, new, kv, page)
+    T, inv = sum(new), (theta ** (-np.arange(64) / 64)).astype(np.float32)
+    pos = np.concatenate([np.arange(L - n, L) for _, _, L, n in ref.spans(lens, new)]) + past
+    qs, ks = heads * 128 + (64 if strided else 0), kv * 128 + (24 if strided else 0)
+    q, k, v = (rng.standard_normal((T, s)).astype(BF) for s in (qs, ks, ks))
+    bias = [(0.5 * rng.standard_normal(n * 128)).astype(BF) for n in (heads, kv, kv)]
+    q_out = torch.full((T, qs), 7.0, dtype=torch.float16, device="cuda")
+    ops.kv4_append(cache, batch, *map(util.to_dev, (q, k, v)), *map(util.to_dev, bias), i32(pos) if past else None, util.to_dev(inv), q_out, heads,
+                   qs if strided else 0, ks if strided else 0)
+    kr, vr = (torch.empty(T, kv, 128, dtype=torch.float16, device="cuda") for _ in range(2))
+    ops.kv4_read(cache, batch, kr, vr)
+
+    def row(x, b, n):
+        return (x[:, :n * 128].astype(np.float64) + b.astype(np.float64)).reshape(T, n, 128)
+
+    want = ref.rotate(row(q, bias[0], heads), pos, inv)
+    got = util.to_np(q_out)
+    size = np.abs(row(q, bias[0], heads))
+    size = np.concatenate([size[..., :64] + size[..., 64:]] * 2, -1)
+    # one rounding to fp16; the angle's turn as fp32 (2^-25 of a turn), sine and cosine and three fp32 roundings before it
+    room = size * (2 * math.pi * 2.0 ** -24 + 6 * 2.0 ** -24)
+    assert np.all(np.abs(got[:, :heads * 128].reshape(T, heads, 128) - want) <= np.abs(want) * 2.0 ** -11 + room + 2.0 ** -24)
+    assert (got[:, heads * 128:] == 7).all()
+    for got, want in ((kr, ref.rotate(row(k, bias[1], kv), pos, inv)), (vr, row(v, bias[2], kv))):
+        got = util.to_np(got).astype(np.float64)
+        step = (want.max(-1, keepdims=True) - want.min(-1, keepdims=True)) / 15
+        big = np.abs(want).max(-1, keepdims=True)
+        # half a step, the scale's rounding 7.5 steps from the zero, and the zero's, the row's and the output's roundings
+        assert np.all(np.abs(got - want) <= step * (0.5 + 8 * 2.0 ** -11) + 3 * big * 2.0 ** -11 + 1e-6)
+
+
+def test_append_leaves_alone_what_it_may_not_touch(ops):
+    """Rows behind the last sequence, positions past the table, page numbers outside the pool, a row with an infinity."""
+    lens, new, kv, heads, page = [20, 40, 34], [4, 8, 2], 2, 2, 16
+    rng, pool, table, cache, batch = make(ops, 3, lens, new, kv, page, seqs_pages=2, bad=[(2, 1, 10 ** 6), (0, 0, -5)])
+    T = sum(new) + 3
+    batch.num_tokens = T
+    k, v = (rng.standard_normal((T, kv, 128)).astype(BF) for _ in range(2))
+    k[1, 1, 5], v[2, 0, 127] = np.inf, np.nan
+    q = rng.standard_normal((T, heads * 128)).astype(BF)
+    q_out = torch.full((T, heads * 128), 7.0, dtype=torch.float16, device="cuda")
+    for b, first, L, n in ref.spans(lens, new):
+        for i in range(n):
+            at = L - n + i
+            if at < 2 * page and 0 <= table[b, at // page] < pool.num_pages:
+                for h in range(kv):
+                    for part, x in enumerate((k, v)):
+                        w, s, z = ref.quantise(x[first + i, h])
+                        pool.put(table[b, at // page], h, at % page, part, w, s, z)
+                    pool.weight[table[b, at // page], h, at % page] = 0
+    ops.kv4_append(cache, batch, util.to_dev(q), util.to_dev(k), util.to_dev(v), None, None, None, None, None, q_out, heads)
+    got = words_of(cache).copy()
+    ps = page
+    for a in (got, pool.words):     # NaNs of any payload are the same
+        p = a[..., 32 * ps:].view(np.uint16)
+        p[(p & 0x7FFF) > 0x7C00] = 0x7E00
+    assert np.array_equal(got, pool.words)
+    assert np.array_equal(util.to_np(cache.key_weight), pool.weight)
+    assert (util.to_np(q_out)[sum(new):] == 7).all() and np.array_equal(util.to_np(q_out)[:sum(new)], q[:sum(new)])
+    kr = torch.full((T, kv, 128), 7.0, dtype=torch.float16, device="cuda")
+    ops.kv4_read(cache, batch, kr, None)
+    kr = util.to_np(kr)
+    assert np.isnan(kr[1, 1]).all() and np.isfinite(kr[1, 0]).all()
+    assert (kr[sum(new):] == 7).all()
+    assert (kr[4:12][[i for i in range(8) if 40 - 8 + i >= 32]] == 0).all() and (kr[12:14] == 0).all()
+
+
+# ---- attention -----------------------------------------------------------------------------------------------------------
+
+
+def attend(ops, cache, batch, q, heads, f32, scale=SCALE, q_stride=0, lse=True):
+    T = batch.num_tokens
+    out = torch.full((T + 1, heads, 128), 7.0, dtype=torch.float32 if f32 else torch.float16, device="cuda")
+    l = torch.full((T + 1, heads), 7.0, device="cuda") if lse else None
+    n = ops.attention_kv4_workspace_bytes(T, batch.num_seqs, heads, cache.num_kv_heads)
+    ws = torch.full((n,), 0xFF, dtype=torch.uint8, device="cuda") if n else None       # NaNs: nothing in it may be read unwritten
+    ops.attention_kv4(cache, batch, q, out, l, ws, heads, n, f32, scale, q_stride)
+    return util.to_np(out), util.to_np(l) if lse else None
+
+
+SHAPES = [
+    ([1], [1], 2, 12, 16), ([16], [1], 2, 12, 16), ([17], [1], 1, 1, 16), ([1021], [1], 2, 12, 16), ([2500], [1], 2, 14, 64),
+    ([5, 0, 33, 64, 65, 127], [1] * 6, 2, 2, 32), ([100] * 40, [1] * 40, 8, 32, 16), ([200, 77], [1, 1], 1, 20, 16),
+    ([30, 12, 9, 0], [5, 1, 0, 0], 4, 28, 16), ([300], [3], 1, 16, 128), ([65, 64, 63], [65, 1, 30], 2, 4, 16), ([7], [20], 2, 4, 16),
+    ([190, 250], [130, 250], 1, 3, 64),
+]
+
+
+def check_attention(got, lse, want, T, f32):
+    out, wl, eout, el = want
+    room = eout if f32 else eout + np.abs(out) * 2.0 ** -11 + 2.0 ** -25
+    off = np.abs(got[:T] - out)
+    assert np.all(off <= room), (off.max(), (off / np.maximum(room, 1e-30)).max())
+    assert (got[T] == 7).all()
+    if lse is not None:
+        empty = np.isneginf(wl)
+        assert np.array_equal(np.isneginf(lse[:T]), empty) and (lse[T] == 7).all()
+        assert np.all(np.abs(lse[:T] - wl)[~empty] <= el[~empty])
+
+
+@pytest.mark.parametrize("f32", [True, False])
+@pytest.mark.parametrize("lens,new,kv,heads,page", SHAPES)
+def test_attention(ops, lens, new, kv, heads, page, f32):
+    rng, pool, table, cache, batch = make(ops, 4, lens, new, kv, page)
+    q = (1.2 * rng.standard_normal((batch.num_tokens, heads, 128))).astype(BF)
+    got, lse = attend(ops, cache, batch, util.to_dev(q), heads, f32)
+    check_attention(got, lse, ref.attention(pool, table, lens, new, q, SCALE), batch.num_tokens, f32)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [4, 2, 40]])
+def test_attention_does_not_see_what_it_may_not(ops, new):
+    """Page numbers outside the pool, positions past the table; tokens behind the last sequence stay; strided q; no lse."""
+    lens, kv, heads, page = [60, 50, 70], 2, 6, 16
+    rng, pool, table, cache, batch = make(ops, 5, lens, new, kv, page, seqs_pages=4, bad=[(0, 1, -1), (1, 3, 1 << 30), (2, 0, 10 ** 5)])
+    T = sum(new)
+    q = np.full((T, heads * 128 + 8), np.nan, BF)
+    q[:, :heads * 128] = (1.2 * rng.standard_normal((T, heads * 128))).astype(BF)
+    got, lse = attend(ops, cache, batch, util.to_dev(q), heads, True, lse=False, q_stride=heads * 128 + 8)
+    check_attention(got, lse, ref.attention(pool, table, lens, new, q[:, :heads * 128].reshape(T, heads, 128), SCALE), T, True)
+
+
+@pytest.mark.parametrize("heads", [4, 40])
+def test_a_poisoned_row_reaches_the_tokens_that_see_it_only(ops, heads):
+    lens, new, kv, page = [50], [20], 1, 16
+    rng, pool, table, cache, batch = make(ops, 6, lens, new, kv, page)
+    q = rng.standard_normal((20, heads, 128)).astype(BF)
+    for part in range(2):
+        clean = cache.pages.clone()
+        slot = 40 % page
+        cache.pages[int(table[0, 40 // page]), 0, (32 + part) * page + slot] = 0x7E007E00
+        got, lse = attend(ops, cache, batch, util.to_dev(q), heads, True)
+        want = ref.attention(pool, table, lens, new, q, SCALE)
+        # token i is position 30 + i: those from 10 on see position 40
+        assert np.isnan(got[10:20]).all()
+        assert np.all(np.abs(got[:10] - want[0][:10]) <= want[2][:10])
+        cache.pages.copy_(clean)
+
+
+@pytest.mark.parametrize("factor", [1e-3, 1.0, 3e3])
+def test_attention_of_values_of_any_size(ops, factor):
+    """Value scales from 2^-14 to above 2^10, and a few rows that are larger by a thousand: the weights' power of two follows."""
+    lens, new, kv, heads, page = [700], [1], 1, 4, 16
+    rng, pool, table, cache, batch = make(ops, 7, lens, new, kv, page)
+    for page_no in table[0]:
+        for s in range(page):
+            x = (rng.standard_normal(128) * factor * (1.0 if rng.random() < 0.95 else 5.0 if factor > 1 else 1000.0)).astype(BF)
+            pool.put(page_no, 0, s, 1, *ref.quantise(x))
+    cache.pages.copy_(util.to_dev(pool.words))
+    q = rng.standard_normal((1, heads, 128)).astype(BF)
+    got, lse = attend(ops, cache, batch, util.to_dev(q), heads, True)
+    check_attention(got, lse, ref.attention(pool, table, lens, new, q, SCALE), 1, True)
+
+
+def test_attention_with_steep_scores(ops):
+    """Scores in the hundreds, rising along the sequence, so that the running maximum keeps moving."""
+    lens, new, kv, heads, page = [600], [2], 1, 4, 32
+    rng, pool, table, cache, batch = make(ops, 8, lens, new, kv, page)
+    direction = rng.standard_normal(128)
+    for j in range(600):
+        x = (direction * (j / 60) + 0.1 * rng.standard_normal(128)).astype(BF)
+        pool.put(table[0, j // page], 0, j % page, 0, *ref.quantise(x))
+    cache.pages.copy_(util.to_dev(pool.words))
+    q = (direction * np.array([1, -1, 3, -3])[:, None] + np.zeros((2, 4, 128))).astype(BF)
+    got, lse = attend(ops, cache, batch, util.to_dev(q), heads, True)
+    check_attention(got, lse, ref.attention(pool, table, lens, new, q, SCALE), 2, True)
+
+
+# ---- weights and eviction ----------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("lens,new,kv,heads,page", SHAPES)
+def test_key_weights(ops, lens, new, kv, heads, page):
+    rng, pool, table, cache, batch = make(ops, 9, lens, new, kv, page)
+    q = (1.2 * rng.standard_normal((batch.num_tokens, heads, 128))).astype(BF)
+    lse = ref.attention(pool, table, lens, new, q, SCALE)[1].astype(np.float32)
+    add, rel = ref.key_weights(pool, table, lens, new, q, lse.astype(np.float64), SCALE)
+    for turn in range(2):
+        ops.kv4_add_key_weights(cache, batch, util.to_dev(q), util.to_dev(lse), heads, SCALE)
+        want = pool.weight + (turn + 1) * add
+        got = util.to_np(cache.key_weight)
+        assert np.all(np.abs(got - want) <= add * 2 * rel + np.abs(want) * 2.0 ** -22), turn
+        assert np.array_equal(got[add == 0], pool.weight[add == 0])
+
+
+@pytest.mark.parametrize("lens,kv,page,budget,sink,recent", [
+    ([100], 2, 16, 33, 4, 8), ([5, 0, 64, 65, 200], 1, 16, 64, 0, 0), ([1100], 2, 16, 512, 4, 64), ([3000, 2999], 3, 64, 1, 0, 1),
+    ([4000], 1, 128, 3999, 2, 5), ([50], 2, 16, 20, 10, 10), ([9000], 1, 32, 700, 4, 256), ([40000], 2, 64, 5000, 4, 256)])
+@pytest.mark.parametrize("kind", ["random", "equal", "odd"])
+def test_eviction(ops, lens, kv, page, budget, sink, recent, kind):
+    bad = [(0, 1, -3)] if kind == "odd" and max(lens) > page else []
+    rng, pool, table, cache, batch = make(ops, 10, lens, [1] * len(lens), kv, page, fill=0x3C003C00, bad=bad)
+    if kind == "equal":
+        pool.weight[:] = np.round(pool.weight * 3) / 3
+    elif kind == "odd":
+        pool.weight[:] = np.exp(8 * rng.standard_normal(pool.weight.shape)) * rng.choice([1, -1, 0, -0.0], pool.weight.shape)
+        pool.weight[rng.random(pool.weight.shape) < 0.1] = np.nan
+        pool.weight[rng.random(pool.weight.shape) < 0.05] = np.inf
+    cache.key_weight.copy_(util.to_dev(pool.weight))
+    B, per = len(lens), -(-budget // page)
+    n = pool.num_pages
+    cache = ops.KV4Cache(torch.cat([cache.pages, torch.full_like(cache.pages[:1], 9).expand(B * per, -1, -1)]),
+                         torch.cat([cache.key_weight, torch.full((B * per, kv, page), 9.0, device="cuda")]), n + B * per, kv, page)
+    dst = n + rng.permutation(B * per).reshape(B, per)
+    new_lens, kept = i32(np.full(B, 77)), i32(np.full((B, kv, budget), 77))
+    ops.kv4_evict(cache, batch, i32(dst), new_lens, kept, per, budget, sink, recent)
+    words, weight, kept = words_of(cache), util.to_np(cache.key_weight), util.to_np(kept)
+    assert np.array_equal(words[:n], pool.words) and np.array_equal(weight[:n], pool.weight, equal_nan=True)
+    assert util.to_np(new_lens).tolist() == [min(L, budget) for L in lens]
+    for b, L in enumerate(lens):
+        for h in range(kv):
+            want = ref.evict(pool.weight, table[b], L, h, page, n, budget, sink, recent)
+            assert kept[b, h].tolist() == want + [-1] * (budget - len(want)), (b, h)
+            for j in range(per * page):
+                rec, slot = words[dst[b, j // page], h], j % page
+                old = want[j] if j < len(want) else None
+                page_no = table[b, old // page] if old is not None else -1
+                for part in range(2):
+                    mine = np.append(rec[(part * page + slot) * 16:][:16], rec[(32 + part) * page + slot])
+                    if 0 <= page_no < n:
+                        src, s = pool.words[page_no, h], old % page
+                        assert np.array_equal(mine, np.append(src[(part * page + s) * 16:][:16], src[(32 + part) * page + s]))
+                    else:
+                        assert (mine == 9).all()
+                if 0 <= page_no < n:
+                    assert np.array_equal(weight[dst[b, j // page], h, slot], pool.weight[page_no, h, old % page], equal_nan=True)
+                else:
+                    assert weight[dst[b, j // page], h, slot] == 9
+
+
+# ---- as they are used ----------------------------------------------------------------------------------------------------
+
+
+def test_decode_steps_between_qkv_and_o(ops):
+    """QKV projection -> append -> attention (fp32 heads) -> O projection from the heads, captured once and replayed while the
+    sequence grows; then weights, eviction, and attention over what is left."""
+    from qwen_engine_b200 import synth
+    H, heads, kv, page, steps = 1536, 12, 2, 16, 40
+    dev = lambda a: util.to_dev(a)  # noqa: E731
+    W = {n: (dev(synth.packed_weights(1, n, r, H)), dev(synth.scales(1, n, r, H))) for n, r in (("q", H), ("k", 256), ("v", 256), ("o", H))}
+    h = dev(synth.activations(1, "h", H))
+    gamma = torch.full((H,), 0.05, dtype=torch.float16, device="cuda")
+    bufs = {n: torch.empty(r, dtype=torch.float16, device="cuda") for n, r in (("q", H), ("k", 256), ("v", 256), ("o", H))}
+    view = ops.QKVProjectionView(*W["q"], bufs["q"], *W["k"], bufs["k"], *W["v"], bufs["v"])
+    per = 4
+    cache = ops.KV4Cache.allocate(2 * per, page, kv, key_weight=True)
+    table, lens = i32(np.arange(per)[None, ::-1].copy()), i32([0])
+    batch = ops.KV4Batch.of(table, lens)
+    inv = torch.tensor(1e6 ** (-np.arange(64) / 64), dtype=torch.float32, device="cuda")
+    acc, lse = torch.empty(1, heads, 128, device="cuda"), torch.empty(1, heads, device="cuda")
+    n = ops.attention_kv4_workspace_bytes(1, 1, heads, kv)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    out = torch.empty(H, dtype=torch.float16, device="cuda")
+
+    def step():
+        lens.add_(1)
+        ops.launch_gemv_qkv_rmsnorm_w4a16(view, h, gamma, in_features=H, num_q_heads=heads, num_kv_heads=kv)
+        ops.kv4_append(cache, batch, bufs["q"], bufs["k"], bufs["v"], None, None, None, None, inv, bufs["q"], heads)
+        ops.attention_kv4(cache, batch, bufs["q"], acc, lse, ws, heads, n, True, SCALE)
+        ops.gemv_attn_heads_f32_w4a16(*W["o"], acc, h, out, H, H)
+        ops.kv4_add_key_weights(cache, batch, bufs["q"], lse, heads, SCALE)
+        h.copy_(out)
+
+    h0 = h.clone()
+    step()                                       # eager, then captured
+    stream = torch.cuda.Stream()
+    lens.zero_(), h.copy_(h0), cache.pages.zero_(), cache.key_weight.zero_()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    seen = []
+    for _ in range(steps):
+        before = h.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        seen.append((before, bufs["q"].clone(), acc.clone(), out.clone(), lse.clone()))
+    assert lens.item() == steps
+    pool = ref.Pool(2 * per, kv, page)
+    pool.words[:] = words_of(cache)
+    total = np.zeros_like(pool.weight, dtype=np.float64)
+    for i in (0, 1, 15, 16, steps - 1):
+        before, q, heads_acc, o, l = seen[i]
+        qh = util.to_np(q).reshape(1, heads, 128)
+        want = ref.attention(pool, util.to_np(table), [i + 1], [1], qh, SCALE)
+        assert np.all(np.abs(util.to_np(heads_acc) - want[0]) <= want[2])
+        o2 = torch.empty_like(o)
+        ops.gemv_attn_heads_f32_w4a16(*W["o"], heads_acc, before, o2, H, H)
+        assert torch.equal(o, o2)
+    rel = 0.0
+    for i in range(steps):
+        add, r = ref.key_weights(pool, util.to_np(table), [i + 1], [1], util.to_np(seen[i][1]).reshape(1, heads, 128), util.to_np(seen[i][4]).astype(np.float64), SCALE)
+        total += add
+        rel = max(rel, r)
+    got = util.to_np(cache.key_weight)
+    assert np.all(np.abs(got - total) <= total * (2 * rel + steps * 2.0 ** -24))
+    dst, new_lens, kept = i32(np.array([[6, 4]])), i32([0]), i32(np.zeros((1, kv, 20)))
+    ops.kv4_evict(cache, batch, dst, new_lens, kept, 2, 20, 2, 6)
+    after = ops.KV4Batch.of(dst, new_lens)
+    ops.attention_kv4(cache, after, bufs["q"], acc, lse, ws, heads, n, True, SCALE)
+    pool.words[:] = words_of(cache)
+    want = ref.attention(pool, np.array([[6, 4]]), [20], [1], util.to_np(bufs["q"]).reshape(1, heads, 128), SCALE)
+    assert np.all(np.abs(util.to_np(acc) - want[0]) <= want[2])
+    for h_ in range(kv):
+        assert util.to_np(kept)[0, h_].tolist() == ref.evict(got, util.to_np(table)[0], steps, h_, page, 2 * per, 20, 2, 6)

@@ -1,0 +1,128 @@
+"""Refusals of the 4-bit key/value cache's entry points and the sizes they report; nothing is launched."""
+import ctypes
+import random
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from qwen_engine_b200 import build
+    build.build()
+    from qwen_engine_b200 import _lib
+    return _lib.load()
+
+
+P = 4096          # an address that is never followed: argument checks come first
+
+
+def views(**changes):
+    from qwen_engine_b200._lib import KV4BatchView, KV4CacheView
+    c = dict(pages=P, key_weight=P, num_pages=8, num_kv_heads=2, page_size=16)
+    b = dict(block_table=P, seq_lens=P, query_start=P, num_seqs=3, max_pages_per_seq=4, num_tokens=5)
+    for k, v in changes.items():
+        (c if k in c else b)[k] = v
+    return ctypes.byref(KV4CacheView(*c.values())), ctypes.byref(KV4BatchView(*b.values()))
+
+
+def calls(lib, **changes):
+    """Every entry point with good arguments but for `changes`; their statuses."""
+    c, b = views(**{k: v for k, v in changes.items() if k in (
+        "pages", "key_weight", "num_pages", "num_kv_heads", "page_size", "block_table", "seq_lens", "query_start", "num_seqs", "max_pages_per_seq", "num_tokens")})
+    a = dict(q=P, k=P, v=P, q_bias=None, k_bias=None, v_bias=None, positions=None, inv=None, q_out=P, heads=12, q_stride=0, kv_stride=0, out=P, lse=P, ws=P,
+             ws_bytes=1 << 40, f32=0, scale=0.088, dst=2 * P, new_lens=P, kept=P, dst_pages=2, budget=32, sink=4, recent=8)
+    a.update({k: v for k, v in changes.items() if k in a})
+    return {
+        "append": lib.w4a16_kv4_append(c, b, a["q"], a["k"], a["v"], a["q_bias"], a["k_bias"], a["v_bias"], a["positions"], a["inv"], a["q_out"], a["heads"],
+                                       a["q_stride"], a["kv_stride"], None),
+        "read": lib.w4a16_kv4_read(c, b, a["k"], a["v"], None),
+        "attention": lib.w4a16_attention_kv4(c, b, a["q"], a["out"], a["lse"], a["ws"], a["heads"], a["ws_bytes"], a["f32"], a["scale"], a["q_stride"], None),
+        "weights": lib.w4a16_kv4_add_key_weights(c, b, a["q"], a["lse"], a["heads"], a["scale"], a["q_stride"], None),
+        "evict": lib.w4a16_kv4_evict(c, b, a["dst"], a["new_lens"], a["kept"], a["dst_pages"], a["budget"], a["sink"], a["recent"], None),
+    }
+
+
+ALL = {"append", "read", "attention", "weights", "evict"}
+REFUSED = [
+    (dict(pages=None), -1, ALL), (dict(block_table=None), -1, ALL), (dict(seq_lens=None), -1, ALL), (dict(num_pages=0), -1, ALL),
+    (dict(num_kv_heads=0), -1, ALL), (dict(num_seqs=0), -1, ALL), (dict(max_pages_per_seq=0), -1, ALL), (dict(num_tokens=0), -1, ALL),
+    (dict(query_start=None), -1, ALL), (dict(page_size=8), -2, ALL), (dict(page_size=48), -2, ALL), (dict(page_size=8192), -2, ALL),
+    (dict(pages=P + 8), -3, ALL), (dict(seq_lens=P + 2), -3, ALL), (dict(num_seqs=70000), -5, ALL), (dict(num_tokens=1 << 25), -5, ALL),
+    (dict(k=None), -1, {"append"}), (dict(v=None), -1, {"append"}), (dict(q_out=None), -1, {"append"}), (dict(q=None), -1, {"append", "attention", "weights"}),
+    (dict(q=None, q_out=None, q_bias=P), -1, {"append"}), (dict(k=None, v=None), -1, {"append", "read"}),
+    (dict(heads=0), -1, {"append", "attention", "weights"}), (dict(heads=11), -2, {"append", "attention", "weights"}),
+    (dict(q_stride=-8), -1, {"append", "attention", "weights"}), (dict(q_stride=1528), -2, {"append", "attention", "weights"}),
+    (dict(q_stride=1540), -3, {"append", "attention", "weights"}), (dict(kv_stride=248), -2, {"append"}), (dict(q=P + 8), -3, {"append", "attention", "weights"}),
+    (dict(k=P + 2), -3, {"append", "read"}), (dict(heads=1 << 12, num_tokens=1 << 20), -5, {"append", "attention", "weights"}),
+    (dict(out=None), -1, {"attention"}), (dict(scale=0.0), -1, {"attention", "weights"}), (dict(scale=float("nan")), -1, {"attention", "weights"}),
+    (dict(scale=float("inf")), -1, {"attention", "weights"}), (dict(ws=None), -1, {"attention"}), (dict(ws_bytes=16), -1, {"attention"}),
+    (dict(ws=P + 8), -3, {"attention"}), (dict(lse=None), -1, {"weights"}), (dict(key_weight=None), -1, {"weights", "evict"}),
+    (dict(dst=None), -1, {"evict"}), (dict(dst=P), -1, {"evict"}), (dict(kept=None), -1, {"evict"}), (dict(new_lens=None), -1, {"evict"}),
+    (dict(budget=0), -1, {"evict"}), (dict(sink=-1), -1, {"evict"}), (dict(sink=30), -2, {"evict"}), (dict(budget=33), -2, {"evict"}),
+    (dict(sink=2147483647, recent=2147483647), -2, {"evict"}),
+]
+
+
+@pytest.mark.parametrize("changes,status,where", REFUSED, ids=[str(sorted(r[0].items())) for r in REFUSED])
+def test_refusals(lib, changes, status, where):
+    got = calls(lib, **changes)
+    assert {n for n in where if got[n] == status} == where, got
+    if not torch.cuda.is_available():      # what is not refused gets as far as asking for a device
+        assert all(s > 0 or s == -4 for n, s in got.items() if n not in where), got
+
+
+def test_null_views_are_refused(lib):
+    c, b = views()
+    assert lib.w4a16_kv4_read(None, b, P, P, None) == -1 and lib.w4a16_kv4_read(c, None, P, P, None) == -1
+
+
+def test_workspace_sizes(lib):
+    f = lib.w4a16_attention_kv4_workspace_bytes
+    assert f(0, 1, 12, 2) == -1 and f(1, 1, 12, 5) == -2 and f(1 << 25, 1, 12, 2) == -5 and f(1 << 20, 1, 1 << 12, 2) == -5
+    rng = random.Random(1)
+    for _ in range(500):
+        kv = rng.randint(1, 16)
+        heads, seqs = kv * rng.randint(1, 16), rng.randint(1, 300)
+        n = f(rng.randint(1, 5000), seqs, heads, kv)
+        assert 0 <= n < 1 << 31 and n % 8 == 0
+    assert lib.w4a16_kv4_page_bytes(16, 2) == 16 * 2 * 136 and lib.w4a16_kv4_page_bytes(24, 2) == -2 and lib.w4a16_kv4_page_bytes(16, 0) == -1
+
+
+def test_the_batch_takes_its_sizes_from_the_tensors():
+    from qwen_engine_b200 import KV4Batch
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    b = KV4Batch.of(i32(3, 5), i32(3))
+    assert (b.num_seqs, b.max_pages_per_seq, b.num_tokens, b.query_start) == (3, 5, 3, None)
+    assert KV4Batch.of(i32(3, 5), i32(3), i32(4), num_tokens=17).num_tokens == 17
+    for bad in (lambda: KV4Batch.of(i32(3, 5), i32(2)), lambda: KV4Batch.of(i32(3, 5), i32(3), i32(3), 9), lambda: KV4Batch.of(i32(3, 5), i32(3), i32(4)),
+                lambda: KV4Batch.of(i32(3, 5).long(), i32(3)), lambda: KV4Batch.of(i32(5, 3).t(), i32(3))):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_arguments_of_the_python_functions(lib):
+    from types import SimpleNamespace
+
+    from qwen_engine_b200 import _lib, ops
+
+    class Device:
+        is_cuda = True
+
+        def data_ptr(self):
+            return P
+
+    d = Device()
+    cache = SimpleNamespace(pages=d, key_weight=d, num_pages=8, num_kv_heads=2, page_size=24)
+    batch = SimpleNamespace(block_table=d, seq_lens=d, query_start=None, num_seqs=3, max_pages_per_seq=4, num_tokens=3)
+    with pytest.raises(_lib.W4A16Error) as e:
+        ops.attention_kv4(cache, batch, d, d, None, None, 12, 0, True, 0.1, stream=0)
+    assert e.value.status == -2 and "w4a16_attention_kv4" in str(e.value)
+    with pytest.raises(TypeError):
+        ops.attention_kv4(cache, batch, d, d, None, None, 12, 0, True, "0.1", stream=0)
+    with pytest.raises(AttributeError):
+        ops.kv4_read(SimpleNamespace(pages=d), batch, d, d, stream=0)
+    with pytest.raises(ValueError):
+        ops.kv4_read(SimpleNamespace(pages=torch.zeros(1), key_weight=None, num_pages=8, num_kv_heads=2, page_size=16), batch, d, d, stream=0)
+    with pytest.raises(OverflowError):
+        ops.attention_kv4(cache, batch, d, d, None, None, 12, 1 << 70, True, 0.1, stream=0)
