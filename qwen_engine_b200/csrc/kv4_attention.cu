@@ -36,63 +36,87 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Query rows of a tile and the positions they see.
-struct QTile {
-    int seq, first_token, n;      // the sequence, its first row in the batch, its new tokens
-    int row0, rows;               // rows of (token, query head of the group) in the sequence, token major
-    int past;                     // positions in front of the first new token (negative where the batch has more tokens than positions)
-    int seen;                     // positions that the tile's last row sees
-};
+// How the work is cut.  A unit is 64 positions (16 a warp) against one tile of query rows and one head; units are numbered by
+// sequence, tile, head, position, and every CTA of a persistent grid takes the same number of consecutive ones.  So the CTAs
+// finish together whatever the lengths are (they live on the device, the host does not know them), and a CTA has at most two
+// parts of a (tile, head) that others have parts of too: its first and its last one.
+constexpr int kUnit = kKvTile * kAttnWarps;
 
-// The tile with number `index`, in order of the sequences; false past the last one.  A whole warp calls it.
-__device__ __forceinline__ bool find_qtile(const Kv4View& c, int group, int tile_rows, int index, QTile* out) {
-    const int lane = threadIdx.x & 31;
-    int b = -1, t = 0;
-    if (c.qstart == nullptr) {
-        const int per = (group + tile_rows - 1) / tile_rows;
-        b = index / per;
-        t = index - b * per;
-        if (b >= c.num_seqs) return false;
-    } else {
-        int before = 0;
-        for (int b0 = 0; b0 < c.num_seqs; b0 += 32) {
-            int mine = 0;
-            if (b0 + lane < c.num_seqs) mine = (kv4_new_tokens(c, b0 + lane).y * group + tile_rows - 1) / tile_rows;
-            int upto = mine;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-                if (lane >= d) upto += o;
-            }
-            const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + upto > index);
-            if (past != 0) {
-                const int l = __ffs(past) - 1;
-                b = b0 + l;
-                t = index - before - __shfl_sync(0xFFFFFFFFu, upto - mine, l);
-                break;
-            }
-            before += __shfl_sync(0xFFFFFFFFu, upto, 31);
-        }
-        if (b < 0) return false;
-    }
+struct SeqWork {
+    int first, n;                 // rows of the batch
+    int past;                     // positions in front of the first new token (negative: tokens without a position)
+    int tiles, units;             // tiles of query rows; units of one tile and head
+};
+__device__ __forceinline__ SeqWork seq_work(const Kv4View& c, int b, int group, int tile_rows) {
+    SeqWork w;
     const int2 mine = kv4_new_tokens(c, b);
     const int len = max(__ldcg(c.lens + b), 0);
-    out->seq = b;
-    out->first_token = mine.x;
-    out->n = mine.y;
-    out->row0 = t * tile_rows;
-    out->rows = min(tile_rows, mine.y * group - out->row0);
-    out->past = len - mine.y;
-    out->seen = min(max(out->past + (out->row0 + out->rows - 1) / group + 1, 0), kv4_capacity(c));
-    return out->rows > 0;
+    w.first = mine.x;
+    w.n = mine.y;
+    w.past = len - mine.y;
+    w.tiles = (mine.y * group + tile_rows - 1) / tile_rows;
+    w.units = max(1, (min(len, kv4_capacity(c)) + kUnit - 1) / kUnit);
+    return w;
+}
+// A place in the order of the units.
+struct Place {
+    SeqWork w;
+    int seq;
+    long long in_seq;             // unit of the sequence
+};
+// Units of the whole batch, and the place of unit `per * index` with per = ceil(all / parts); false where there is none.
+// All threads of the CTA call it; `s_scan` holds a value a thread, and two more.
+template <int THREADS>
+__device__ __forceinline__ bool find_unit(const Kv4View& c, int group, int tile_rows, int index, int parts, long long* s_scan, long long* per, long long* all, Place* out) {
+    const int tid = threadIdx.x, lane = tid & 31, each = (c.num_seqs + THREADS - 1) / THREADS;
+    const int b0 = min(tid * each, c.num_seqs), b1 = min(b0 + each, c.num_seqs);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) {
+        const SeqWork w = seq_work(c, b, group, tile_rows);
+        mine += static_cast<long long>(w.tiles) * c.kv_heads * w.units;
+    }
+    long long upto = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+        if (lane >= d) upto += o;
+    }
+    if (lane == 31) s_scan[tid >> 5] = upto;
+    __syncthreads();
+    long long total = 0, before = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w == tid >> 5) before = total;
+        total += s_scan[w];
+    }
+    *all = total;
+    *per = (total + parts - 1) / parts;
+    const long long want = *per * index;
+    if (want >= total) return false;
+    upto += before;
+    if (upto > want && upto - mine <= want) {        // the sequence is one of this thread's
+        long long at = upto - mine;
+        for (int b = b0; b < b1; ++b) {
+            const SeqWork w = seq_work(c, b, group, tile_rows);
+            const long long units = static_cast<long long>(w.tiles) * c.kv_heads * w.units;
+            if (want < at + units) {
+                s_scan[THREADS / 32] = b;
+                s_scan[THREADS / 32 + 1] = want - at;
+                break;
+            }
+            at += units;
+        }
+    }
+    __syncthreads();
+    out->seq = static_cast<int>(s_scan[THREADS / 32]);
+    out->in_seq = s_scan[THREADS / 32 + 1];
+    out->w = seq_work(c, out->seq, group, tile_rows);
+    return true;
 }
 
-// Positions of one split of `seen`; a multiple of what a CTA takes in one go.
-__device__ __forceinline__ int split_positions(int seen, int splits, int least) {
-    const int n = min(splits, max(1, (seen + least - 1) / least));
-    const int per = (seen + n - 1) / n;
-    constexpr int kStep = kKvTile * kAttnWarps;
-    return max(kStep, (per + kStep - 1) / kStep * kStep);
+// Output row r of a tile.
+__device__ __forceinline__ size_t out_row(const SeqWork& w, int heads, int group, int head, int row) {
+    return static_cast<size_t>(w.first + row / group) * (static_cast<size_t>(heads) * group) + head * group + row % group;
 }
 
 // What a lane holds of 16 positions: rows g and g + 8 of the keys, four positions' share of the values.
@@ -140,28 +164,59 @@ __device__ __forceinline__ float sum_half8(const uint4& w) {
     return s;
 }
 
+// One part's four dimensions, with its maximum and sum, into a sum around `top` (the largest maximum).  A part without any
+// position has maximum -infinity and sum 0; where all parts are such, the factor is 1 and what is added is 0.
+__device__ __forceinline__ void add_part(float4& x, float& sum, const float4& p, float2 ml, float top) {
+    const float f = ml.x == top ? 1.0f : ex2(ml.x - top);
+    sum = fmaf(ml.y, f, sum);
+    x.x = fmaf(p.x, f, x.x);
+    x.y = fmaf(p.y, f, x.y);
+    x.z = fmaf(p.z, f, x.z);
+    x.w = fmaf(p.w, f, x.w);
+}
+// A finished row: a warp, four dimensions a lane.
 template <bool F32>
-__device__ __forceinline__ void store_out(void* out, size_t at, float x) {
-    if constexpr (F32) static_cast<float*>(out)[at] = x;
-    else static_cast<__half*>(out)[at] = __float2half_rn(x);
+__device__ __forceinline__ void store_row(const Kv4AttentionArgs& a, size_t row, const float4& x, float top, float sum) {
+    const int lane = threadIdx.x & 31;
+    const float f = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+    const float4 y = sum == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
+    if constexpr (F32) {
+        reinterpret_cast<float4*>(static_cast<float*>(a.out) + row * kKvDim)[lane] = y;
+    } else {
+        const uint2 h = make_uint2(pack_half2(y.x, y.y), pack_half2(y.z, y.w));
+        reinterpret_cast<uint2*>(static_cast<__half*>(a.out) + row * kKvDim)[lane] = h;
+    }
+    if (lane == 0 && a.lse != nullptr) a.lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
 template <int NT, bool F32>
-__global__ void __launch_bounds__(kAttnThreads) kv4_attention_kernel(const __grid_constant__ Kv4AttentionArgs a) {
+__global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_kernel(const __grid_constant__ Kv4AttentionArgs a) {
     constexpr int R = 8 * NT, kPitch = kKvDim + 4;
     __shared__ float s_o[kAttnWarps][R][kPitch];
     __shared__ float2 s_ml[kAttnWarps][R];
+    __shared__ long long s_scan[kAttnWarps + 2];
     pdl_wait_prior_grids();
     pdl_release_dependents();
     const Kv4View& c = a.c;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int tile_index = blockIdx.x / a.splits, split = blockIdx.x - tile_index * a.splits, head = blockIdx.y;
-    QTile q;
-    if (!find_qtile(c, a.group, R, tile_index, &q)) return;
-    const int per = split_positions(q.seen, a.splits, a.least);
-    const int used = max(1, (q.seen + per - 1) / per);
-    if (split >= used) return;
-    const int k0 = split * per, k1 = min(k0 + per, q.seen);
+    long long per, all;
+    Place pl;
+    if (!find_unit<kAttnThreads>(c, a.group, R, blockIdx.x, gridDim.x, s_scan, &per, &all, &pl)) return;
+    long long left = min(per, all - per * blockIdx.x);
+    for (bool first_part = true; left > 0; first_part = false) {
+    while (pl.in_seq >= static_cast<long long>(pl.w.tiles) * c.kv_heads * pl.w.units) {      // past the sequence: the next one with work
+        pl.w = seq_work(c, ++pl.seq, a.group, R);
+        pl.in_seq = 0;
+    }
+    const int tile_head = static_cast<int>(pl.in_seq / pl.w.units), unit0 = static_cast<int>(pl.in_seq - static_cast<long long>(tile_head) * pl.w.units);
+    const int head = tile_head % c.kv_heads, row0 = tile_head / c.kv_heads * R;
+    const int units = static_cast<int>(min(left, static_cast<long long>(pl.w.units - unit0)));
+    const bool whole = units == pl.w.units;
+    left -= units;
+    pl.in_seq += units;
+    struct { int seq, first_token, row0, rows, past; } q = {pl.seq, pl.w.first, row0, min(R, pl.w.n * a.group - row0), pl.w.past};
+    const int seen = min(max(q.past + (q.row0 + q.rows - 1) / a.group + 1, 0), kv4_capacity(c));
+    const int k0 = unit0 * kUnit, k1 = min(k0 + units * kUnit, seen);
 
     // queries: B fragments of rows g (+ 8), and for the lane's columns 2 t, 2 t + 1 the sum of q and how far the row sees
     uint32_t qb[NT][16];
@@ -197,7 +252,7 @@ __global__ void __launch_bounds__(kAttnThreads) kv4_attention_kernel(const __gri
     for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY;
     float pw = 0.0f;                                        // power of two on the value scales; 0: not chosen yet
 
-    constexpr int kStep = kKvTile * kAttnWarps;
+    constexpr int kStep = kUnit;
     int at = k0 + warp * kKvTile;
     KvRegs cur;
     int next_page = -1;
@@ -225,7 +280,8 @@ __global__ void __launch_bounds__(kAttnThreads) kv4_attention_kernel(const __gri
             }
             const float ks[2] = {kv4_scale(cur.kp[0]) * to_log2, kv4_scale(cur.kp[1]) * to_log2};
             const float kz[2] = {kv4_zero(cur.kp[0]), kv4_zero(cur.kp[1])};
-            float vs[2] = {kv4_scale(cur.vp[0]), kv4_scale(cur.vp[1])}, vz[2] = {kv4_zero(cur.vp[0]), kv4_zero(cur.vp[1])};
+            float vs[2] = {kv4_scale(cur.vp[0]), kv4_scale(cur.vp[1])};
+            float vz[2] = {fmaf(-0.5f, vs[0], kv4_zero(cur.vp[0])), fmaf(-0.5f, vs[1], kv4_zero(cur.vp[1]))};     // codes are taken around 7.5
             const bool cut = at + kKvTile > all_see;        // some row does not see some of these positions
             bool above = false;
 #pragma unroll
@@ -300,10 +356,10 @@ __global__ void __launch_bounds__(kAttnThreads) kv4_attention_kernel(const __gri
             for (int half = 0; half < 2; ++half) {
                 const uint32_t sel = half ? 0x7632u : 0x5410u;
                 uint32_t f[4][4];
-                kv4_codes_to_half2(__byte_perm(cur.v[0].x, cur.v[1].x, sel), f[0]);
-                kv4_codes_to_half2(__byte_perm(cur.v[0].y, cur.v[1].y, sel), f[1]);
-                kv4_codes_to_half2(__byte_perm(cur.v[2].x, cur.v[3].x, sel), f[2]);
-                kv4_codes_to_half2(__byte_perm(cur.v[2].y, cur.v[3].y, sel), f[3]);
+                kv4_value_codes_to_half2(__byte_perm(cur.v[0].x, cur.v[1].x, sel), f[0]);
+                kv4_value_codes_to_half2(__byte_perm(cur.v[0].y, cur.v[1].y, sel), f[1]);
+                kv4_value_codes_to_half2(__byte_perm(cur.v[2].x, cur.v[3].x, sel), f[2]);
+                kv4_value_codes_to_half2(__byte_perm(cur.v[2].y, cur.v[3].y, sel), f[3]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t av[4] = {f[0][i], f[1][i], f[2][i], f[3][i]};
@@ -335,64 +391,98 @@ __global__ void __launch_bounds__(kAttnThreads) kv4_attention_kernel(const __gri
             if (g == 0) s_ml[warp][r] = make_float2(m[n][e], ls);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                s_o[warp][r][16 * g + kElement[i]] = fmaf(o[n][i][e], undo, zs);
-                s_o[warp][r][16 * g + 8 + kElement[i]] = fmaf(o[n][i][e + 2], undo, zs);
+                s_o[warp][r][16 * g + kElement[i]] = fmaf(o[n][i][e], undo * kv4_value_undo(i), zs);
+                s_o[warp][r][16 * g + 8 + kElement[i]] = fmaf(o[n][i][e + 2], undo * kv4_value_undo(i), zs);
             }
         }
     __syncthreads();
-    const size_t part = (static_cast<size_t>(tile_index) * c.kv_heads + head) * a.splits + split;
-    for (int r = 0; r < q.rows; ++r) {
-        float top = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kAttnWarps; ++w) top = fmaxf(top, s_ml[w][r].x);
-        float sum = 0.0f, x = 0.0f;
+    const size_t part = 2 * static_cast<size_t>(blockIdx.x) + (first_part ? 0 : 1);
+    // a warp a row, four dimensions a lane
+    for (int r = warp; r < q.rows; r += kAttnWarps) {
+        float2 ml[kAttnWarps];
+        float top = -INFINITY, sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < kAttnWarps; ++w) {
-            const float2 ml = s_ml[w][r];
-            const float f = ml.x == top ? 1.0f : ex2(ml.x - top);
-            sum = fmaf(ml.y, f, sum);
-            x = fmaf(s_o[w][r][threadIdx.x], f, x);
+            ml[w] = s_ml[w][r];
+            top = fmaxf(top, ml[w].x);
         }
-        if (used > 1) {
-            a.part_o[(part * R + r) * kKvDim + threadIdx.x] = x;
-            if (threadIdx.x == 0) a.part_ml[part * R + r] = make_float2(top, sum);
-            continue;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < kAttnWarps; ++w) add_part(x, sum, *reinterpret_cast<const float4*>(&s_o[w][r][4 * lane]), ml[w], top);
+        if (whole) {
+            store_row<F32>(a, out_row(pl.w, c.kv_heads, a.group, head, q.row0 + r), x, top, sum);
+        } else {
+            __stcg(reinterpret_cast<float4*>(a.part_o + (part * R + r) * kKvDim + 4 * lane), x);
+            if (lane == 0) __stcg(a.part_ml + part * R + r, make_float2(top, sum));
         }
-        const int row = q.row0 + r, token = q.first_token + row / a.group, h = head * a.group + row % a.group;
-        const size_t at_row = static_cast<size_t>(token) * c.kv_heads * a.group + h;
-        store_out<F32>(a.out, at_row * kKvDim + threadIdx.x, sum == 0.0f ? 0.0f : x / sum);
-        if (threadIdx.x == 0 && a.lse != nullptr) a.lse[at_row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+    }
+    __syncthreads();
     }
 }
 
-// The splits of a tile joined; a CTA a tile and head.
+// The parts of a (tile, head) joined.  A CTA stands at the boundary of the CTAs blockIdx.x and blockIdx.x + 1 of the launch above, and
+// works if that is the first boundary inside a (tile, head); blockIdx.y is a row of the tile.
+constexpr int kJoinWarps = 8;
 template <bool F32>
-__global__ void __launch_bounds__(kKvDim) kv4_attention_join_kernel(const __grid_constant__ Kv4AttentionArgs a, int tile_rows) {
+__global__ void __launch_bounds__(32 * kJoinWarps) kv4_attention_join_kernel(const __grid_constant__ Kv4AttentionArgs a, int tile_rows, int parts) {
+    __shared__ long long s_scan[kJoinWarps + 2];
+    __shared__ float4 s_x[kJoinWarps][32];
+    __shared__ float2 s_ml[kJoinWarps];
     pdl_wait_prior_grids();
     pdl_release_dependents();
     const Kv4View& c = a.c;
-    const int head = blockIdx.y;
-    QTile q;
-    if (!find_qtile(c, a.group, tile_rows, blockIdx.x, &q)) return;
-    const int per = split_positions(q.seen, a.splits, a.least);
-    const int used = max(1, (q.seen + per - 1) / per);
-    if (used == 1) return;
-    const size_t part = (static_cast<size_t>(blockIdx.x) * c.kv_heads + head) * a.splits;
-    for (int r = 0; r < q.rows; ++r) {
-        float top = -INFINITY;
-        for (int s = 0; s < used; ++s) top = fmaxf(top, __ldcg(&a.part_ml[(part + s) * tile_rows + r].x));
-        float sum = 0.0f, x = 0.0f;
-        for (int s = 0; s < used; ++s) {
-            const float2 ml = __ldcg(&a.part_ml[(part + s) * tile_rows + r]);
-            const float f = ml.x == top ? 1.0f : ex2(ml.x - top);
-            sum = fmaf(ml.y, f, sum);
-            x = fmaf(__ldcg(a.part_o + ((part + s) * tile_rows + r) * kKvDim + threadIdx.x), f, x);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long per, all;
+    Place pl;
+    const int boundary = blockIdx.x + 1;
+    if (!find_unit<32 * kJoinWarps>(c, a.group, tile_rows, boundary, parts, s_scan, &per, &all, &pl)) return;
+    const int tile_head = static_cast<int>(pl.in_seq / pl.w.units);
+    const long long unit0 = per * boundary - (pl.in_seq - static_cast<long long>(tile_head) * pl.w.units);
+    const int c0 = static_cast<int>(unit0 / per), c1 = static_cast<int>((unit0 + pl.w.units - 1) / per);
+    const int head = tile_head % c.kv_heads, row = tile_head / c.kv_heads * tile_rows + blockIdx.y;
+    if (unit0 == per * boundary || c0 != boundary - 1 || row >= pl.w.n * a.group) return;
+    // part of CTA i: its first, unless the (tile, head) begins inside of it
+    auto part_row = [&](int i) { return (2 * static_cast<size_t>(i) + (i == c0 && unit0 != per * c0 ? 1 : 0)) * tile_rows + blockIdx.y; };
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float top = -INFINITY, sum = 0.0f;
+    constexpr int kDeep = 4;
+    for (int i0 = c0 + warp; i0 <= c1; i0 += kJoinWarps * kDeep) {
+        float4 p[kDeep];
+        float2 ml[kDeep];
+        float fresh = top;
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {
+            const int i = i0 + d * kJoinWarps;
+            ml[d] = make_float2(-INFINITY, 0.0f);
+            p[d] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (i <= c1) {
+                ml[d] = __ldcg(a.part_ml + part_row(i));
+                p[d] = __ldcg(reinterpret_cast<const float4*>(a.part_o + part_row(i) * kKvDim) + lane);
+            }
         }
-        const int row = q.row0 + r, token = q.first_token + row / a.group, h = head * a.group + row % a.group;
-        const size_t at_row = static_cast<size_t>(token) * c.kv_heads * a.group + h;
-        store_out<F32>(a.out, at_row * kKvDim + threadIdx.x, sum == 0.0f ? 0.0f : x / sum);
-        if (threadIdx.x == 0 && a.lse != nullptr) a.lse[at_row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) fresh = fmaxf(fresh, ml[d].x);
+        const float4 old = x;
+        const float2 old_ml = make_float2(top, sum);
+        x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        sum = 0.0f;
+        top = fresh;
+        add_part(x, sum, old, old_ml, top);
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) add_part(x, sum, p[d], ml[d], top);
     }
+    s_x[warp][lane] = x;
+    if (lane == 0) s_ml[warp] = make_float2(top, sum);
+    __syncthreads();
+    if (warp != 0) return;
+    top = -INFINITY;
+    sum = 0.0f;
+    x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, s_ml[w].x);
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) add_part(x, sum, s_x[w][lane], s_ml[w], top);
+    store_row<F32>(a, out_row(pl.w, c.kv_heads, a.group, head, row), x, top, sum);
 }
 
 // ---- attention weight of the cached positions ------------------------------------------------------------------
@@ -511,16 +601,10 @@ __global__ void __launch_bounds__(kAttnThreads) kv4_key_weight_kernel(const __gr
 
 Kv4AttentionPlan kv4_attention_plan(int num_tokens, int num_seqs, int q_heads, int kv_heads) {
     Kv4AttentionPlan p;
-    const long long group = q_heads / kv_heads, rows = group * num_tokens;
+    const long long rows = static_cast<long long>(q_heads / kv_heads) * num_tokens;
     p.nt = rows > 8ll * num_seqs ? 2 : 1;
-    const long long R = 8 * p.nt;
-    const long long by_token = num_tokens * ((group + R - 1) / R), by_rows = rows / R + num_seqs;
-    p.tiles = by_token < by_rows ? by_token : by_rows;
-    const long long ctas = p.tiles * kv_heads, want = 148 * 8;
-    p.splits = static_cast<int>(ctas >= want ? 1 : (want + ctas - 1) / ctas);
-    if (p.splits > 128) p.splits = 128;
-    p.least = 128;
-    const long long parts = p.splits > 1 ? ctas * p.splits * R : 0;
+    p.ctas = 148 * (p.nt == 1 ? 4 : 2);
+    const long long parts = 2ll * p.ctas * 8 * p.nt;
     p.ml_offset = parts * kKvDim * 4;
     p.bytes = p.ml_offset + parts * 8;
     return p;
@@ -529,19 +613,14 @@ Kv4AttentionPlan kv4_attention_plan(int num_tokens, int num_seqs, int q_heads, i
 int kv4_attention(Kv4AttentionArgs a, int q_heads, bool f32, void* workspace, cudaStream_t stream) {
     const Kv4View& c = a.c;
     const Kv4AttentionPlan p = kv4_attention_plan(c.num_tokens, c.num_seqs, q_heads, c.kv_heads);
-    if (p.tiles * p.splits > 0x7FFFFFFFll) return W4A16_ERR_TOO_LARGE;
-    a.splits = p.splits;
-    a.least = p.least;
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.ml_offset);
-    const dim3 grid(static_cast<unsigned>(p.tiles * p.splits), c.kv_heads);
     auto kernel = p.nt == 1 ? (f32 ? kv4_attention_kernel<1, true> : kv4_attention_kernel<1, false>)
                             : (f32 ? kv4_attention_kernel<2, true> : kv4_attention_kernel<2, false>);
-    cudaError_t e = launch_kernel(kernel, grid, dim3(kAttnThreads), 0, stream, pdl_enabled(), a);
-    if (e != cudaSuccess || p.splits == 1) return static_cast<int>(e);
-    const dim3 join(static_cast<unsigned>(p.tiles), c.kv_heads);
-    return static_cast<int>(launch_kernel(f32 ? kv4_attention_join_kernel<true> : kv4_attention_join_kernel<false>, join, dim3(kKvDim), 0, stream,
-                                          pdl_enabled(), a, 8 * p.nt));
+    cudaError_t e = launch_kernel(kernel, dim3(p.ctas), dim3(kAttnThreads), 0, stream, pdl_enabled(), a);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    return static_cast<int>(launch_kernel(f32 ? kv4_attention_join_kernel<true> : kv4_attention_join_kernel<false>, dim3(p.ctas - 1, 8 * p.nt),
+                                          dim3(32 * kJoinWarps), 0, stream, pdl_enabled(), a, 8 * p.nt, p.ctas));
 }
 
 int kv4_add_key_weights(const Kv4WeightArgs& a, cudaStream_t stream) {

@@ -10,10 +10,10 @@ struct Kv4AttentionArgs {
     const __half* q;
     void* out;
     float* lse;              // may be null
-    float* part_o;           // splits: unnormalised sums [tile][head][split][row][128] ...
+    float* part_o;           // parts: unnormalised sums [CTA][first, last][row][128] ...
     float2* part_ml;         // ... and maximum (base 2) and sum of weights
     float scale;
-    int group, q_stride, splits, least;
+    int group, q_stride;
 };
 struct Kv4WeightArgs {
     Kv4View c;
@@ -24,8 +24,8 @@ struct Kv4WeightArgs {
 };
 // How a call is cut; a function of its sizes alone, so that the workspace can be sized without a device.
 struct Kv4AttentionPlan {
-    int nt, splits, least;
-    long long tiles, ml_offset, bytes;
+    int nt, ctas;
+    long long ml_offset, bytes;
 };
 Kv4AttentionPlan kv4_attention_plan(int num_tokens, int num_seqs, int q_heads, int kv_heads);
 int kv4_attention(Kv4AttentionArgs a, int q_heads, bool f32, void* workspace, cudaStream_t stream);

@@ -50,7 +50,7 @@ REFUSED = [
     (dict(query_start=None), -1, ALL), (dict(page_size=8), -2, ALL), (dict(page_size=48), -2, ALL), (dict(page_size=8192), -2, ALL),
     (dict(pages=P + 8), -3, ALL), (dict(seq_lens=P + 2), -3, ALL), (dict(num_seqs=70000), -5, ALL), (dict(num_tokens=1 << 25), -5, ALL),
     (dict(k=None), -1, {"append"}), (dict(v=None), -1, {"append"}), (dict(q_out=None), -1, {"append"}), (dict(q=None), -1, {"append", "attention", "weights"}),
-    (dict(q=None, q_out=None, q_bias=P), -1, {"append"}), (dict(k=None, v=None), -1, {"append", "read"}),
+    (dict(q=None, q_out=None, q_bias=P), -1, {"append", "attention", "weights"}), (dict(k=None, v=None), -1, {"append", "read"}),
     (dict(heads=0), -1, {"append", "attention", "weights"}), (dict(heads=11), -2, {"append", "attention", "weights"}),
     (dict(q_stride=-8), -1, {"append", "attention", "weights"}), (dict(q_stride=1528), -2, {"append", "attention", "weights"}),
     (dict(q_stride=1540), -3, {"append", "attention", "weights"}), (dict(kv_stride=248), -2, {"append"}), (dict(q=P + 8), -3, {"append", "attention", "weights"}),
