@@ -441,8 +441,8 @@ W4A16_API int w4a16_gemm_prefill_dual_gate_up_swiglu_w4a16(const uint32_t* gate_
  */
 typedef struct w4a16_kv4_cache {
     void* pages;               /* the pool, 16-byte aligned */
-    float* key_weight;         /* fp32 [num_pages][num_kv_heads][page_size]: attention weight a position has got; may be
-                                  NULL where nothing is evicted */
+    float* key_weight;         /* fp32 [num_pages][num_kv_heads][page_size], 16-byte aligned: attention weight a position
+                                  has got; may be NULL where nothing is evicted */
     int num_pages, num_kv_heads, page_size;
 } w4a16_kv4_cache;
 /*

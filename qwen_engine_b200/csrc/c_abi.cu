@@ -65,6 +65,7 @@ int ensure_device_ready(const DeviceInfo** out) {
             if (int st = quantize_set_attributes()) return st;
             if (int st = gemv_set_attributes()) return st;
             if (int st = gemm_set_attributes()) return st;
+            if (int st = kv4_set_attributes()) return st;
             info.ready = true;
             g_dev[dev] = info;
             g_dev_ready[dev].store(true, std::memory_order_release);
@@ -93,7 +94,7 @@ int kv4_view(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, Kv4View
     if (!batch->query_start && batch->num_tokens != batch->num_seqs) return W4A16_ERR_INVALID_ARG;
     const int ps = cache->page_size;
     if (ps < 16 || ps > 4096 || (ps & (ps - 1)) != 0) return W4A16_ERR_SHAPE;
-    if (misaligned(cache->pages, 16) || misaligned(cache->key_weight, 4) || misaligned(batch->block_table, 4) || misaligned(batch->seq_lens, 4) ||
+    if (misaligned(cache->pages, 16) || misaligned(cache->key_weight, 16) || misaligned(batch->block_table, 4) || misaligned(batch->seq_lens, 4) ||
         misaligned(batch->query_start, 4))
         return W4A16_ERR_ALIGNMENT;
     if (cache->num_kv_heads > 65535 || batch->num_seqs > 65535 || batch->num_tokens > (1 << 24)) return W4A16_ERR_TOO_LARGE;

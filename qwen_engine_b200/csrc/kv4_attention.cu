@@ -6,10 +6,11 @@
 // head has query heads, and these, not the positions, are what is padded.  The rows of a head (token major) are cut into tiles
 // of 8 or 16; a tile's positions are split over CTAs, a CTA's over its four warps, 16 positions at a time.
 //
-//   scores^T [16 positions x 8 queries] = codes [16 x 128] . q^T;  then scale * score + zero * (sum of q), because a row is
-//       (code - 8) * scale + zero: the codes are exact in fp16 and no key is ever rounded.
-//   out^T [128 x 8] += codes^T [128 x 16] . (p * value scale)^T: the weight enters as two fp16 numbers whose sum has 22
-//       bits (one would leave 2^-11 in a 32-bit result), zeros as one 32-bit sum a query.
+//   scores^T [16 positions x 8 queries] = codes [16 x 128] . q^T;  then scale * score + (zero - 8 scale) * (sum of q), because a
+//       row is (code - 8) * scale + zero: the codes are exact in fp16 and no key is ever rounded.
+//   out^T [128 x 8] += codes^T [128 x 16] . (p * value scale)^T: for a 32-bit result the weight enters as two fp16 numbers
+//       whose sum has 22 bits, for an fp16 result as one (2^-12 of a weight is less than the result's own rounding, and
+//       the weights' roundings average out); zeros enter as one 32-bit sum a query.
 //   running maximum: renewed only where a score exceeds it by 2^8, which a vote finds; p <= 2^8 fits.
 #include "kv4.cuh"
 #include "kv4_attention.hpp"
@@ -126,31 +127,41 @@ struct KvRegs {
     uint32_t kp[2], vp[2];
     bool ok;
 };
-__device__ __forceinline__ void load_tile(const Kv4View& c, int page, int head, int at, int g, int t, KvRegs& r) {
-    const uint32_t* record = kv4_record_of_page(c, page, head);
-    r.ok = record != nullptr;
+// Where a lane's pieces of a record lie.
+struct KvOffsets {
+    const char* head;             // the head's record of page 0
+    size_t page;                  // bytes from page to page
+    int ps, key, value, param;    // the lane's first key and value row, and parameters, in bytes from a row's place
+};
+__device__ __forceinline__ KvOffsets kv_offsets(const Kv4View& c, int head, int g, int t) {
+    const int ps = 1 << c.page_shift;
+    const size_t record = static_cast<size_t>(kKvSlotWords * 4) << c.page_shift;
+    return {reinterpret_cast<const char*>(c.pages) + head * record, record * c.kv_heads, ps, 64 * g + 16 * t, 64 * ps + 128 * t + 8 * g, 128 * ps + 4 * g};
+}
+__device__ __forceinline__ void load_tile(const Kv4View& c, const KvOffsets& f, int page, int at, KvRegs& r) {
+    r.ok = static_cast<unsigned>(page) < static_cast<unsigned>(c.num_pages);
     if (!r.ok) return;
-    const int ps = 1 << c.page_shift, s = at & (ps - 1);
-    const uint32_t* keys = record + s * kKvRowWords;
-    const uint32_t* values = keys + ps * kKvRowWords;
-    const uint32_t* params = record + 32 * ps + s;
-    r.k[0] = __ldcg(reinterpret_cast<const uint4*>(keys + g * kKvRowWords + 4 * t));
-    r.k[1] = __ldcg(reinterpret_cast<const uint4*>(keys + (g + 8) * kKvRowWords + 4 * t));
-    r.kp[0] = __ldcg(params + g);
-    r.kp[1] = __ldcg(params + g + 8);
+    const int s = at & (f.ps - 1);
+    const char* rows = f.head + page * f.page + 64 * s;
+    const char* keys = rows + f.key;
+    const char* values = rows + f.value;
+    const char* params = rows + (f.param - 60 * s);
+    r.k[0] = __ldcg(reinterpret_cast<const uint4*>(keys));
+    r.k[1] = __ldcg(reinterpret_cast<const uint4*>(keys + 512));
+    r.kp[0] = __ldcg(reinterpret_cast<const uint32_t*>(params));
+    r.kp[1] = __ldcg(reinterpret_cast<const uint32_t*>(params + 32));
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        r.v[i] = __ldcg(reinterpret_cast<const uint2*>(values + (2 * t + (i & 1) + 8 * (i >> 1)) * kKvRowWords + 2 * g));
-    r.vp[0] = __ldcg(params + ps + g);
-    r.vp[1] = __ldcg(params + ps + g + 8);
+    for (int i = 0; i < 4; ++i) r.v[i] = __ldcg(reinterpret_cast<const uint2*>(values + 64 * (i & 1) + 512 * (i >> 1)));
+    r.vp[0] = __ldcg(reinterpret_cast<const uint32_t*>(params + 4 * f.ps));
+    r.vp[1] = __ldcg(reinterpret_cast<const uint32_t*>(params + 4 * f.ps + 32));
 }
 
-// B fragments of eight query rows for the eight k steps: step 2 j and 2 j + 1 take the elements of word 4 t + j in the order in
-// which the code conversion gives them.
+// B fragments of eight query rows for the eight k steps: steps 2 j and 2 j + 1 take the elements of word 4 t + j in the order in
+// which the code conversion gives them, 0 2 1 3 and 4 6 5 7.
 __device__ __forceinline__ void query_words(const uint4& w, uint32_t* b) {
     b[0] = __byte_perm(w.x, w.y, 0x5410);
-    b[1] = __byte_perm(w.z, w.w, 0x5410);
-    b[2] = __byte_perm(w.x, w.y, 0x7632);
+    b[1] = __byte_perm(w.x, w.y, 0x7632);
+    b[2] = __byte_perm(w.z, w.w, 0x5410);
     b[3] = __byte_perm(w.z, w.w, 0x7632);
 }
 __device__ __forceinline__ float sum_half8(const uint4& w) {
@@ -252,126 +263,150 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
     for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY;
     float pw = 0.0f;                                        // power of two on the value scales; 0: not chosen yet
 
-    constexpr int kStep = kUnit;
-    int at = k0 + warp * kKvTile;
-    KvRegs cur;
-    int next_page = -1;
-    if (at < k1) load_tile(c, kv4_page(c, q.seq, at), head, at, g, t, cur);
-    if (at + kStep < k1) next_page = kv4_page(c, q.seq, at + kStep);
-    for (; at < k1; at += kStep) {
-        KvRegs nxt;
-        nxt.ok = false;
-        if (at + kStep < k1) load_tile(c, next_page, head, at + kStep, g, t, nxt);
-        if (at + 2 * kStep < k1) next_page = kv4_page(c, q.seq, at + 2 * kStep);
-        if (cur.ok) {
-            float s[NT][4] = {};
-            const uint32_t kw0[4] = {cur.k[0].x, cur.k[0].y, cur.k[0].z, cur.k[0].w}, kw1[4] = {cur.k[1].x, cur.k[1].y, cur.k[1].z, cur.k[1].w};
+    float mu[NT][2];                                        // m, or 0 where nothing has been seen
+    for (int n = 0; n < NT; ++n) mu[n][0] = mu[n][1] = 0.0f;
+    const KvOffsets f = kv_offsets(c, head, g, t);
+    auto take = [&](const KvRegs& r, int at) {
+        if (!r.ok) return;
+        float even[NT][4] = {}, s[NT][4] = {};
+        const uint32_t kw0[4] = {r.k[0].x, r.k[0].y, r.k[0].z, r.k[0].w}, kw1[4] = {r.k[1].x, r.k[1].y, r.k[1].z, r.k[1].w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t lo[4], hi[4];
-                kv4_codes_to_half2(kw0[j], lo);
-                kv4_codes_to_half2(kw1[j], hi);
-                const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]}, a1[4] = {lo[2], hi[2], lo[3], hi[3]};
+        for (int j = 0; j < 4; ++j) {
+            uint32_t lo[4], hi[4];
+            kv4_key_codes(kw0[j], lo);
+            kv4_key_codes(kw1[j], hi);
+            const uint32_t a0[4] = {lo[0], hi[0], lo[2], hi[2]}, a1[4] = {lo[1], hi[1], lo[3], hi[3]};
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    mma_16816(s[n], a0, qb[n][4 * j], qb[n][4 * j + 1]);
-                    mma_16816(s[n], a1, qb[n][4 * j + 2], qb[n][4 * j + 3]);
-                }
+            for (int n = 0; n < NT; ++n) {
+                mma_16816(even[n], a0, qb[n][4 * j], qb[n][4 * j + 1]);
+                mma_16816(s[n], a1, qb[n][4 * j + 2], qb[n][4 * j + 3]);
             }
-            const float ks[2] = {kv4_scale(cur.kp[0]) * to_log2, kv4_scale(cur.kp[1]) * to_log2};
-            const float kz[2] = {kv4_zero(cur.kp[0]), kv4_zero(cur.kp[1])};
-            float vs[2] = {kv4_scale(cur.vp[0]), kv4_scale(cur.vp[1])};
-            float vz[2] = {fmaf(-0.5f, vs[0], kv4_zero(cur.vp[0])), fmaf(-0.5f, vs[1], kv4_zero(cur.vp[1]))};     // codes are taken around 7.5
-            const bool cut = at + kKvTile > all_see;        // some row does not see some of these positions
-            bool above = false;
+        }
+        float ks[2], kz[2], vs[2], vz[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            ks[i] = kv4_scale(r.kp[i]);
+            kz[i] = fmaf(-8.0f, ks[i], kv4_zero(r.kp[i]));
+            ks[i] *= to_log2 * kKvKeyUndo;
+            vs[i] = kv4_scale(r.vp[i]);
+            vz[i] = fmaf(-0.5f, vs[i], kv4_zero(r.vp[i]));  // codes are taken around 7.5
+        }
+        const bool cut = at + kKvTile > all_see;            // some row does not see some of these positions
+        bool above = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = fmaf(kv4_key_sum(even[n][e], s[n][e]), ks[e >> 1], kz[e >> 1] * qsum[n][e & 1]);
+        if (cut) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[n][e] = fmaf(s[n][e], ks[e >> 1], kz[e >> 1] * qsum[n][e & 1]);
-                    if (cut && at + g + 8 * (e >> 1) >= limit[n][e & 1]) s[n][e] = -INFINITY;
-                    above = above || s[n][e] > m[n][e & 1] + 8.0f;
-                }
-            if (cut) {
+                for (int e = 0; e < 4; ++e)
+                    if (at + g + 8 * (e >> 1) >= limit[n][e & 1]) s[n][e] = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (at + g + 8 * i >= k1) vs[i] = vz[i] = 0.0f;
+            for (int i = 0; i < 2; ++i)
+                if (at + g + 8 * i >= k1) vs[i] = vz[i] = 0.0f;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) above = above || fmaxf(s[n][e], s[n][e + 2]) > m[n][e] + 8.0f;
+        if (__any_sync(0xFFFFFFFFu, above || pw == 0.0f || fmaxf(vs[0], vs[1]) * pw > 64.0f)) {
+            float big = fmaxf(vs[0], vs[1]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, d));
+            float ratio = 1.0f;
+            if (pw == 0.0f || big * pw > 64.0f) {           // the largest value scale times pw into [8, 16)
+                const float fresh = big > 0.0f ? __uint_as_float((130u + 127u - (__float_as_uint(big) >> 23)) << 23) : 1.0f;
+                ratio = pw == 0.0f ? 1.0f : fresh / pw;
+                pw = fresh;
             }
-            const bool far = pw == 0.0f || vs[0] * pw > 64.0f || vs[1] * pw > 64.0f;
-            if (__any_sync(0xFFFFFFFFu, above || far)) {
-                float big = fmaxf(vs[0], vs[1]);
 #pragma unroll
-                for (int d = 4; d < 32; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, d));
-                float ratio = 1.0f;
-                if (pw == 0.0f || big * pw > 64.0f) {       // the largest value scale times pw into [8, 16)
-                    const float fresh = big > 0.0f ? __uint_as_float((130u + 127u - (__float_as_uint(big) >> 23)) << 23) : 1.0f;
-                    ratio = pw == 0.0f ? 1.0f : fresh / pw;
-                    pw = fresh;
-                }
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int e = 0; e < 2; ++e) {
+                    float x = fmaxf(s[n][e], s[n][e + 2]);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float x = fmaxf(s[n][e], s[n][e + 2]);
+                    for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
+                    const float fresh = fmaxf(m[n][e], x);
+                    const float f = fresh == m[n][e] ? 1.0f : ex2(m[n][e] - fresh);
+                    m[n][e] = fresh;
+                    mu[n][e] = fresh == -INFINITY ? 0.0f : fresh;
+                    l[n][e] *= f;
+                    zacc[n][e] *= f;
 #pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
-                        const float fresh = fmaxf(m[n][e], x);
-                        const float f = fresh == m[n][e] ? 1.0f : ex2(m[n][e] - fresh);
-                        m[n][e] = fresh;
-                        l[n][e] *= f;
-                        zacc[n][e] *= f;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            o[n][i][e] *= f * ratio;
-                            o[n][i][e + 2] *= f * ratio;
-                        }
+                    for (int i = 0; i < 8; ++i) {
+                        o[n][i][e] *= f * ratio;
+                        o[n][i][e + 2] *= f * ratio;
                     }
-            }
-            vs[0] *= pw;
-            vs[1] *= pw;
-            uint32_t ph[NT][2], pl[NT][2];                  // p * value scale in two fp16 parts, columns = positions
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float x[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float top = m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1];
-                    const float p = ex2(s[n][e] - top);
-                    l[n][e & 1] += p;
-                    x[e] = p * vs[e >> 1];
-                    float z = p * vz[e >> 1];
-                    if (cut && at + g + 8 * (e >> 1) >= limit[n][e & 1]) x[e] = z = 0.0f;   // whatever the row holds
-                    zacc[n][e & 1] += z;
                 }
+        }
+        vs[0] *= pw;
+        vs[1] *= pw;
+        uint32_t ph[NT][2], pl[NT][2];                      // p * value scale in one or two fp16 parts, columns = positions
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-                    const float2 f = __half22float2(h);
-                    ph[n][i] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&h));
-                    pl[n][i] = transpose_8x8(pack_half2(x[2 * i] - f.x, x[2 * i + 1] - f.y));
-                }
+        for (int n = 0; n < NT; ++n) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p = ex2(s[n][e] - mu[n][e & 1]);
+                l[n][e & 1] += p;
+                x[e] = p * vs[e >> 1];
+                float z = p * vz[e >> 1];
+                if (cut && at + g + 8 * (e >> 1) >= limit[n][e & 1]) x[e] = z = 0.0f;   // whatever the row holds
+                zacc[n][e & 1] += z;
             }
-            // values: pair two positions' words by 16-bit halves, then each nibble place is one dimension of both
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const uint32_t sel = half ? 0x7632u : 0x5410u;
-                uint32_t f[4][4];
-                kv4_value_codes_to_half2(__byte_perm(cur.v[0].x, cur.v[1].x, sel), f[0]);
-                kv4_value_codes_to_half2(__byte_perm(cur.v[0].y, cur.v[1].y, sel), f[1]);
-                kv4_value_codes_to_half2(__byte_perm(cur.v[2].x, cur.v[3].x, sel), f[2]);
-                kv4_value_codes_to_half2(__byte_perm(cur.v[2].y, cur.v[3].y, sel), f[3]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t av[4] = {f[0][i], f[1][i], f[2][i], f[3][i]};
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        mma_16816(o[n][half * 4 + i], av, ph[n][0], ph[n][1]);
-                        mma_16816(o[n][half * 4 + i], av, pl[n][0], pl[n][1]);
-                    }
+            for (int i = 0; i < 2; ++i) {
+                const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+                ph[n][i] = transpose_8x8(*reinterpret_cast<const uint32_t*>(&h));
+                if constexpr (F32) {
+                    const float2 b = __half22float2(h);
+                    pl[n][i] = transpose_8x8(pack_half2(x[2 * i] - b.x, x[2 * i + 1] - b.y));
                 }
             }
         }
-        cur = nxt;
+        // values: pair two positions' words by 16-bit halves, then each nibble place is one dimension of both
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const uint32_t sel = half ? 0x7632u : 0x5410u;
+            uint32_t w[4][4];
+            kv4_value_codes_to_half2(__byte_perm(r.v[0].x, r.v[1].x, sel), w[0]);
+            kv4_value_codes_to_half2(__byte_perm(r.v[0].y, r.v[1].y, sel), w[1]);
+            kv4_value_codes_to_half2(__byte_perm(r.v[2].x, r.v[3].x, sel), w[2]);
+            kv4_value_codes_to_half2(__byte_perm(r.v[2].y, r.v[3].y, sel), w[3]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t av[4] = {w[0][i], w[1][i], w[2][i], w[3][i]};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    mma_16816(o[n][half * 4 + i], av, ph[n][0], ph[n][1]);
+                    if constexpr (F32) mma_16816(o[n][half * 4 + i], av, pl[n][0], pl[n][1]);
+                }
+            }
+        }
+    };
+
+    // 16 positions in use, the next 16 on their way, the page number of those behind them too
+    int at = k0 + warp * kKvTile;
+    KvRegs r0, r1;
+    r0.ok = r1.ok = false;
+    int next_page = -1;
+    if (at < k1) load_tile(c, f, kv4_page(c, q.seq, at), at, r0);
+    if (at + kUnit < k1) next_page = kv4_page(c, q.seq, at + kUnit);
+    auto ahead = [&](KvRegs& r) {
+        r.ok = false;
+        if (at + kUnit < k1) load_tile(c, f, next_page, at + kUnit, r);
+        if (at + 2 * kUnit < k1) next_page = kv4_page(c, q.seq, at + 2 * kUnit);
+    };
+    while (at < k1) {
+        ahead(r1);
+        take(r0, at);
+        at += kUnit;
+        if (at >= k1) break;
+        ahead(r0);
+        take(r1, at);
+        at += kUnit;
     }
 
     // the warps' parts into shared memory: a lane has dimensions 16 g .. 16 g + 15 of queries 2 t and 2 t + 1
@@ -526,12 +561,12 @@ __global__ void __launch_bounds__(kAttnThreads) kv4_key_weight_kernel(const __gr
                     w = __ldcg(reinterpret_cast<const uint4*>(record + s * kKvRowWords + 4 * t));
                     params = __ldcg(record + 32 * ps + s);
                 }
-                ks[2 * u + i] = kv4_scale(params) * to_log2;
-                kz[2 * u + i] = kv4_zero(params);
-                kv4_codes_to_half2(w.x, codes[u][0][i]);
-                kv4_codes_to_half2(w.y, codes[u][1][i]);
-                kv4_codes_to_half2(w.z, codes[u][2][i]);
-                kv4_codes_to_half2(w.w, codes[u][3][i]);
+                ks[2 * u + i] = kv4_scale(params) * (to_log2 * kKvKeyUndo);
+                kz[2 * u + i] = fmaf(-8.0f, kv4_scale(params), kv4_zero(params));
+                kv4_key_codes(w.x, codes[u][0][i]);
+                kv4_key_codes(w.y, codes[u][1][i]);
+                kv4_key_codes(w.z, codes[u][2][i]);
+                kv4_key_codes(w.w, codes[u][3][i]);
             }
         }
         for (int r0 = 0; r0 < rows; r0 += kWeightRows) {
@@ -557,15 +592,15 @@ __global__ void __launch_bounds__(kAttnThreads) kv4_key_weight_kernel(const __gr
             __syncthreads();
             const int blocks = (min(rows - r0, kWeightRows) + 7) / 8;
             for (int n = 0; n < blocks; ++n) {
-                float s[2][4] = {};
+                float even[2][4] = {}, s[2][4] = {};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint4 f = s_q[n][j][lane];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const uint32_t a0[4] = {codes[u][j][0][0], codes[u][j][1][0], codes[u][j][0][1], codes[u][j][1][1]};
-                        const uint32_t a1[4] = {codes[u][j][0][2], codes[u][j][1][2], codes[u][j][0][3], codes[u][j][1][3]};
-                        mma_16816(s[u], a0, f.x, f.y);
+                        const uint32_t a0[4] = {codes[u][j][0][0], codes[u][j][1][0], codes[u][j][0][2], codes[u][j][1][2]};
+                        const uint32_t a1[4] = {codes[u][j][0][1], codes[u][j][1][1], codes[u][j][0][3], codes[u][j][1][3]};
+                        mma_16816(even[u], a0, f.x, f.y);
                         mma_16816(s[u], a1, f.z, f.w);
                     }
                 }
@@ -578,7 +613,7 @@ __global__ void __launch_bounds__(kAttnThreads) kv4_key_weight_kernel(const __gr
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const float x = fmaf(s[u][2 * i + e], ks[2 * u + i], kz[2 * u + i] * qs) - lse;
+                            const float x = fmaf(kv4_key_sum(even[u][2 * i + e], s[u][2 * i + e]), ks[2 * u + i], kz[2 * u + i] * qs) - lse;
                             if (at + 16 * u + 8 * i + g < limit) got[2 * u + i] += ex2(x);
                         }
                 }

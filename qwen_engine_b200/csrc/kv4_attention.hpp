@@ -45,6 +45,7 @@ struct Kv4EvictArgs {
 };
 int kv4_append(const Kv4View& c, const Kv4AppendArgs& x, cudaStream_t stream);
 int kv4_read(const Kv4View& c, __half* k_out, __half* v_out, cudaStream_t stream);
+int kv4_set_attributes();
 int kv4_evict(const Kv4View& c, const Kv4EvictArgs& x, cudaStream_t stream);
 
 }  // namespace w4

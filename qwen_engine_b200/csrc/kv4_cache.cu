@@ -38,8 +38,9 @@ __device__ __forceinline__ uint4 float_to_half8(const float (&x)[8]) {
 }
 
 // One row of 128 fp16 values, 8 a lane of a half-warp, to its code word and (scale, zero).  Both halves of a warp call it.
-// IEEE division and rounding throughout, so the codes are those of the formula.  A row with an infinity or a NaN gets a
-// NaN scale: it reads back as NaN instead of as finite values that it does not hold.
+// The codes are those of the formula in IEEE arithmetic: a product with the reciprocal is off by less than 1e-5 (|quotient|
+// < 11), so only where that lands nearer than this to a border between two codes is the division made.  A row with an infinity
+// or a NaN gets a NaN scale: it reads back as NaN instead of as finite values that it does not hold.
 __device__ __forceinline__ uint32_t kv4_quantise_lane(const float (&x)[8], uint32_t* params) {
     float lo = x[0], hi = x[0];
     bool finite = true;
@@ -60,120 +61,174 @@ __device__ __forceinline__ uint32_t kv4_quantise_lane(const float (&x)[8], uint3
     const float s = __half2float(scale);
     __half zero = __float2half_rn(__fadd_rn(lo, 8.0f * s));
     const float z = __half2float(zero);
-    uint32_t word = 0;
+    uint32_t word = 0x88888888u;
     constexpr int kShift[8] = {0, 8, 16, 24, 4, 12, 20, 28};
+    if (row_finite && s > 0.0f) {
+        word = 0;
+        const float inv = __frcp_rn(s);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        int code = 8;
-        if (row_finite && s > 0.0f) code = min(max(__float2int_rn(__fdiv_rn(x[j] - z, s)) + 8, 0), 15);
-        word |= static_cast<uint32_t>(code) << kShift[j];
+        for (int j = 0; j < 8; ++j) {
+            float t = (x[j] - z) * inv;
+            if (fabsf(fabsf(t - rintf(t)) - 0.5f) < 2e-5f) t = __fdiv_rn(x[j] - z, s);
+            word |= static_cast<uint32_t>(min(max(__float2int_rn(t) + 8, 0), 15)) << kShift[j];
+        }
     }
     if (!row_finite) scale = zero = __ushort_as_half(0x7FFF);
     *params = static_cast<uint32_t>(__half_as_ushort(scale)) | (static_cast<uint32_t>(__half_as_ushort(zero)) << 16);
     return word;
 }
 
-// One token's rows: q_heads of q (rotated into q_out), kv_heads of k (rotated, quantised), kv_heads of v (quantised).
-// A CTA takes 16 of them.  Angles are position * inv_freq in 64 bits, reduced to a turn there (a 32-bit angle of
-// position 100 000 is off by 0.004 rad), the 64 sines and cosines of a token worked out once a CTA.
+// Where a token of the batch goes.
+struct Spot {
+    int seq, at, page;       // seq < 0: the token belongs to no sequence; page < 0: it has no place in the cache
+};
+__device__ __forceinline__ Spot find_spot(const Kv4View& c, int token) {     // a whole warp calls it
+    Spot s{-1, 0, -1};
+    if (token >= c.num_tokens) return s;
+    const int seq = kv4_seq_of_token(c, token);
+    if (seq >= c.num_seqs) return s;
+    const int2 mine = kv4_new_tokens(c, seq);
+    if (token < mine.x || token >= mine.x + mine.y) return s;
+    s.seq = seq;
+    s.at = __ldcg(c.lens + seq) - mine.y + (token - mine.x);
+    if (s.at >= 0 && s.at < kv4_capacity(c)) {
+        const int page = kv4_page(c, seq, s.at);
+        if (static_cast<unsigned>(page) < static_cast<unsigned>(c.num_pages)) s.page = page;
+    }
+    return s;
+}
+
+// The rows of TOK tokens: q_heads of q (rotated into q_out), kv_heads of k (rotated, quantised), kv_heads of v (quantised).
+// A CTA takes 16 of a token's rows; all its rows are requested first, then a warp a token finds its place (three dependent
+// round trips), then the threads share the tokens' 64 angles.  Angles are position * inv_freq in 64 bits, reduced to a turn
+// there (a 32-bit angle of position 100 000 is off by 0.004 rad).  What bounds a prompt are those round trips: with one token a
+// CTA instead of four 4 prompts of up to 4100 tokens took 79 us.
+template <int TOK>
 __global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(const __grid_constant__ AppendArgs a) {
-    __shared__ float2 s_turn[kKvDim / 2];
+    __shared__ float2 s_turn[TOK][kKvDim / 2];
+    __shared__ Spot s_spot[TOK];
+    __shared__ int s_pos[TOK];
     pdl_wait_prior_grids();
     pdl_release_dependents();
     const Kv4View& c = a.c;
-    const int token = blockIdx.x / a.blocks_per_token;
-    const int row = (blockIdx.x - token * a.blocks_per_token) * (kAppendThreads / kRowThreads) + (threadIdx.x >> 4);
-    const int hl = threadIdx.x & 15;
+    const int token0 = blockIdx.x / a.blocks_per_token * TOK;
+    const int row = (blockIdx.x % a.blocks_per_token) * (kAppendThreads / kRowThreads) + (threadIdx.x >> 4);
+    const int hl = threadIdx.x & 15, warp = threadIdx.x >> 5;
     const int n_q = a.q != nullptr ? a.q_heads : 0, rows = n_q + 2 * c.kv_heads;
     // what the row is: 0 q, 1 k, 2 v
     const int kind = row < n_q ? 0 : row < n_q + c.kv_heads ? 1 : 2;
     const int head = row - (kind == 0 ? 0 : kind == 1 ? n_q : n_q + c.kv_heads);
     const bool on = row < rows;
-    uint4 raw = make_uint4(0, 0, 0, 0), bias = raw;
-    if (on) {
-        const __half* src = kind == 0 ? a.q + static_cast<size_t>(token) * a.q_stride
-                                      : (kind == 1 ? a.k : a.v) + static_cast<size_t>(token) * a.kv_stride;
-        raw = __ldcg(reinterpret_cast<const uint4*>(src + head * kKvDim + hl * 8));
-        const __half* b = kind == 0 ? a.q_bias : kind == 1 ? a.k_bias : a.v_bias;
-        if (b != nullptr) bias = __ldcg(reinterpret_cast<const uint4*>(b + head * kKvDim + hl * 8));
-    }
-    const int seq = kv4_seq_of_token(c, token);
-    if (seq >= c.num_seqs) return;                               // behind the last sequence: left as it is
-    const int2 mine = kv4_new_tokens(c, seq);
-    const int at = __ldcg(c.lens + seq) - mine.y + (token - mine.x);
-    if (token < mine.x || token >= mine.x + mine.y) return;
-    if (a.inv_freq != nullptr && threadIdx.x < kKvDim / 2) {
-        const int pos = a.positions != nullptr ? __ldcg(a.positions + token) : at;
-        const double turns = static_cast<double>(pos) * static_cast<double>(__ldcg(a.inv_freq + threadIdx.x)) * 0.15915494309189533577;
-        float sn, cs;
-        sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sn, &cs);
-        s_turn[threadIdx.x] = make_float2(cs, sn);
-    }
-    __syncthreads();
-    float x[8], b[8];
-    half8_to_float(raw, x);
-    half8_to_float(bias, b);
+    const __half* src = (kind == 0 ? a.q : kind == 1 ? a.k : a.v) + head * kKvDim + hl * 8;
+    const int stride = kind == 0 ? a.q_stride : a.kv_stride;
+    uint4 raw[TOK], bias = make_uint4(0, 0, 0, 0);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] += b[j];
-    if (a.inv_freq != nullptr) {
-        // values d and d + 64 are a pair: lanes hl and hl ^ 8
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float other = __shfl_xor_sync(0xFFFFFFFFu, x[j], 8);
-            const float2 t = s_turn[(hl & 7) * 8 + j];
-            if (kind != 2) x[j] = hl < 8 ? x[j] * t.x - other * t.y : x[j] * t.x + other * t.y;
+    for (int i = 0; i < TOK; ++i)
+        raw[i] = on && token0 + i < c.num_tokens ? __ldcg(reinterpret_cast<const uint4*>(src + static_cast<size_t>(token0 + i) * stride)) : make_uint4(0, 0, 0, 0);
+    const __half* b = kind == 0 ? a.q_bias : kind == 1 ? a.k_bias : a.v_bias;
+    if (on && b != nullptr) bias = __ldcg(reinterpret_cast<const uint4*>(b + head * kKvDim + hl * 8));
+    if (warp < TOK) {
+        const int token = token0 + warp;
+        int pos = 0;
+        if (a.positions != nullptr && token < c.num_tokens) pos = __ldcg(a.positions + token);
+        const Spot s = find_spot(c, token);
+        if ((threadIdx.x & 31) == 0) {
+            s_spot[warp] = s;
+            s_pos[warp] = a.positions != nullptr ? pos : s.at;
         }
     }
-    const uint4 rounded = float_to_half8(x);
-    if (on && kind == 0)
-        *reinterpret_cast<uint4*>(a.q_out + static_cast<size_t>(token) * a.q_stride + head * kKvDim + hl * 8) = rounded;
-    half8_to_float(rounded, x);
-    uint32_t params;
-    const uint32_t word = kv4_quantise_lane(x, &params);
-    if (!on || kind == 0 || at < 0 || at >= kv4_capacity(c)) return;
-    const int page = kv4_page(c, seq, at);
-    uint32_t* record = kv4_record_of_page(c, page, head);
-    if (record == nullptr) return;
-    const int ps = 1 << c.page_shift, slot = at & (ps - 1), part = kind - 1;
-    record[(part * ps + slot) * kKvRowWords + hl] = word;
-    if (hl == 0) {
-        record[(32 + part) * ps + slot] = params;
-        if (kind == 1 && c.key_weight != nullptr) c.key_weight[kv4_weight_index(c, page, head, at)] = 0.0f;
+    __syncthreads();
+    if (a.inv_freq != nullptr) {
+        for (int i = threadIdx.x; i < TOK * kKvDim / 2; i += kAppendThreads) {
+            const double turns = static_cast<double>(s_pos[i >> 6]) * static_cast<double>(__ldcg(a.inv_freq + (i & 63))) * 0.15915494309189533577;
+            float sn, cs;
+            sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sn, &cs);
+            s_turn[i >> 6][i & 63] = make_float2(cs, sn);
+        }
+    }
+    __syncthreads();
+    float bf[8];
+    half8_to_float(bias, bf);
+    const int ps = 1 << c.page_shift, part = kind - 1;
+#pragma unroll
+    for (int i = 0; i < TOK; ++i) {
+        const Spot s = s_spot[i];
+        if (s.seq < 0) continue;                                 // behind the last sequence: left as it is
+        float x[8];
+        half8_to_float(raw[i], x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] += bf[j];
+        if (a.inv_freq != nullptr) {
+            // values d and d + 64 are a pair: lanes hl and hl ^ 8
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float other = __shfl_xor_sync(0xFFFFFFFFu, x[j], 8);
+                const float2 t = s_turn[i][(hl & 7) * 8 + j];
+                if (kind != 2) x[j] = hl < 8 ? x[j] * t.x - other * t.y : x[j] * t.x + other * t.y;
+            }
+        }
+        const uint4 rounded = float_to_half8(x);
+        if (on && kind == 0)
+            *reinterpret_cast<uint4*>(a.q_out + static_cast<size_t>(token0 + i) * a.q_stride + head * kKvDim + hl * 8) = rounded;
+        const bool stored = on && kind != 0 && s.page >= 0;
+        if (__any_sync(0xFFFFFFFFu, stored)) {
+            half8_to_float(rounded, x);
+            uint32_t params;
+            const uint32_t word = kv4_quantise_lane(x, &params);
+            if (stored) {
+                uint32_t* record = kv4_record_of_page(c, s.page, head);
+                const int slot = s.at & (ps - 1);
+                record[(part * ps + slot) * kKvRowWords + hl] = word;
+                if (hl == 0) {
+                    record[(32 + part) * ps + slot] = params;
+                    if (kind == 1 && c.key_weight != nullptr) c.key_weight[kv4_weight_index(c, s.page, head, s.at)] = 0.0f;
+                }
+            }
+        }
     }
 }
 
-// The rows that an append of this batch writes, as fp16.  A half-warp a row.
+// The rows that an append of this batch writes, as fp16.  A half-warp a row, TOK tokens a CTA as above.
+template <int TOK>
 __global__ void __launch_bounds__(kAppendThreads) kv4_read_kernel(const __grid_constant__ Kv4View c, __half* k_out, __half* v_out, int blocks_per_token) {
+    __shared__ Spot s_spot[TOK];
     pdl_wait_prior_grids();
     pdl_release_dependents();
-    const int token = blockIdx.x / blocks_per_token;
-    const int row = (blockIdx.x - token * blocks_per_token) * (kAppendThreads / kRowThreads) + (threadIdx.x >> 4);
-    const int hl = threadIdx.x & 15;
-    const int seq = kv4_seq_of_token(c, token);
-    if (seq >= c.num_seqs || row >= 2 * c.kv_heads) return;
-    const int2 mine = kv4_new_tokens(c, seq);
-    if (token < mine.x || token >= mine.x + mine.y) return;
-    const int part = row >= c.kv_heads, head = row - part * c.kv_heads;
+    const int token0 = blockIdx.x / blocks_per_token * TOK;
+    const int row = (blockIdx.x % blocks_per_token) * (kAppendThreads / kRowThreads) + (threadIdx.x >> 4);
+    const int hl = threadIdx.x & 15, warp = threadIdx.x >> 5;
+    if (warp < TOK) {
+        const Spot s = find_spot(c, token0 + warp);
+        if ((threadIdx.x & 31) == 0) s_spot[warp] = s;
+    }
+    __syncthreads();
+    const int part = row >= c.kv_heads, head = row - part * c.kv_heads, ps = 1 << c.page_shift;
     __half* out = part ? v_out : k_out;
-    if (out == nullptr) return;
-    const int at = __ldcg(c.lens + seq) - mine.y + (token - mine.x);
-    uint4 got = make_uint4(0, 0, 0, 0);
-    const uint32_t* record = at >= 0 && at < kv4_capacity(c) ? kv4_record_of_page(c, kv4_page(c, seq, at), head) : nullptr;
-    if (record != nullptr) {
-        const int ps = 1 << c.page_shift, slot = at & (ps - 1);
-        const uint32_t word = __ldcg(record + (part * ps + slot) * kKvRowWords + hl);
-        const uint32_t params = __ldcg(record + (32 + part) * ps + slot);
-        const float s = kv4_scale(params), z = kv4_zero(params);
+    if (row >= 2 * c.kv_heads || out == nullptr) return;
+    uint32_t word[TOK], params[TOK];
+#pragma unroll
+    for (int i = 0; i < TOK; ++i) {
+        word[i] = params[i] = 0;                                 // a scale of zero: zeros
+        const Spot s = s_spot[i];
+        if (s.page < 0) continue;
+        const uint32_t* record = kv4_record_of_page(c, s.page, head);
+        const int slot = s.at & (ps - 1);
+        word[i] = __ldcg(record + (part * ps + slot) * kKvRowWords + hl);
+        params[i] = __ldcg(record + (32 + part) * ps + slot);
+    }
+#pragma unroll
+    for (int i = 0; i < TOK; ++i) {
+        if (s_spot[i].seq < 0) continue;
+        const float s = kv4_scale(params[i]), z = kv4_zero(params[i]);
         constexpr int kShift[8] = {0, 8, 16, 24, 4, 12, 20, 28};
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            x[j] = fmaf(static_cast<float>(static_cast<int>((word >> kShift[j]) & 15u) - 8), s, z);
+            x[j] = fmaf(static_cast<float>(static_cast<int>((word[i] >> kShift[j]) & 15u) - 8), s, z);
             if (fabsf(x[j]) > 65504.0f) x[j] = copysignf(65504.0f, x[j]);    // the rounding of scale and zero may step over fp16's end
         }
-        got = float_to_half8(x);
+        *reinterpret_cast<uint4*>(out + (static_cast<size_t>(token0 + i) * c.kv_heads + head) * kKvDim + hl * 8) = float_to_half8(x);
     }
-    *reinterpret_cast<uint4*>(out + (static_cast<size_t>(token) * c.kv_heads + head) * kKvDim + hl * 8) = got;
 }
 
 // ---- eviction ------------------------------------------------------------------------------------------------
@@ -184,6 +239,7 @@ struct EvictArgs {
     int32_t* new_lens;
     int32_t* kept;                       // [num_seqs][kv_heads][budget]
     int dst_pages, budget, sink, recent;
+    int cluster;                         // CTAs of a sequence and head
 };
 
 // Order of the weights as unsigned numbers: larger weight, larger key; a NaN is below everything.
@@ -194,136 +250,291 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelectThreads = 1024;
+// Choice and copy in one launch, a cluster of CTAs for each sequence and head, a CTA for a slice of its positions:
+//   1. the weights' keys into shared memory, four a thread and request (or, where a slice is longer, read again in every pass);
+//   2. the n-th largest key of the middle part, narrowed down by histograms of 2048 bins over the range that is left.  The first
+//      range is the weights from 2^-32 to 2^32, 32 bins an octave, with what is outside in the end bins: as many bins
+//      over all 32 bits would be 4 an octave, where the lanes' additions meet.  The histograms stay where they are; the cluster
+//      exchanges sums of 32 bins, then the 32 bins that matter (all bins of 7 other CTAs took 5 us a round);
+//   3. every warp counts what stays of its run of positions; scans over warps and CTAs give each its first new position;
+//   4. the same run again: new positions by ballot, the old ones written down in order;
+//   5. the rows copied, shared out evenly over the cluster, eight lanes a position (16 bytes each), four positions in flight.
+// Integer counts and a fixed order throughout, so equal weights fall the same way every time.
+constexpr int kEvictThreads = 1024, kEvictWarps = kEvictThreads / 32;
+constexpr int kEvictBins = 2048, kEvictCoarse = kEvictBins / 32;
+constexpr int kEvictCached = 16384;      // keys of a slice in shared memory
+constexpr int kEvictMaxCluster = 8;
+constexpr uint32_t kEvictFirst = 0xAF800000u;     // key of 2^-32
+constexpr int kEvictFirstShift = 18;
 
-// Which positions of one sequence and head stay, in order.  The n-th largest key of the middle part by a radix search, a byte
-// a round; then one ordered pass that numbers what stays.
-__global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const __grid_constant__ EvictArgs a) {
-    __shared__ uint32_t s_hist[256];
-    __shared__ uint32_t s_prefix, s_need;
-    __shared__ int s_warp[2][32];
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t ld_cluster(const void* mine, uint32_t rank) {
+    uint32_t at, v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(mine))), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+
+__global__ void __launch_bounds__(kEvictThreads, 1) kv4_evict_kernel(const __grid_constant__ EvictArgs a) {
+    extern __shared__ uint32_t s_keys[];                         // [kEvictCached]
+    __shared__ uint32_t s_hist[kEvictBins], s_coarse[kEvictCoarse];
+    __shared__ uint32_t s_warp[2][kEvictWarps];
+    __shared__ uint32_t s_found[2], s_total[2];
     pdl_wait_prior_grids();
     pdl_release_dependents();
     const Kv4View& c = a.c;
-    const int b = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t ranks = a.cluster, rank = ranks > 1 ? cluster_rank() : 0;
+    const int pair = blockIdx.x / a.cluster, b = pair / c.kv_heads, head = pair - b * c.kv_heads;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto barrier = [&]() { if (ranks > 1) cluster_barrier(); else __syncthreads(); };
     const int len = min(max(__ldcg(c.lens + b), 0), kv4_capacity(c));
     const int keep = min(len, a.budget);
     int32_t* kept = a.kept + (static_cast<size_t>(b) * c.kv_heads + head) * a.budget;
-    if (head == 0 && tid == 0) a.new_lens[b] = keep;
-    for (int i = keep + tid; i < a.budget; i += kSelectThreads) kept[i] = -1;
-    if (len <= a.budget) {
-        for (int i = tid; i < keep; i += kSelectThreads) kept[i] = i;
-        return;
+    if (rank == 0) {
+        if (head == 0 && tid == 0) a.new_lens[b] = keep;
+        for (int i = keep + tid; i < a.budget; i += kEvictThreads) kept[i] = -1;
     }
-    const int lo = a.sink, hi = len - a.recent;                 // the middle: sink + recent <= budget < len
-    const uint32_t want = static_cast<uint32_t>(a.budget - a.sink - a.recent);
-    auto key_at = [&](int i) -> uint32_t {
-        const int page = kv4_page(c, b, i);
+    const bool all_stay = len <= a.budget;
+    const int lo = all_stay ? len : a.sink, hi = all_stay ? len : len - a.recent;      // the middle: sink + recent <= budget < len
+    const uint32_t want = all_stay ? 0u : static_cast<uint32_t>(a.budget - a.sink - a.recent);
+    const int slice = (len / static_cast<int>(ranks) + 32) & ~31;                      // multiple of 32, times ranks above len - 1
+    const int s0 = min(slice * static_cast<int>(rank), len), s1 = min(s0 + slice, len);
+    const bool cached = slice <= kEvictCached;
+    auto page_at = [&](int i) { return kv4_page(c, b, i); };
+    auto key_from = [&](int i) -> uint32_t {
+        const int page = page_at(i);
         if (static_cast<unsigned>(page) >= static_cast<unsigned>(c.num_pages)) return 0u;
         return weight_key(__ldcg(c.key_weight + kv4_weight_index(c, page, head, i)));
     };
-    if (tid == 0) { s_prefix = 0; s_need = want; }
-    uint32_t prefix = 0, need = want;
-    for (int shift = 24; shift >= 0 && want > 0; shift -= 8) {
-        for (int i = tid; i < 256; i += kSelectThreads) s_hist[i] = 0;
-        __syncthreads();
-        for (int i = lo + tid; i < hi; i += kSelectThreads) {
-            const uint32_t k = key_at(i);
-            if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[(k >> shift) & 255u], 1u);
+    auto key_at = [&](int i) -> uint32_t { return cached ? s_keys[i - s0] : key_from(i); };
+    const int m0 = max(s0, lo), m1 = min(s1, hi);                                      // this CTA's share of the middle
+    uint32_t first = kEvictFirst, last = kEvictFirst + (static_cast<uint32_t>(kEvictBins) << kEvictFirstShift) - 1, need = want;
+    if (want > 0) {
+        if (cached) {
+            // quads lie in one page, and a page's weights are there whatever the length is
+            constexpr int kDeep = 2;
+            for (int i0 = s0 + 4 * tid; i0 < s1; i0 += kDeep * 4 * kEvictThreads) {
+                int page[kDeep];
+                float4 w[kDeep];
+#pragma unroll
+                for (int d = 0; d < kDeep; ++d) page[d] = i0 + d * 4 * kEvictThreads < s1 ? page_at(i0 + d * 4 * kEvictThreads) : -1;
+#pragma unroll
+                for (int d = 0; d < kDeep; ++d) {
+                    const float none = __int_as_float(0x7FC00000);
+                    w[d] = make_float4(none, none, none, none);
+                    if (static_cast<unsigned>(page[d]) < static_cast<unsigned>(c.num_pages))
+                        w[d] = __ldcg(reinterpret_cast<const float4*>(c.key_weight + kv4_weight_index(c, page[d], head, i0 + d * 4 * kEvictThreads)));
+                }
+#pragma unroll
+                for (int d = 0; d < kDeep; ++d)
+                    if (i0 + d * 4 * kEvictThreads < s1)
+                        *reinterpret_cast<uint4*>(s_keys + i0 + d * 4 * kEvictThreads - s0) =
+                            make_uint4(weight_key(w[d].x), weight_key(w[d].y), weight_key(w[d].z), weight_key(w[d].w));
+            }
         }
-        __syncthreads();
-        if (tid == 0) {
-            uint32_t above = 0;
-            int d = 255;
-            while (d > 0 && above + s_hist[d] < need) above += s_hist[d--];
-            s_prefix = prefix | (static_cast<uint32_t>(d) << shift);
-            s_need = need - above;
+        int shift = kEvictFirstShift;
+        bool clamp = true;                                       // the first round counts every key, the ends' bins all beyond them
+        while (true) {
+            for (int i = tid; i < kEvictBins; i += kEvictThreads) s_hist[i] = 0;
+            __syncthreads();
+            for (int i = m0 + tid; i < m1; i += kEvictThreads) {
+                uint32_t k = key_at(i);
+                if (clamp) k = min(max(k, first), last);
+                if (k >= first && k <= last) atomicAdd(&s_hist[(k - first) >> shift], 1u);
+            }
+            __syncthreads();
+            for (int k = warp; k < kEvictCoarse; k += kEvictWarps) {
+                const uint32_t n = __reduce_add_sync(0xFFFFFFFFu, s_hist[32 * k + lane]);
+                if (lane == 0) s_coarse[k] = n;
+            }
+            barrier();
+            if (warp == 0) {
+                // from the top: the group of 32 bins, then the bin, in which the count reaches `need`
+                uint32_t left = need, group = 0;
+#pragma unroll 1
+                for (int level = 0; level < 3; ++level) {        // the upper half of the groups, the lower, the bins of the group found
+                    const uint32_t* at = level < 2 ? &s_coarse[kEvictCoarse - 1 - 32 * level - lane] : &s_hist[32 * group + 31 - lane];
+                    uint32_t n = 0, more[kEvictMaxCluster];
+#pragma unroll
+                    for (uint32_t r = 0; r < kEvictMaxCluster; ++r) more[r] = r < ranks ? (ranks > 1 ? ld_cluster(at, r) : *at) : 0u;
+#pragma unroll
+                    for (uint32_t r = 0; r < kEvictMaxCluster; ++r) n += more[r];
+                    uint32_t upto = n;
+#pragma unroll
+                    for (int d = 1; d < 32; d <<= 1) {
+                        const uint32_t o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+                        if (lane >= d) upto += o;
+                    }
+                    const uint32_t reached = __ballot_sync(0xFFFFFFFFu, upto >= left);
+                    if (reached == 0) {                          // the upper half does not reach it
+                        left -= __shfl_sync(0xFFFFFFFFu, upto, 31);
+                        continue;
+                    }
+                    const int l = __ffs(reached) - 1;
+                    left -= __shfl_sync(0xFFFFFFFFu, upto - n, l);
+                    if (level < 2) {
+                        group = static_cast<uint32_t>(kEvictCoarse - 1 - 32 * level - l);
+                        level = 1;
+                    } else if (lane == 0) {
+                        s_found[0] = 32 * group + 31 - l;
+                        s_found[1] = left;
+                    }
+                }
+            }
+            barrier();                                           // and the histograms may be cleared
+            const uint32_t bin = s_found[0];
+            need = s_found[1];
+            const uint32_t base = first;
+            first = clamp && bin == 0 ? 0u : base + (bin << shift);
+            last = clamp && bin == kEvictBins - 1 ? ~0u : base + (bin << shift) + ((1u << shift) - 1u);
+            if (first == last) break;
+            const int bits = 32 - __clz(last - first);
+            shift = max(bits - 11, 0);
+            clamp = false;
+            __syncthreads();                                     // s_found has been read
         }
-        __syncthreads();
-        prefix = s_prefix;
-        need = s_need;
     }
-    // keys above `prefix` stay, and the first `need` of those equal to it
-    int base = 0, equal_base = 0;
-    for (int i0 = 0; i0 < len; i0 += kSelectThreads) {
-        const int i = i0 + tid;
-        bool stay = i < len && (i < lo || i >= hi), equal = false;
-        if (i >= lo && i < hi && want > 0) {
+    const uint32_t prefix = first;
+    // what stays: outside the middle, keys above `prefix`, and the first `need` of those equal to it
+    const int run = ((s1 - s0 + kEvictWarps - 1) / kEvictWarps + 31) & ~31;
+    const int r0 = min(s0 + warp * run, s1), r1 = min(r0 + run, s1);
+    uint32_t above = 0, equal = 0;
+    for (int i = r0 + lane; i < r1; i += 32) {
+        if (i < lo || i >= hi) {
+            ++above;
+        } else if (want > 0) {
             const uint32_t k = key_at(i);
-            stay = k > prefix;
-            equal = k == prefix;
+            above += k > prefix;
+            equal += k == prefix;
         }
-        const uint32_t eq = __ballot_sync(0xFFFFFFFFu, equal);
-        if (lane == 0) s_warp[0][warp] = __popc(eq);
-        __syncthreads();
-        int before = equal_base, total_eq = 0;
-        for (int w = 0; w < 32; ++w) {
-            if (w < warp) before += s_warp[0][w];
-            total_eq += s_warp[0][w];
-        }
-        before += __popc(eq & ((1u << lane) - 1u));
-        if (equal && before < static_cast<int>(need)) stay = true;
-        equal_base += total_eq;
-        const uint32_t st = __ballot_sync(0xFFFFFFFFu, stay);
-        if (lane == 0) s_warp[1][warp] = __popc(st);
-        __syncthreads();
-        int at = base, total = 0;
-        for (int w = 0; w < 32; ++w) {
-            if (w < warp) at += s_warp[1][w];
-            total += s_warp[1][w];
-        }
-        at += __popc(st & ((1u << lane) - 1u));
-        if (stay && at < a.budget) kept[at] = i;
-        base += total;
     }
-}
-
-// The kept rows to their fresh pages: a half-warp moves a position, two 64-byte rows, their parameters and the weight.
-__global__ void __launch_bounds__(256) kv4_move_kernel(const __grid_constant__ EvictArgs a) {
-    pdl_wait_prior_grids();
-    pdl_release_dependents();
-    const Kv4View& c = a.c;
-    const int b = blockIdx.z, head = blockIdx.y, hl = threadIdx.x & 15;
-    const int j = blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (j >= a.budget) return;
-    const int i = __ldcg(a.kept + (static_cast<size_t>(b) * c.kv_heads + head) * a.budget + j);
-    if (i < 0) return;
-    const int old_page = kv4_page(c, b, i), ps = 1 << c.page_shift;
-    const int new_page = __ldcg(a.dst_table + static_cast<size_t>(b) * a.dst_pages + (j >> c.page_shift));
-    const uint32_t* from = kv4_record_of_page(c, old_page, head);
-    uint32_t* to = kv4_record_of_page(c, new_page, head);
-    if (from == nullptr || to == nullptr) return;
-    const int s0 = i & (ps - 1), s1 = j & (ps - 1);
-    to[s1 * kKvRowWords + hl] = __ldcg(from + s0 * kKvRowWords + hl);
-    to[(ps + s1) * kKvRowWords + hl] = __ldcg(from + (ps + s0) * kKvRowWords + hl);
-    if (hl < 2) to[(32 + hl) * ps + s1] = __ldcg(from + (32 + hl) * ps + s0);
-    if (hl == 2) c.key_weight[kv4_weight_index(c, new_page, head, j)] = __ldcg(c.key_weight + kv4_weight_index(c, old_page, head, i));
+    above = __reduce_add_sync(0xFFFFFFFFu, above);
+    equal = __reduce_add_sync(0xFFFFFFFFu, equal);
+    if (lane == 0) { s_warp[0][warp] = above; s_warp[1][warp] = equal; }
+    __syncthreads();
+    const uint32_t wa = lane < kEvictWarps ? s_warp[0][lane] : 0u, we = lane < kEvictWarps ? s_warp[1][lane] : 0u;
+    if (tid < 32) {
+        const uint32_t ta = __reduce_add_sync(0xFFFFFFFFu, wa), te = __reduce_add_sync(0xFFFFFFFFu, we);
+        if (tid == 0) { s_total[0] = ta; s_total[1] = te; }
+    }
+    barrier();
+    uint32_t at_above = __reduce_add_sync(0xFFFFFFFFu, lane < warp ? wa : 0u), at_equal = __reduce_add_sync(0xFFFFFFFFu, lane < warp ? we : 0u);
+    for (uint32_t r = 0; r < rank; ++r) {
+        at_above += ld_cluster(&s_total[0], r);
+        at_equal += ld_cluster(&s_total[1], r);
+    }
+    for (int i0 = r0; i0 < r1; i0 += 32) {
+        const int i = i0 + lane;
+        bool more = false, same = false;
+        if (i < r1) {
+            if (i < lo || i >= hi) more = true;
+            else if (want > 0) {
+                const uint32_t k = key_at(i);
+                more = k > prefix;
+                same = k == prefix;
+            }
+        }
+        const uint32_t mm = __ballot_sync(0xFFFFFFFFu, more), ms = __ballot_sync(0xFFFFFFFFu, same);
+        const uint32_t below = (1u << lane) - 1u;
+        const uint32_t eq = at_equal + __popc(ms & below);       // equal keys in front of this one
+        const bool stay = more || (same && eq < need);
+        const int at = static_cast<int>(at_above + __popc(mm & below) + min(eq, need));
+        at_above += __popc(mm);
+        at_equal += __popc(ms);
+        if (stay && at < keep) __stcg(kept + at, i);
+    }
+    barrier();                                                   // the cluster's list is complete, and no CTA leaves while its totals are read
+    const int ps = 1 << c.page_shift, sub = lane & 7, part = sub >> 2;
+    constexpr int kMove = 4;
+    const int groups = static_cast<int>(ranks) * (kEvictThreads / 8);
+    for (int j0 = static_cast<int>(rank) * (kEvictThreads / 8) + (tid >> 3); j0 < keep; j0 += kMove * groups) {
+        int i[kMove], from[kMove], to[kMove];
+#pragma unroll
+        for (int u = 0; u < kMove; ++u) i[u] = j0 + u * groups < keep ? __ldcg(kept + j0 + u * groups) : -1;
+#pragma unroll
+        for (int u = 0; u < kMove; ++u) {
+            from[u] = to[u] = -1;
+            if (i[u] >= 0) {
+                from[u] = page_at(i[u]);
+                to[u] = __ldcg(a.dst_table + static_cast<size_t>(b) * a.dst_pages + ((j0 + u * groups) >> c.page_shift));
+            }
+        }
+        uint4 w[kMove];
+        uint32_t extra[kMove];
+#pragma unroll
+        for (int u = 0; u < kMove; ++u) {
+            // a page outside the pool moves nothing
+            if (static_cast<unsigned>(to[u]) >= static_cast<unsigned>(c.num_pages)) from[u] = -1;
+            const uint32_t* old = kv4_record_of_page(c, from[u], head);
+            w[u] = make_uint4(0, 0, 0, 0);
+            extra[u] = 0;
+            if (old != nullptr) {
+                const int slot = i[u] & (ps - 1);
+                w[u] = __ldcg(reinterpret_cast<const uint4*>(old + (part * ps + slot) * kKvRowWords) + (sub & 3));
+                if (sub < 2) extra[u] = __ldcg(old + (32 + sub) * ps + slot);
+                if (sub == 2) extra[u] = __ldcg(reinterpret_cast<const uint32_t*>(c.key_weight) + kv4_weight_index(c, from[u], head, i[u]));
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kMove; ++u) {
+            if (static_cast<unsigned>(from[u]) >= static_cast<unsigned>(c.num_pages)) continue;
+            uint32_t* fresh = kv4_record_of_page(c, to[u], head);
+            const int j = j0 + u * groups, slot = j & (ps - 1);
+            *(reinterpret_cast<uint4*>(fresh + (part * ps + slot) * kKvRowWords) + (sub & 3)) = w[u];
+            if (sub < 2) fresh[(32 + sub) * ps + slot] = extra[u];
+            if (sub == 2) reinterpret_cast<uint32_t*>(c.key_weight)[kv4_weight_index(c, to[u], head, j)] = extra[u];
+        }
+    }
 }
 
 }  // namespace
+
+// Four tokens a CTA where that leaves every SM enough CTAs: one token 4.9 us an append + read, either way; 4 prompts of 2100 to
+// 4100 tokens see the kernel.
+static int tokens_per_cta(int num_tokens, int blocks_per_token) { return static_cast<long long>(num_tokens) * blocks_per_token >= 4 * 148 * 4 ? 4 : 1; }
 
 int kv4_append(const Kv4View& c, const Kv4AppendArgs& x, cudaStream_t stream) {
     AppendArgs a{c, x.q, x.k, x.v, x.q_bias, x.k_bias, x.v_bias, x.q_out, x.positions, x.inv_freq, x.q_heads, x.q_stride, x.kv_stride, 0};
     const int rows = (x.q != nullptr ? x.q_heads : 0) + 2 * c.kv_heads;
     a.blocks_per_token = (rows + 15) / 16;
-    const long long blocks = static_cast<long long>(a.blocks_per_token) * c.num_tokens;
+    const int tok = tokens_per_cta(c.num_tokens, a.blocks_per_token);
+    const long long blocks = static_cast<long long>(a.blocks_per_token) * ((c.num_tokens + tok - 1) / tok);
     if (blocks > 0x7FFFFFFFll) return W4A16_ERR_TOO_LARGE;
-    return static_cast<int>(launch_kernel(kv4_append_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kAppendThreads), 0, stream, pdl_enabled(), a));
+    return static_cast<int>(launch_kernel(tok == 4 ? kv4_append_kernel<4> : kv4_append_kernel<1>, dim3(static_cast<unsigned>(blocks)), dim3(kAppendThreads), 0,
+                                          stream, pdl_enabled(), a));
 }
 
 int kv4_read(const Kv4View& c, __half* k_out, __half* v_out, cudaStream_t stream) {
-    const int per = (2 * c.kv_heads + 15) / 16;
-    const long long blocks = static_cast<long long>(per) * c.num_tokens;
+    const int per = (2 * c.kv_heads + 15) / 16, tok = tokens_per_cta(c.num_tokens, per);
+    const long long blocks = static_cast<long long>(per) * ((c.num_tokens + tok - 1) / tok);
     if (blocks > 0x7FFFFFFFll) return W4A16_ERR_TOO_LARGE;
-    return static_cast<int>(launch_kernel(kv4_read_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kAppendThreads), 0, stream, pdl_enabled(), c, k_out, v_out, per));
+    return static_cast<int>(launch_kernel(tok == 4 ? kv4_read_kernel<4> : kv4_read_kernel<1>, dim3(static_cast<unsigned>(blocks)), dim3(kAppendThreads), 0, stream,
+                                          pdl_enabled(), c, k_out, v_out, per));
+}
+
+int kv4_set_attributes() {
+    return static_cast<int>(cudaFuncSetAttribute(kv4_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvictCached * 4));
 }
 
 int kv4_evict(const Kv4View& c, const Kv4EvictArgs& x, cudaStream_t stream) {
-    EvictArgs a{c, x.dst_table, x.new_lens, x.kept, x.dst_pages, x.budget, x.sink, x.recent};
-    cudaError_t e = launch_kernel(kv4_select_kernel, dim3(c.num_seqs, c.kv_heads), dim3(kSelectThreads), 0, stream, pdl_enabled(), a);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    const dim3 grid((x.budget + 15) / 16, c.kv_heads, c.num_seqs);
-    return static_cast<int>(launch_kernel(kv4_move_kernel, grid, dim3(256), 0, stream, pdl_enabled(), a));
+    EvictArgs a{c, x.dst_table, x.new_lens, x.kept, x.dst_pages, x.budget, x.sink, x.recent, 1};
+    // CTAs of a (sequence, head): about 4096 positions each while all have an SM of their own (clusters of 8 fill no more than 96:
+    // 16 of them took 35 us for what 16 of 4 do in 26), and as many more as it takes to keep the keys in shared memory
+    const long long capacity = static_cast<long long>(c.max_pages) << c.page_shift, pairs = static_cast<long long>(c.num_seqs) * c.kv_heads;
+    while (a.cluster < kEvictMaxCluster && capacity > 4096ll * a.cluster && (pairs * a.cluster * 2 <= (a.cluster < 4 ? 148 : 96) || capacity > static_cast<long long>(kEvictCached) * a.cluster))
+        a.cluster *= 2;
+    if (pairs * a.cluster > 0x7FFFFFFFll) return W4A16_ERR_TOO_LARGE;
+    const long long slice = capacity / a.cluster + 64;
+    const size_t smem = static_cast<size_t>(slice < kEvictCached ? slice : kEvictCached) * 4;
+    return static_cast<int>(launch_kernel_cluster(kv4_evict_kernel, dim3(static_cast<unsigned>(pairs * a.cluster)), dim3(kEvictThreads), smem, stream, pdl_enabled(),
+                                                  dim3(a.cluster), a));
 }
 
 }  // namespace w4

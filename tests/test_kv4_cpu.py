@@ -48,7 +48,7 @@ REFUSED = [
     (dict(pages=None), -1, ALL), (dict(block_table=None), -1, ALL), (dict(seq_lens=None), -1, ALL), (dict(num_pages=0), -1, ALL),
     (dict(num_kv_heads=0), -1, ALL), (dict(num_seqs=0), -1, ALL), (dict(max_pages_per_seq=0), -1, ALL), (dict(num_tokens=0), -1, ALL),
     (dict(query_start=None), -1, ALL), (dict(page_size=8), -2, ALL), (dict(page_size=48), -2, ALL), (dict(page_size=8192), -2, ALL),
-    (dict(pages=P + 8), -3, ALL), (dict(seq_lens=P + 2), -3, ALL), (dict(num_seqs=70000), -5, ALL), (dict(num_tokens=1 << 25), -5, ALL),
+    (dict(pages=P + 8), -3, ALL), (dict(seq_lens=P + 2), -3, ALL), (dict(key_weight=P + 4), -3, ALL), (dict(num_seqs=70000), -5, ALL), (dict(num_tokens=1 << 25), -5, ALL),
     (dict(k=None), -1, {"append"}), (dict(v=None), -1, {"append"}), (dict(q_out=None), -1, {"append"}), (dict(q=None), -1, {"append", "attention", "weights"}),
     (dict(q=None, q_out=None, q_bias=P), -1, {"append", "attention", "weights"}), (dict(k=None, v=None), -1, {"append", "read"}),
     (dict(heads=0), -1, {"append", "attention", "weights"}), (dict(heads=11), -2, {"append", "attention", "weights"}),
