@@ -65,15 +65,25 @@ struct Place {
     int seq;
     long long in_seq;             // unit of the sequence
 };
-// Units of the whole batch, and the place of unit `per * index` with per = ceil(all / parts); false where there is none.
-// All threads of the CTA call it; `s_scan` holds a value a thread, and two more.
 template <int THREADS>
-__device__ __forceinline__ bool find_unit(const Kv4View& c, int group, int tile_rows, int index, int parts, long long* s_scan, long long* per, long long* all, Place* out) {
+struct FindScratch {
+    long long sums[THREADS / 32];
+    Place found;
+};
+__device__ __forceinline__ long long ceil_div(long long a, int b) {
+    // a division of 64 bits is a long subroutine in the way of the first load
+    return a >> 31 == 0 ? static_cast<long long>((static_cast<uint32_t>(a) + static_cast<uint32_t>(b) - 1u) / static_cast<uint32_t>(b)) : (a + b - 1) / b;
+}
+// Units of the whole batch, and the place of unit `per * index` with per = ceil(all / parts); false where there is none.
+// All threads of the CTA call it.  One round trip, for up to THREADS sequences.
+template <int THREADS>
+__device__ __forceinline__ bool find_unit(const Kv4View& c, int group, int tile_rows, int index, int parts, FindScratch<THREADS>& s, long long* per, long long* all, Place* out) {
     const int tid = threadIdx.x, lane = tid & 31, each = (c.num_seqs + THREADS - 1) / THREADS;
     const int b0 = min(tid * each, c.num_seqs), b1 = min(b0 + each, c.num_seqs);
     long long mine = 0;
+    SeqWork w{};
     for (int b = b0; b < b1; ++b) {
-        const SeqWork w = seq_work(c, b, group, tile_rows);
+        w = seq_work(c, b, group, tile_rows);
         mine += static_cast<long long>(w.tiles) * c.kv_heads * w.units;
     }
     long long upto = mine;
@@ -82,36 +92,33 @@ __device__ __forceinline__ bool find_unit(const Kv4View& c, int group, int tile_
         const long long o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
         if (lane >= d) upto += o;
     }
-    if (lane == 31) s_scan[tid >> 5] = upto;
+    if (lane == 31) s.sums[tid >> 5] = upto;
     __syncthreads();
     long long total = 0, before = 0;
 #pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
-        if (w == tid >> 5) before = total;
-        total += s_scan[w];
+    for (int i = 0; i < THREADS / 32; ++i) {
+        if (i == tid >> 5) before = total;
+        total += s.sums[i];
     }
     *all = total;
-    *per = (total + parts - 1) / parts;
+    *per = ceil_div(total, parts);
     const long long want = *per * index;
     if (want >= total) return false;
     upto += before;
     if (upto > want && upto - mine <= want) {        // the sequence is one of this thread's
         long long at = upto - mine;
         for (int b = b0; b < b1; ++b) {
-            const SeqWork w = seq_work(c, b, group, tile_rows);
+            if (each > 1) w = seq_work(c, b, group, tile_rows);
             const long long units = static_cast<long long>(w.tiles) * c.kv_heads * w.units;
             if (want < at + units) {
-                s_scan[THREADS / 32] = b;
-                s_scan[THREADS / 32 + 1] = want - at;
+                s.found = Place{w, b, want - at};
                 break;
             }
             at += units;
         }
     }
     __syncthreads();
-    out->seq = static_cast<int>(s_scan[THREADS / 32]);
-    out->in_seq = s_scan[THREADS / 32 + 1];
-    out->w = seq_work(c, out->seq, group, tile_rows);
+    *out = s.found;
     return true;
 }
 
@@ -120,41 +127,45 @@ __device__ __forceinline__ size_t out_row(const SeqWork& w, int heads, int group
     return static_cast<size_t>(w.first + row / group) * (static_cast<size_t>(heads) * group) + head * group + row % group;
 }
 
-// What a lane holds of 16 positions: rows g and g + 8 of the keys, four positions' share of the values.
-struct KvRegs {
-    uint4 k[2];
-    uint2 v[4];
-    uint32_t kp[2], vp[2];
-    bool ok;
-};
-// Where a lane's pieces of a record lie.
-struct KvOffsets {
+// A warp's 16 positions in shared memory, copied there by itself (cp.async, 5 a lane) several steps ahead: what is in flight
+// is what bounds this kernel (with one step ahead, in registers, 64 sequences of up to 8190 positions took 115 us), and registers
+// are short.  Chunks of 16 bytes are placed so that no access meets another in a bank:
+//   keys: the row of A number r holds position key_position(r), which makes the columns of p^T that the transposition leaves with
+//         a lane the positions t, 4 + t, 8 + t and 12 + t; rows lie in order of r;
+//   values: a lane reads 8 bytes of the rows t, 4 + t, ...; rows 2 and 3 of four have their halves swapped.
+constexpr int kStageBytes = kKvTile * 136, kStages = 4;
+constexpr int kStageValues = 1024, kStageKeyParams = 2048, kStageValueParams = 2112;
+__device__ __forceinline__ int key_position(int r) { return ((r >> 1) & 3) + 4 * (r & 1) + (r & 8); }
+__device__ __forceinline__ int key_row(int position) { return 2 * (position & 3) + ((position >> 2) & 1) + (position & 8); }
+
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+struct TileCopy {
     const char* head;             // the head's record of page 0
     size_t page;                  // bytes from page to page
-    int ps, key, value, param;    // the lane's first key and value row, and parameters, in bytes from a row's place
+    int ps;
+    uint32_t key_to, value_to;    // where the lane's first chunks go; its second ones lie 512 bytes on, as in the record
+
+    __device__ __forceinline__ TileCopy(const Kv4View& c, int head_no, int lane) {
+        const size_t record = static_cast<size_t>(kKvSlotWords * 4) << c.page_shift;
+        head = reinterpret_cast<const char*>(c.pages) + head_no * record;
+        page = record * c.kv_heads;
+        ps = 1 << c.page_shift;
+        const int row = lane >> 2, chunk = lane & 3;          // and row + 8
+        key_to = static_cast<uint32_t>(key_row(row) * 64 + chunk * 16);
+        value_to = static_cast<uint32_t>(kStageValues + row * 64 + (chunk ^ (row & 2)) * 16);
+    }
+    __device__ __forceinline__ void issue(uint32_t stage, int page_no, int at, int lane) const {
+        const int s = at & (ps - 1);
+        const char* rows = head + page_no * page + 64 * s + 16 * lane;
+        cp_async_16(stage + key_to, rows);
+        cp_async_16(stage + key_to + 512, rows + 512);
+        cp_async_16(stage + value_to, rows + 64 * ps);
+        cp_async_16(stage + value_to + 512, rows + 64 * ps + 512);
+        if (lane < 8) cp_async_16(stage + kStageKeyParams + 16 * lane, head + page_no * page + 128 * ps + 4 * s + 16 * (lane & 3) + (lane >> 2) * 4 * ps);
+    }
 };
-__device__ __forceinline__ KvOffsets kv_offsets(const Kv4View& c, int head, int g, int t) {
-    const int ps = 1 << c.page_shift;
-    const size_t record = static_cast<size_t>(kKvSlotWords * 4) << c.page_shift;
-    return {reinterpret_cast<const char*>(c.pages) + head * record, record * c.kv_heads, ps, 64 * g + 16 * t, 64 * ps + 128 * t + 8 * g, 128 * ps + 4 * g};
-}
-__device__ __forceinline__ void load_tile(const Kv4View& c, const KvOffsets& f, int page, int at, KvRegs& r) {
-    r.ok = static_cast<unsigned>(page) < static_cast<unsigned>(c.num_pages);
-    if (!r.ok) return;
-    const int s = at & (f.ps - 1);
-    const char* rows = f.head + page * f.page + 64 * s;
-    const char* keys = rows + f.key;
-    const char* values = rows + f.value;
-    const char* params = rows + (f.param - 60 * s);
-    r.k[0] = __ldcg(reinterpret_cast<const uint4*>(keys));
-    r.k[1] = __ldcg(reinterpret_cast<const uint4*>(keys + 512));
-    r.kp[0] = __ldcg(reinterpret_cast<const uint32_t*>(params));
-    r.kp[1] = __ldcg(reinterpret_cast<const uint32_t*>(params + 32));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r.v[i] = __ldcg(reinterpret_cast<const uint2*>(values + 64 * (i & 1) + 512 * (i >> 1)));
-    r.vp[0] = __ldcg(reinterpret_cast<const uint32_t*>(params + 4 * f.ps));
-    r.vp[1] = __ldcg(reinterpret_cast<const uint32_t*>(params + 4 * f.ps + 32));
-}
 
 // B fragments of eight query rows for the eight k steps: steps 2 j and 2 j + 1 take the elements of word 4 t + j in the order in
 // which the code conversion gives them, 0 2 1 3 and 4 6 5 7.
@@ -203,16 +214,18 @@ __device__ __forceinline__ void store_row(const Kv4AttentionArgs& a, size_t row,
 template <int NT, bool F32>
 __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_kernel(const __grid_constant__ Kv4AttentionArgs a) {
     constexpr int R = 8 * NT, kPitch = kKvDim + 4;
-    __shared__ float s_o[kAttnWarps][R][kPitch];
+    __shared__ __align__(128) uint8_t s_ring[kAttnWarps][kStages * kStageBytes];     // and, behind the last position, the warps' sums
     __shared__ float2 s_ml[kAttnWarps][R];
-    __shared__ long long s_scan[kAttnWarps + 2];
+    __shared__ FindScratch<kAttnThreads> s_find;
+    static_assert(R * kPitch * 4 <= kStages * kStageBytes);
+    auto s_o = [&](int w, int r, int d) -> float& { return reinterpret_cast<float*>(s_ring[w])[r * kPitch + d]; };
     pdl_wait_prior_grids();
     pdl_release_dependents();
     const Kv4View& c = a.c;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     long long per, all;
     Place pl;
-    if (!find_unit<kAttnThreads>(c, a.group, R, blockIdx.x, gridDim.x, s_scan, &per, &all, &pl)) return;
+    if (!find_unit<kAttnThreads>(c, a.group, R, blockIdx.x, gridDim.x, s_find, &per, &all, &pl)) return;
     long long left = min(per, all - per * blockIdx.x);
     for (bool first_part = true; left > 0; first_part = false) {
     while (pl.in_seq >= static_cast<long long>(pl.w.tiles) * c.kv_heads * pl.w.units) {      // past the sequence: the next one with work
@@ -265,9 +278,21 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
 
     float mu[NT][2];                                        // m, or 0 where nothing has been seen
     for (int n = 0; n < NT; ++n) mu[n][0] = mu[n][1] = 0.0f;
-    const KvOffsets f = kv_offsets(c, head, g, t);
-    auto take = [&](const KvRegs& r, int at) {
-        if (!r.ok) return;
+    const TileCopy copy(c, head, lane);
+    const uint8_t* ring = s_ring[warp];
+    const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+    const int pos = key_position(g);                        // positions of rows g and g + 8 of A: pos and pos + 8
+    const int value_from = kStageValues + 64 * t + ((8 * g) ^ (16 * (t & 2)));
+    auto take = [&](const uint8_t* st, int at) {
+        struct { uint4 k[2]; uint2 v[4]; uint32_t kp[2], vp[2]; } r;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            r.k[i] = *reinterpret_cast<const uint4*>(st + 512 * i + 64 * g + 16 * t);
+            r.kp[i] = *reinterpret_cast<const uint32_t*>(st + kStageKeyParams + 4 * pos + 32 * i);
+            r.vp[i] = *reinterpret_cast<const uint32_t*>(st + kStageValueParams + 4 * pos + 32 * i);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.v[i] = *reinterpret_cast<const uint2*>(st + value_from + 256 * i);
         float even[NT][4] = {}, s[NT][4] = {};
         const uint32_t kw0[4] = {r.k[0].x, r.k[0].y, r.k[0].z, r.k[0].w}, kw1[4] = {r.k[1].x, r.k[1].y, r.k[1].z, r.k[1].w};
 #pragma unroll
@@ -302,10 +327,10 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (at + g + 8 * (e >> 1) >= limit[n][e & 1]) s[n][e] = -INFINITY;
+                    if (at + pos + 8 * (e >> 1) >= limit[n][e & 1]) s[n][e] = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                if (at + g + 8 * i >= k1) vs[i] = vz[i] = 0.0f;
+                if (at + pos + 8 * i >= k1) vs[i] = vz[i] = 0.0f;
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -353,7 +378,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
                 l[n][e & 1] += p;
                 x[e] = p * vs[e >> 1];
                 float z = p * vz[e >> 1];
-                if (cut && at + g + 8 * (e >> 1) >= limit[n][e & 1]) x[e] = z = 0.0f;   // whatever the row holds
+                if (cut && at + pos + 8 * (e >> 1) >= limit[n][e & 1]) x[e] = z = 0.0f;   // whatever the row holds
                 zacc[n][e & 1] += z;
             }
 #pragma unroll
@@ -387,27 +412,31 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
         }
     };
 
-    // 16 positions in use, the next 16 on their way, the page number of those behind them too
-    int at = k0 + warp * kKvTile;
-    KvRegs r0, r1;
-    r0.ok = r1.ok = false;
-    int next_page = -1;
-    if (at < k1) load_tile(c, f, kv4_page(c, q.seq, at), at, r0);
-    if (at + kUnit < k1) next_page = kv4_page(c, q.seq, at + kUnit);
-    auto ahead = [&](KvRegs& r) {
-        r.ok = false;
-        if (at + kUnit < k1) load_tile(c, f, next_page, at + kUnit, r);
-        if (at + 2 * kUnit < k1) next_page = kv4_page(c, q.seq, at + 2 * kUnit);
+    // a page number is fetched one step before the copies that need it; a page outside the pool is a step without copies
+    const int first_at = k0 + warp * kKvTile, steps = first_at < k1 ? (k1 - first_at + kUnit - 1) / kUnit : 0;
+    uint32_t there = 0;                                     // bit i: the step i from now has rows
+    int next_page = steps > 0 ? kv4_page(c, q.seq, first_at) : -1;
+    auto ahead = [&](int step) {
+        const bool ok = step < steps && static_cast<unsigned>(next_page) < static_cast<unsigned>(c.num_pages);
+        if (ok) copy.issue(ring_at + static_cast<uint32_t>(step % kStages) * kStageBytes, next_page, first_at + step * kUnit, lane);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (step + 1 < steps) next_page = kv4_page(c, q.seq, first_at + (step + 1) * kUnit);
+        there |= (ok ? 1u : 0u) << (kStages - 1);
     };
-    while (at < k1) {
-        ahead(r1);
-        take(r0, at);
-        at += kUnit;
-        if (at >= k1) break;
-        ahead(r0);
-        take(r1, at);
-        at += kUnit;
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+        ahead(i);
+        there >>= 1;
     }
+    for (int i = 0; i < steps; ++i) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        __syncwarp();                                       // every lane's copies are there, and the slot of the step before has been read
+        ahead(i + kStages - 1);
+        if (there & 1u) take(ring + (i % kStages) * kStageBytes, first_at + i * kUnit);
+        there >>= 1;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
 
     // the warps' parts into shared memory: a lane has dimensions 16 g .. 16 g + 15 of queries 2 t and 2 t + 1
     const float undo = pw == 0.0f ? 1.0f : 1.0f / pw;
@@ -426,8 +455,8 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
             if (g == 0) s_ml[warp][r] = make_float2(m[n][e], ls);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                s_o[warp][r][16 * g + kElement[i]] = fmaf(o[n][i][e], undo * kv4_value_undo(i), zs);
-                s_o[warp][r][16 * g + 8 + kElement[i]] = fmaf(o[n][i][e + 2], undo * kv4_value_undo(i), zs);
+                s_o(warp, r, 16 * g + kElement[i]) = fmaf(o[n][i][e], undo * kv4_value_undo(i), zs);
+                s_o(warp, r, 16 * g + 8 + kElement[i]) = fmaf(o[n][i][e + 2], undo * kv4_value_undo(i), zs);
             }
         }
     __syncthreads();
@@ -443,7 +472,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
         }
         float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int w = 0; w < kAttnWarps; ++w) add_part(x, sum, *reinterpret_cast<const float4*>(&s_o[w][r][4 * lane]), ml[w], top);
+        for (int w = 0; w < kAttnWarps; ++w) add_part(x, sum, *reinterpret_cast<const float4*>(&s_o(w, r, 4 * lane)), ml[w], top);
         if (whole) {
             store_row<F32>(a, out_row(pl.w, c.kv_heads, a.group, head, q.row0 + r), x, top, sum);
         } else {
@@ -456,11 +485,12 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
 }
 
 // The parts of a (tile, head) joined.  A CTA stands at the boundary of the CTAs blockIdx.x and blockIdx.x + 1 of the launch above, and
-// works if that is the first boundary inside a (tile, head); blockIdx.y is a row of the tile.
+// works if that is the first boundary inside a (tile, head).  SPLIT: there are few (tile, head), so of many parts each, and a CTA
+// joins one row (blockIdx.y), its warps sharing the parts; else a warp joins the rows of its number.
 constexpr int kJoinWarps = 8;
-template <bool F32>
+template <bool F32, bool SPLIT>
 __global__ void __launch_bounds__(32 * kJoinWarps) kv4_attention_join_kernel(const __grid_constant__ Kv4AttentionArgs a, int tile_rows, int parts) {
-    __shared__ long long s_scan[kJoinWarps + 2];
+    __shared__ FindScratch<32 * kJoinWarps> s_find;
     __shared__ float4 s_x[kJoinWarps][32];
     __shared__ float2 s_ml[kJoinWarps];
     pdl_wait_prior_grids();
@@ -470,54 +500,58 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv4_attention_join_kernel(con
     long long per, all;
     Place pl;
     const int boundary = blockIdx.x + 1;
-    if (!find_unit<32 * kJoinWarps>(c, a.group, tile_rows, boundary, parts, s_scan, &per, &all, &pl)) return;
+    if (!find_unit<32 * kJoinWarps>(c, a.group, tile_rows, boundary, parts, s_find, &per, &all, &pl)) return;
     const int tile_head = static_cast<int>(pl.in_seq / pl.w.units);
     const long long unit0 = per * boundary - (pl.in_seq - static_cast<long long>(tile_head) * pl.w.units);
-    const int c0 = static_cast<int>(unit0 / per), c1 = static_cast<int>((unit0 + pl.w.units - 1) / per);
-    const int head = tile_head % c.kv_heads, row = tile_head / c.kv_heads * tile_rows + blockIdx.y;
-    if (unit0 == per * boundary || c0 != boundary - 1 || row >= pl.w.n * a.group) return;
-    // part of CTA i: its first, unless the (tile, head) begins inside of it
-    auto part_row = [&](int i) { return (2 * static_cast<size_t>(i) + (i == c0 && unit0 != per * c0 ? 1 : 0)) * tile_rows + blockIdx.y; };
-    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float top = -INFINITY, sum = 0.0f;
-    constexpr int kDeep = 4;
-    for (int i0 = c0 + warp; i0 <= c1; i0 += kJoinWarps * kDeep) {
-        float4 p[kDeep];
-        float2 ml[kDeep];
-        float fresh = top;
+    if (unit0 == per * boundary || unit0 < per * (boundary - 1)) return;
+    const int c0 = boundary - 1, c1 = static_cast<int>((unit0 + pl.w.units - 1) / per);
+    const int head = tile_head % c.kv_heads, row0 = tile_head / c.kv_heads * tile_rows, rows = min(tile_rows, pl.w.n * a.group - row0);
+    constexpr int kDeep = 4, kStride = SPLIT ? kJoinWarps : 1;
+    for (int r = SPLIT ? blockIdx.y : warp; r < rows; r += SPLIT ? tile_rows : kJoinWarps) {
+        // part of CTA i: its first, unless the (tile, head) begins inside of it
+        auto part_row = [&](int i) { return (2 * static_cast<size_t>(i) + (i == c0 && unit0 != per * c0 ? 1 : 0)) * tile_rows + r; };
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float top = -INFINITY, sum = 0.0f;
+        for (int i0 = c0 + (SPLIT ? warp : 0); i0 <= c1; i0 += kStride * kDeep) {
+            float4 p[kDeep];
+            float2 ml[kDeep];
+            float fresh = top;
 #pragma unroll
-        for (int d = 0; d < kDeep; ++d) {
-            const int i = i0 + d * kJoinWarps;
-            ml[d] = make_float2(-INFINITY, 0.0f);
-            p[d] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (i <= c1) {
-                ml[d] = __ldcg(a.part_ml + part_row(i));
-                p[d] = __ldcg(reinterpret_cast<const float4*>(a.part_o + part_row(i) * kKvDim) + lane);
+            for (int d = 0; d < kDeep; ++d) {
+                const int i = i0 + d * kStride;
+                ml[d] = make_float2(-INFINITY, 0.0f);
+                p[d] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (i <= c1) {
+                    ml[d] = __ldcg(a.part_ml + part_row(i));
+                    p[d] = __ldcg(reinterpret_cast<const float4*>(a.part_o + part_row(i) * kKvDim) + lane);
+                }
             }
+#pragma unroll
+            for (int d = 0; d < kDeep; ++d) fresh = fmaxf(fresh, ml[d].x);
+            const float4 old = x;
+            const float2 old_ml = make_float2(top, sum);
+            x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            sum = 0.0f;
+            top = fresh;
+            add_part(x, sum, old, old_ml, top);
+#pragma unroll
+            for (int d = 0; d < kDeep; ++d) add_part(x, sum, p[d], ml[d], top);
         }
+        if constexpr (SPLIT) {
+            s_x[warp][lane] = x;
+            if (lane == 0) s_ml[warp] = make_float2(top, sum);
+            __syncthreads();
+            if (warp != 0) return;
+            top = -INFINITY;
+            sum = 0.0f;
+            x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int d = 0; d < kDeep; ++d) fresh = fmaxf(fresh, ml[d].x);
-        const float4 old = x;
-        const float2 old_ml = make_float2(top, sum);
-        x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        sum = 0.0f;
-        top = fresh;
-        add_part(x, sum, old, old_ml, top);
+            for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, s_ml[w].x);
 #pragma unroll
-        for (int d = 0; d < kDeep; ++d) add_part(x, sum, p[d], ml[d], top);
+            for (int w = 0; w < kJoinWarps; ++w) add_part(x, sum, s_x[w][lane], s_ml[w], top);
+        }
+        store_row<F32>(a, out_row(pl.w, c.kv_heads, a.group, head, row0 + r), x, top, sum);
     }
-    s_x[warp][lane] = x;
-    if (lane == 0) s_ml[warp] = make_float2(top, sum);
-    __syncthreads();
-    if (warp != 0) return;
-    top = -INFINITY;
-    sum = 0.0f;
-    x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, s_ml[w].x);
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) add_part(x, sum, s_x[w][lane], s_ml[w], top);
-    store_row<F32>(a, out_row(pl.w, c.kv_heads, a.group, head, row), x, top, sum);
 }
 
 // ---- attention weight of the cached positions ------------------------------------------------------------------
@@ -636,10 +670,12 @@ __global__ void __launch_bounds__(kAttnThreads) kv4_key_weight_kernel(const __gr
 
 Kv4AttentionPlan kv4_attention_plan(int num_tokens, int num_seqs, int q_heads, int kv_heads) {
     Kv4AttentionPlan p;
-    const long long rows = static_cast<long long>(q_heads / kv_heads) * num_tokens;
+    const long long group = q_heads / kv_heads, rows = group * num_tokens;
     p.nt = rows > 8ll * num_seqs ? 2 : 1;
     p.ctas = 148 * (p.nt == 1 ? 4 : 2);
-    const long long parts = 2ll * p.ctas * 8 * p.nt;
+    const long long R = 8 * p.nt, by_token = num_tokens * ((group + R - 1) / R), by_rows = rows / R + num_seqs;
+    p.tile_heads = (by_token < by_rows ? by_token : by_rows) * kv_heads;
+    const long long parts = 2ll * p.ctas * R;
     p.ml_offset = parts * kKvDim * 4;
     p.bytes = p.ml_offset + parts * 8;
     return p;
@@ -652,10 +688,15 @@ int kv4_attention(Kv4AttentionArgs a, int q_heads, bool f32, void* workspace, cu
     a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.ml_offset);
     auto kernel = p.nt == 1 ? (f32 ? kv4_attention_kernel<1, true> : kv4_attention_kernel<1, false>)
                             : (f32 ? kv4_attention_kernel<2, true> : kv4_attention_kernel<2, false>);
-    cudaError_t e = launch_kernel(kernel, dim3(p.ctas), dim3(kAttnThreads), 0, stream, pdl_enabled(), a);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    return static_cast<int>(launch_kernel(f32 ? kv4_attention_join_kernel<true> : kv4_attention_join_kernel<false>, dim3(p.ctas - 1, 8 * p.nt),
-                                          dim3(32 * kJoinWarps), 0, stream, pdl_enabled(), a, 8 * p.nt, p.ctas));
+    // no more CTAs than there can be units
+    const long long most = p.tile_heads * (((static_cast<long long>(c.max_pages) << c.page_shift) + kUnit - 1) / kUnit);
+    const int ctas = static_cast<int>(most < p.ctas ? most : p.ctas);
+    cudaError_t e = launch_kernel(kernel, dim3(ctas), dim3(kAttnThreads), 0, stream, pdl_enabled(), a);
+    if (e != cudaSuccess || ctas == 1) return static_cast<int>(e);
+    const bool split = p.tile_heads * 8 <= ctas;     // more than eight parts each
+    auto join = split ? (f32 ? kv4_attention_join_kernel<true, true> : kv4_attention_join_kernel<false, true>)
+                      : (f32 ? kv4_attention_join_kernel<true, false> : kv4_attention_join_kernel<false, false>);
+    return static_cast<int>(launch_kernel(join, dim3(ctas - 1, split ? 8 * p.nt : 1), dim3(32 * kJoinWarps), 0, stream, pdl_enabled(), a, 8 * p.nt, ctas));
 }
 
 int kv4_add_key_weights(const Kv4WeightArgs& a, cudaStream_t stream) {

@@ -25,7 +25,7 @@ struct Kv4WeightArgs {
 // How a call is cut; a function of its sizes alone, so that the workspace can be sized without a device.
 struct Kv4AttentionPlan {
     int nt, ctas;
-    long long ml_offset, bytes;
+    long long tile_heads, ml_offset, bytes;
 };
 Kv4AttentionPlan kv4_attention_plan(int num_tokens, int num_seqs, int q_heads, int kv_heads);
 int kv4_attention(Kv4AttentionArgs a, int q_heads, bool f32, void* workspace, cudaStream_t stream);
