@@ -142,38 +142,40 @@ __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 struct TileCopy {
-    const char* head;             // the head's record of page 0
-    size_t page;                  // bytes from page to page
-    int ps;
-    uint32_t key_to, value_to;    // where the lane's first chunks go; its second ones lie 512 bytes on, as in the record
+    const char *keys, *values, *params;      // the lane's first chunk of each in the head's record of page 0
+    size_t page;                             // bytes from page to page
+    int in_page;                             // positions of a page, less one
+    uint32_t key_to, value_to, param_to;     // where they go; the second ones lie 512 bytes on, as in the record
 
-    __device__ __forceinline__ TileCopy(const Kv4View& c, int head_no, int lane) {
+    __device__ __forceinline__ TileCopy(const Kv4View& c, int head_no, int lane, uint32_t ring) {
         const size_t record = static_cast<size_t>(kKvSlotWords * 4) << c.page_shift;
-        head = reinterpret_cast<const char*>(c.pages) + head_no * record;
+        const int ps = 1 << c.page_shift;
+        const char* head = reinterpret_cast<const char*>(c.pages) + head_no * record;
+        keys = head + 16 * lane;
+        values = keys + 64 * ps;
+        params = head + 128 * ps + 16 * (lane & 3) + (lane & 4) * ps;
         page = record * c.kv_heads;
-        ps = 1 << c.page_shift;
+        in_page = ps - 1;
         const int row = lane >> 2, chunk = lane & 3;          // and row + 8
-        key_to = static_cast<uint32_t>(key_row(row) * 64 + chunk * 16);
-        value_to = static_cast<uint32_t>(kStageValues + row * 64 + (chunk ^ (row & 2)) * 16);
+        key_to = ring + static_cast<uint32_t>(key_row(row) * 64 + chunk * 16);
+        value_to = ring + static_cast<uint32_t>(kStageValues + row * 64 + (chunk ^ (row & 2)) * 16);
+        param_to = ring + static_cast<uint32_t>(kStageKeyParams + 16 * lane);
     }
     __device__ __forceinline__ void issue(uint32_t stage, int page_no, int at, int lane) const {
-        const int s = at & (ps - 1);
-        const char* rows = head + page_no * page + 64 * s + 16 * lane;
-        cp_async_16(stage + key_to, rows);
-        cp_async_16(stage + key_to + 512, rows + 512);
-        cp_async_16(stage + value_to, rows + 64 * ps);
-        cp_async_16(stage + value_to + 512, rows + 64 * ps + 512);
-        if (lane < 8) cp_async_16(stage + kStageKeyParams + 16 * lane, head + page_no * page + 128 * ps + 4 * s + 16 * (lane & 3) + (lane >> 2) * 4 * ps);
+        const int s = at & in_page;
+        const size_t rows = page_no * page + 64 * s;
+        cp_async_16(key_to + stage, keys + rows);
+        cp_async_16(key_to + stage + 512, keys + rows + 512);
+        cp_async_16(value_to + stage, values + rows);
+        cp_async_16(value_to + stage + 512, values + rows + 512);
+        if (lane < 8) cp_async_16(param_to + stage, params + rows - 60 * s);
     }
 };
 
 // B fragments of eight query rows for the eight k steps: steps 2 j and 2 j + 1 take the elements of word 4 t + j in the order in
 // which the code conversion gives them, 0 2 1 3 and 4 6 5 7.
-__device__ __forceinline__ void query_words(const uint4& w, uint32_t* b) {
-    b[0] = __byte_perm(w.x, w.y, 0x5410);
-    b[1] = __byte_perm(w.x, w.y, 0x7632);
-    b[2] = __byte_perm(w.z, w.w, 0x5410);
-    b[3] = __byte_perm(w.z, w.w, 0x7632);
+__device__ __forceinline__ uint4 query_words(const uint4& w) {
+    return make_uint4(__byte_perm(w.x, w.y, 0x5410), __byte_perm(w.x, w.y, 0x7632), __byte_perm(w.z, w.w, 0x5410), __byte_perm(w.z, w.w, 0x7632));
 }
 __device__ __forceinline__ float sum_half8(const uint4& w) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -215,6 +217,7 @@ template <int NT, bool F32>
 __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_kernel(const __grid_constant__ Kv4AttentionArgs a) {
     constexpr int R = 8 * NT, kPitch = kKvDim + 4;
     __shared__ __align__(128) uint8_t s_ring[kAttnWarps][kStages * kStageBytes];     // and, behind the last position, the warps' sums
+    __shared__ uint4 s_q[NT][4][32];         // the queries as B fragments; in registers they would leave too few for the rest
     __shared__ float2 s_ml[kAttnWarps][R];
     __shared__ FindScratch<kAttnThreads> s_find;
     static_assert(R * kPitch * 4 <= kStages * kStageBytes);
@@ -243,7 +246,6 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
     const int k0 = unit0 * kUnit, k1 = min(k0 + units * kUnit, seen);
 
     // queries: B fragments of rows g (+ 8), and for the lane's columns 2 t, 2 t + 1 the sum of q and how far the row sees
-    uint32_t qb[NT][16];
     float qsum[NT][2];
     int limit[NT][2];
     const float to_log2 = a.scale * kLog2e;
@@ -259,7 +261,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
                 w = __ldcg(reinterpret_cast<const uint4*>(a.q + static_cast<size_t>(token) * a.q_stride + h * kKvDim + 32 * t + 8 * j));
             }
             s += sum_half8(w);
-            query_words(w, &qb[n][4 * j]);
+            if (j == warp) s_q[n][j][lane] = query_words(w);
         }
         s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
         s += __shfl_xor_sync(0xFFFFFFFFu, s, 2);
@@ -270,6 +272,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
         }
     }
     const int all_see = q.past + q.row0 / a.group + 1;      // positions that every row of the tile sees
+    __syncthreads();
 
     float o[NT][8][4] = {}, m[NT][2], l[NT][2] = {}, zacc[NT][2] = {};
 #pragma unroll
@@ -278,12 +281,13 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
 
     float mu[NT][2];                                        // m, or 0 where nothing has been seen
     for (int n = 0; n < NT; ++n) mu[n][0] = mu[n][1] = 0.0f;
-    const TileCopy copy(c, head, lane);
     const uint8_t* ring = s_ring[warp];
-    const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+    const TileCopy copy(c, head, lane, static_cast<uint32_t>(__cvta_generic_to_shared(ring)));
+    const int32_t* table = c.table + static_cast<size_t>(q.seq) * c.max_pages;
     const int pos = key_position(g);                        // positions of rows g and g + 8 of A: pos and pos + 8
     const int value_from = kStageValues + 64 * t + ((8 * g) ^ (16 * (t & 2)));
-    auto take = [&](const uint8_t* st, int at) {
+    // CUT: some row does not see some of these positions
+    auto take = [&]<bool CUT>(const uint8_t* st, int at) {
         struct { uint4 k[2]; uint2 v[4]; uint32_t kp[2], vp[2]; } r;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -303,8 +307,9 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
             const uint32_t a0[4] = {lo[0], hi[0], lo[2], hi[2]}, a1[4] = {lo[1], hi[1], lo[3], hi[3]};
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                mma_16816(even[n], a0, qb[n][4 * j], qb[n][4 * j + 1]);
-                mma_16816(s[n], a1, qb[n][4 * j + 2], qb[n][4 * j + 3]);
+                const uint4 b = s_q[n][j][lane];
+                mma_16816(even[n], a0, b.x, b.y);
+                mma_16816(s[n], a1, b.z, b.w);
             }
         }
         float ks[2], kz[2], vs[2], vz[2];
@@ -316,13 +321,12 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
             vs[i] = kv4_scale(r.vp[i]);
             vz[i] = fmaf(-0.5f, vs[i], kv4_zero(r.vp[i]));  // codes are taken around 7.5
         }
-        const bool cut = at + kKvTile > all_see;            // some row does not see some of these positions
         bool above = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[n][e] = fmaf(kv4_key_sum(even[n][e], s[n][e]), ks[e >> 1], kz[e >> 1] * qsum[n][e & 1]);
-        if (cut) {
+        if constexpr (CUT) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -378,7 +382,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
                 l[n][e & 1] += p;
                 x[e] = p * vs[e >> 1];
                 float z = p * vz[e >> 1];
-                if (cut && at + pos + 8 * (e >> 1) >= limit[n][e & 1]) x[e] = z = 0.0f;   // whatever the row holds
+                if (CUT && at + pos + 8 * (e >> 1) >= limit[n][e & 1]) x[e] = z = 0.0f;   // whatever the row holds
                 zacc[n][e & 1] += z;
             }
 #pragma unroll
@@ -415,12 +419,12 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
     // a page number is fetched one step before the copies that need it; a page outside the pool is a step without copies
     const int first_at = k0 + warp * kKvTile, steps = first_at < k1 ? (k1 - first_at + kUnit - 1) / kUnit : 0;
     uint32_t there = 0;                                     // bit i: the step i from now has rows
-    int next_page = steps > 0 ? kv4_page(c, q.seq, first_at) : -1;
+    int next_page = steps > 0 ? __ldcg(table + (first_at >> c.page_shift)) : -1;
     auto ahead = [&](int step) {
         const bool ok = step < steps && static_cast<unsigned>(next_page) < static_cast<unsigned>(c.num_pages);
-        if (ok) copy.issue(ring_at + static_cast<uint32_t>(step % kStages) * kStageBytes, next_page, first_at + step * kUnit, lane);
+        if (ok) copy.issue(static_cast<uint32_t>(step % kStages) * kStageBytes, next_page, first_at + step * kUnit, lane);
         asm volatile("cp.async.commit_group;" ::: "memory");
-        if (step + 1 < steps) next_page = kv4_page(c, q.seq, first_at + (step + 1) * kUnit);
+        if (step + 1 < steps) next_page = __ldcg(table + ((first_at + (step + 1) * kUnit) >> c.page_shift));
         there |= (ok ? 1u : 0u) << (kStages - 1);
     };
 #pragma unroll
@@ -432,7 +436,12 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
         __syncwarp();                                       // every lane's copies are there, and the slot of the step before has been read
         ahead(i + kStages - 1);
-        if (there & 1u) take(ring + (i % kStages) * kStageBytes, first_at + i * kUnit);
+        if (there & 1u) {
+            const int at = first_at + i * kUnit;
+            const uint8_t* st = ring + (i % kStages) * kStageBytes;
+            if (at + kKvTile > all_see) take.template operator()<true>(st, at);
+            else take.template operator()<false>(st, at);
+        }
         there >>= 1;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -618,9 +627,7 @@ __global__ void __launch_bounds__(kAttnThreads) kv4_key_weight_kernel(const __gr
                 float s = sum_half8(w);
 #pragma unroll
                 for (int d = 8; d > 0; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
-                uint32_t f[4];
-                query_words(w, f);
-                s_q[r >> 3][piece & 3][(r & 7) * 4 + (piece >> 2)] = make_uint4(f[0], f[1], f[2], f[3]);
+                s_q[r >> 3][piece & 3][(r & 7) * 4 + (piece >> 2)] = query_words(w);
                 if (piece == 0) { s_qsum[r] = s * to_log2; s_lse[r] = lse * kLog2e; }
             }
             __syncthreads();
