@@ -63,58 +63,65 @@ __device__ __forceinline__ SeqWork seq_work(const Kv4View& c, int b, int group, 
 struct Place {
     SeqWork w;
     int seq;
-    long long in_seq;             // unit of the sequence
+    long long in_seq;             // unit (or tile and head) of the sequence
+    long long units_before;       // units of the sequences in front
 };
 template <int THREADS>
 struct FindScratch {
-    long long sums[THREADS / 32];
+    longlong2 sums[THREADS / 32]; // units; units or tiles and heads
     Place found;
 };
 __device__ __forceinline__ long long ceil_div(long long a, int b) {
     // a division of 64 bits is a long subroutine in the way of the first load
     return a >> 31 == 0 ? static_cast<long long>((static_cast<uint32_t>(a) + static_cast<uint32_t>(b) - 1u) / static_cast<uint32_t>(b)) : (a + b - 1) / b;
 }
-// Units of the whole batch, and the place of unit `per * index` with per = ceil(all / parts); false where there is none.
-// All threads of the CTA call it.  One round trip, for up to THREADS sequences.
-template <int THREADS>
+// Units of the whole batch, per = ceil(all / parts), and the place of unit `per * index` or, with BY_TILE, of the (tile, head)
+// number `index`; false where there is none.  All threads of the CTA call it.  One round trip, for up to THREADS sequences.
+template <int THREADS, bool BY_TILE = false>
 __device__ __forceinline__ bool find_unit(const Kv4View& c, int group, int tile_rows, int index, int parts, FindScratch<THREADS>& s, long long* per, long long* all, Place* out) {
     const int tid = threadIdx.x, lane = tid & 31, each = (c.num_seqs + THREADS - 1) / THREADS;
     const int b0 = min(tid * each, c.num_seqs), b1 = min(b0 + each, c.num_seqs);
-    long long mine = 0;
+    longlong2 mine = {0, 0};
     SeqWork w{};
+    auto count = [&](longlong2& n) {
+        const long long tiles = static_cast<long long>(w.tiles) * c.kv_heads;
+        n.x += tiles * w.units;
+        n.y += tiles;
+    };
     for (int b = b0; b < b1; ++b) {
         w = seq_work(c, b, group, tile_rows);
-        mine += static_cast<long long>(w.tiles) * c.kv_heads * w.units;
+        count(mine);
     }
-    long long upto = mine;
+    longlong2 upto = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const long long o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-        if (lane >= d) upto += o;
+        const long long x = __shfl_up_sync(0xFFFFFFFFu, upto.x, d), y = BY_TILE ? __shfl_up_sync(0xFFFFFFFFu, upto.y, d) : 0;
+        if (lane >= d) { upto.x += x; upto.y += y; }
     }
     if (lane == 31) s.sums[tid >> 5] = upto;
     __syncthreads();
-    long long total = 0, before = 0;
+    longlong2 total = {0, 0};
+    longlong2 at = {upto.x - mine.x, upto.y - mine.y};
 #pragma unroll
     for (int i = 0; i < THREADS / 32; ++i) {
-        if (i == tid >> 5) before = total;
-        total += s.sums[i];
+        if (i == tid >> 5) { at.x += total.x; at.y += total.y; }
+        total.x += s.sums[i].x;
+        total.y += s.sums[i].y;
     }
-    *all = total;
-    *per = ceil_div(total, parts);
-    const long long want = *per * index;
-    if (want >= total) return false;
-    upto += before;
-    if (upto > want && upto - mine <= want) {        // the sequence is one of this thread's
-        long long at = upto - mine;
+    *all = total.x;
+    *per = ceil_div(total.x, parts);
+    const long long want = BY_TILE ? index : *per * index;
+    if (want >= (BY_TILE ? total.y : total.x)) return false;
+    if ((BY_TILE ? at.y : at.x) <= want && want < (BY_TILE ? at.y + mine.y : at.x + mine.x)) {        // the sequence is one of this thread's
         for (int b = b0; b < b1; ++b) {
             if (each > 1) w = seq_work(c, b, group, tile_rows);
-            const long long units = static_cast<long long>(w.tiles) * c.kv_heads * w.units;
-            if (want < at + units) {
-                s.found = Place{w, b, want - at};
+            longlong2 next = at;
+            count(next);
+            if (want < (BY_TILE ? next.y : next.x)) {
+                s.found = Place{w, b, want - (BY_TILE ? at.y : at.x), at.x};
                 break;
             }
-            at += units;
+            at = next;
         }
     }
     __syncthreads();
@@ -493,10 +500,10 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
     }
 }
 
-// The parts of a (tile, head) joined.  A CTA stands at the boundary of the CTAs blockIdx.x and blockIdx.x + 1 of the launch above, and
-// works if that is the first boundary inside a (tile, head).  SPLIT: there are few (tile, head), so of many parts each, and a CTA
-// joins one row (blockIdx.y), its warps sharing the parts; else a warp joins the rows of its number.
-constexpr int kJoinWarps = 8;
+// The parts of a (tile, head) joined.  SPLIT: there are few (tile, head), so of many parts each; a CTA joins one row (blockIdx.y) of
+// one (blockIdx.x), its warps sharing the parts.  Else a CTA stands at the boundary of the CTAs blockIdx.x and blockIdx.x + 1 of the
+// launch above, works if that is the first boundary inside a (tile, head), and a warp joins the rows of its number.
+constexpr int kJoinWarps = 16;
 template <bool F32, bool SPLIT>
 __global__ void __launch_bounds__(32 * kJoinWarps) kv4_attention_join_kernel(const __grid_constant__ Kv4AttentionArgs a, int tile_rows, int parts) {
     __shared__ FindScratch<32 * kJoinWarps> s_find;
@@ -509,13 +516,14 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv4_attention_join_kernel(con
     long long per, all;
     Place pl;
     const int boundary = blockIdx.x + 1;
-    if (!find_unit<32 * kJoinWarps>(c, a.group, tile_rows, boundary, parts, s_find, &per, &all, &pl)) return;
-    const int tile_head = static_cast<int>(pl.in_seq / pl.w.units);
-    const long long unit0 = per * boundary - (pl.in_seq - static_cast<long long>(tile_head) * pl.w.units);
-    if (unit0 == per * boundary || unit0 < per * (boundary - 1)) return;
-    const int c0 = boundary - 1, c1 = static_cast<int>((unit0 + pl.w.units - 1) / per);
+    if (!find_unit<32 * kJoinWarps, SPLIT>(c, a.group, tile_rows, SPLIT ? blockIdx.x : boundary, parts, s_find, &per, &all, &pl)) return;
+    const int tile_head = static_cast<int>(SPLIT ? pl.in_seq : pl.in_seq / pl.w.units);
+    const long long unit0 = pl.units_before + static_cast<long long>(tile_head) * pl.w.units;
+    if (!SPLIT && (unit0 == per * boundary || unit0 < per * (boundary - 1))) return;
+    const int c0 = SPLIT ? static_cast<int>(unit0 / per) : boundary - 1, c1 = static_cast<int>((unit0 + pl.w.units - 1) / per);
+    if (c0 == c1) return;                // one CTA had it all
     const int head = tile_head % c.kv_heads, row0 = tile_head / c.kv_heads * tile_rows, rows = min(tile_rows, pl.w.n * a.group - row0);
-    constexpr int kDeep = 4, kStride = SPLIT ? kJoinWarps : 1;
+    constexpr int kDeep = SPLIT ? 8 : 4, kStride = SPLIT ? kJoinWarps : 1;
     for (int r = SPLIT ? blockIdx.y : warp; r < rows; r += SPLIT ? tile_rows : kJoinWarps) {
         // part of CTA i: its first, unless the (tile, head) begins inside of it
         auto part_row = [&](int i) { return (2 * static_cast<size_t>(i) + (i == c0 && unit0 != per * c0 ? 1 : 0)) * tile_rows + r; };
@@ -703,7 +711,7 @@ int kv4_attention(Kv4AttentionArgs a, int q_heads, bool f32, void* workspace, cu
     const bool split = p.tile_heads * 8 <= ctas;     // more than eight parts each
     auto join = split ? (f32 ? kv4_attention_join_kernel<true, true> : kv4_attention_join_kernel<false, true>)
                       : (f32 ? kv4_attention_join_kernel<true, false> : kv4_attention_join_kernel<false, false>);
-    return static_cast<int>(launch_kernel(join, dim3(ctas - 1, split ? 8 * p.nt : 1), dim3(32 * kJoinWarps), 0, stream, pdl_enabled(), a, 8 * p.nt, ctas));
+    return static_cast<int>(launch_kernel(join, split ? dim3(static_cast<unsigned>(p.tile_heads), 8 * p.nt) : dim3(ctas - 1), dim3(32 * kJoinWarps), 0, stream, pdl_enabled(), a, 8 * p.nt, ctas));
 }
 
 int kv4_add_key_weights(const Kv4WeightArgs& a, cudaStream_t stream) {
