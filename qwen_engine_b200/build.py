@@ -17,7 +17,7 @@ LIB = PKG / "libw4a16_b200.so"
 LAUNCH = PKG / "_launch.so"
 LAUNCH_SOURCE = CSRC / "py_launch.cpp"
 SOURCES = ["c_abi.cu", "q8_1_quantize.cu", "gemv_decode.cu", "gemm_prefill.cu", "gemm_tc.cu", "decode_sweep.cu", "sweep_persistent.cu",
-           "gemv_static_scratch.cu", "sampling.cu", "embed_lookup.cu", "qwenbin.cu", "kv4_cache.cu", "kv4_attention.cu"]
+           "gemv_static_scratch.cu", "sampling.cu", "embed_lookup.cu", "qwenbin.cu", "kv4_cache.cu", "kv4_attention.cu", "kv4_attention_tc.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++20", "--expt-relaxed-constexpr",

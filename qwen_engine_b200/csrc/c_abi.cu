@@ -66,6 +66,7 @@ int ensure_device_ready(const DeviceInfo** out) {
             if (int st = gemv_set_attributes()) return st;
             if (int st = gemm_set_attributes()) return st;
             if (int st = kv4_set_attributes()) return st;
+            if (int st = kv4_chunk_set_attributes()) return st;
             info.ready = true;
             g_dev[dev] = info;
             g_dev_ready[dev].store(true, std::memory_order_release);
@@ -691,7 +692,10 @@ int64_t w4a16_attention_kv4_workspace_bytes(int num_tokens, int num_seqs, int nu
     if (num_q_heads % num_kv_heads != 0) return W4A16_ERR_SHAPE;
     if (num_tokens > (1 << 24) || num_seqs > 65535 || num_q_heads > 65535 || static_cast<long long>(num_tokens) * num_q_heads > (1ll << 30))
         return W4A16_ERR_TOO_LARGE;
-    return kv4_attention_plan(num_tokens, num_seqs, num_q_heads, num_kv_heads).bytes;
+    // enough for either form: which one a call takes depends on the type of its result
+    const int64_t few = kv4_attention_plan(num_tokens, num_seqs, num_q_heads, num_kv_heads).bytes;
+    const int64_t many = kv4_takes_chunk(num_tokens, num_seqs, num_q_heads, num_kv_heads, false) ? kv4_chunk_plan(num_tokens, num_seqs, num_q_heads, num_kv_heads).bytes : 0;
+    return few > many ? few : many;
 }
 
 int w4a16_attention_kv4(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, const void* q, void* out, float* lse,
@@ -702,9 +706,14 @@ int w4a16_attention_kv4(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* bat
     if (!q || !out || !std::isfinite(softmax_scale) || softmax_scale <= 0.0f) return W4A16_ERR_INVALID_ARG;
     if (int st = kv4_heads(c, num_q_heads, &q_stride, num_q_heads)) return st;
     if (misaligned(q, 16) || misaligned(out, 16) || misaligned(lse, 4) || misaligned(workspace, 16)) return W4A16_ERR_ALIGNMENT;
-    const int64_t need = kv4_attention_plan(c.num_tokens, c.num_seqs, num_q_heads, c.kv_heads).bytes;
+    const int64_t need = w4a16_attention_kv4_workspace_bytes(c.num_tokens, c.num_seqs, num_q_heads, c.kv_heads);
     if (need > 0 && (!workspace || workspace_bytes < need)) return W4A16_ERR_INVALID_ARG;
     if (int st = ensure_device_ready(nullptr)) return st;
+    if (kv4_takes_chunk(c.num_tokens, c.num_seqs, num_q_heads, c.kv_heads, out_fp32 != 0)) {
+        Kv4ChunkArgs a{};
+        a.c = c; a.q = H(q); a.out = H(out); a.lse = lse; a.scale = softmax_scale; a.group = num_q_heads / c.kv_heads; a.q_stride = q_stride;
+        return kv4_chunk_attention(a, num_q_heads, workspace, S(stream));
+    }
     Kv4AttentionArgs a{};
     a.c = c; a.q = H(q); a.out = out; a.lse = lse; a.scale = softmax_scale; a.group = num_q_heads / c.kv_heads; a.q_stride = q_stride;
     return kv4_attention(a, num_q_heads, out_fp32 != 0, workspace, S(stream));
@@ -739,10 +748,11 @@ int w4a16_debug_counter(int which, unsigned int* out) {
     if (!out) return W4A16_ERR_INVALID_ARG;
     if (int st = ensure_device_ready(nullptr)) return st;
     if (which == 0) {
-        unsigned int tc = 0, mma = 0;
+        unsigned int tc = 0, mma = 0, kv4 = 0;
         if (int st = gemm_tc_timeouts(&tc)) return st;
+        if (int st = kv4_chunk_timeouts(&kv4)) return st;
         if (int st = gemm_mma_timeouts(&mma)) return st;
-        *out = tc + mma;
+        *out = tc + mma + kv4;
         return 0;
     }
     if (which == 1) return gemv_copy_timeouts(out);

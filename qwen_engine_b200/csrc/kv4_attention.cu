@@ -14,13 +14,14 @@
 //   running maximum: renewed only where a score exceeds it by 2^8, which a vote finds; p <= 2^8 fits.
 #include "kv4.cuh"
 #include "kv4_attention.hpp"
+#include "kv4_work.cuh"
 #include "w4a16_internal.hpp"
 
 namespace w4 {
 namespace {
 
 constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+static_assert(kUnit == kKvTile * kAttnWarps);
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -31,107 +32,6 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
-}
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// How the work is cut.  A unit is 64 positions (16 a warp) against one tile of query rows and one head; units are numbered by
-// sequence, tile, head, position, and every CTA of a persistent grid takes the same number of consecutive ones.  So the CTAs
-// finish together whatever the lengths are (they live on the device, the host does not know them), and a CTA has at most two
-// parts of a (tile, head) that others have parts of too: its first and its last one.
-constexpr int kUnit = kKvTile * kAttnWarps;
-
-struct SeqWork {
-    int first, n;                 // rows of the batch
-    int past;                     // positions in front of the first new token (negative: tokens without a position)
-    int tiles, units;             // tiles of query rows; units of one tile and head
-};
-__device__ __forceinline__ SeqWork seq_work(const Kv4View& c, int b, int group, int tile_rows) {
-    SeqWork w;
-    const int2 mine = kv4_new_tokens(c, b);
-    const int len = max(__ldcg(c.lens + b), 0);
-    w.first = mine.x;
-    w.n = mine.y;
-    w.past = len - mine.y;
-    w.tiles = (mine.y * group + tile_rows - 1) / tile_rows;
-    w.units = max(1, (min(len, kv4_capacity(c)) + kUnit - 1) / kUnit);
-    return w;
-}
-// A place in the order of the units.
-struct Place {
-    SeqWork w;
-    int seq;
-    long long in_seq;             // unit (or tile and head) of the sequence
-    long long units_before;       // units of the sequences in front
-};
-template <int THREADS>
-struct FindScratch {
-    longlong2 sums[THREADS / 32]; // units; units or tiles and heads
-    Place found;
-};
-__device__ __forceinline__ long long ceil_div(long long a, int b) {
-    // a division of 64 bits is a long subroutine in the way of the first load
-    return a >> 31 == 0 ? static_cast<long long>((static_cast<uint32_t>(a) + static_cast<uint32_t>(b) - 1u) / static_cast<uint32_t>(b)) : (a + b - 1) / b;
-}
-// Units of the whole batch, per = ceil(all / parts), and the place of unit `per * index` or, with BY_TILE, of the (tile, head)
-// number `index`; false where there is none.  All threads of the CTA call it.  One round trip, for up to THREADS sequences.
-template <int THREADS, bool BY_TILE = false>
-__device__ __forceinline__ bool find_unit(const Kv4View& c, int group, int tile_rows, int index, int parts, FindScratch<THREADS>& s, long long* per, long long* all, Place* out) {
-    const int tid = threadIdx.x, lane = tid & 31, each = (c.num_seqs + THREADS - 1) / THREADS;
-    const int b0 = min(tid * each, c.num_seqs), b1 = min(b0 + each, c.num_seqs);
-    longlong2 mine = {0, 0};
-    SeqWork w{};
-    auto count = [&](longlong2& n) {
-        const long long tiles = static_cast<long long>(w.tiles) * c.kv_heads;
-        n.x += tiles * w.units;
-        n.y += tiles;
-    };
-    for (int b = b0; b < b1; ++b) {
-        w = seq_work(c, b, group, tile_rows);
-        count(mine);
-    }
-    longlong2 upto = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const long long x = __shfl_up_sync(0xFFFFFFFFu, upto.x, d), y = BY_TILE ? __shfl_up_sync(0xFFFFFFFFu, upto.y, d) : 0;
-        if (lane >= d) { upto.x += x; upto.y += y; }
-    }
-    if (lane == 31) s.sums[tid >> 5] = upto;
-    __syncthreads();
-    longlong2 total = {0, 0};
-    longlong2 at = {upto.x - mine.x, upto.y - mine.y};
-#pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) {
-        if (i == tid >> 5) { at.x += total.x; at.y += total.y; }
-        total.x += s.sums[i].x;
-        total.y += s.sums[i].y;
-    }
-    *all = total.x;
-    *per = ceil_div(total.x, parts);
-    const long long want = BY_TILE ? index : *per * index;
-    if (want >= (BY_TILE ? total.y : total.x)) return false;
-    if ((BY_TILE ? at.y : at.x) <= want && want < (BY_TILE ? at.y + mine.y : at.x + mine.x)) {        // the sequence is one of this thread's
-        for (int b = b0; b < b1; ++b) {
-            if (each > 1) w = seq_work(c, b, group, tile_rows);
-            longlong2 next = at;
-            count(next);
-            if (want < (BY_TILE ? next.y : next.x)) {
-                s.found = Place{w, b, want - (BY_TILE ? at.y : at.x), at.x};
-                break;
-            }
-            at = next;
-        }
-    }
-    __syncthreads();
-    *out = s.found;
-    return true;
-}
-
-// Output row r of a tile.
-__device__ __forceinline__ size_t out_row(const SeqWork& w, int heads, int group, int head, int row) {
-    return static_cast<size_t>(w.first + row / group) * (static_cast<size_t>(heads) * group) + head * group + row % group;
 }
 
 // A warp's 16 positions in shared memory, copied there by itself (cp.async, 5 a lane) several steps ahead: what is in flight
@@ -193,31 +93,6 @@ __device__ __forceinline__ float sum_half8(const uint4& w) {
         s += f.x + f.y;
     }
     return s;
-}
-
-// One part's four dimensions, with its maximum and sum, into a sum around `top` (the largest maximum).  A part without any
-// position has maximum -infinity and sum 0; where all parts are such, the factor is 1 and what is added is 0.
-__device__ __forceinline__ void add_part(float4& x, float& sum, const float4& p, float2 ml, float top) {
-    const float f = ml.x == top ? 1.0f : ex2(ml.x - top);
-    sum = fmaf(ml.y, f, sum);
-    x.x = fmaf(p.x, f, x.x);
-    x.y = fmaf(p.y, f, x.y);
-    x.z = fmaf(p.z, f, x.z);
-    x.w = fmaf(p.w, f, x.w);
-}
-// A finished row: a warp, four dimensions a lane.
-template <bool F32>
-__device__ __forceinline__ void store_row(const Kv4AttentionArgs& a, size_t row, const float4& x, float top, float sum) {
-    const int lane = threadIdx.x & 31;
-    const float f = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
-    const float4 y = sum == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
-    if constexpr (F32) {
-        reinterpret_cast<float4*>(static_cast<float*>(a.out) + row * kKvDim)[lane] = y;
-    } else {
-        const uint2 h = make_uint2(pack_half2(y.x, y.y), pack_half2(y.z, y.w));
-        reinterpret_cast<uint2*>(static_cast<__half*>(a.out) + row * kKvDim)[lane] = h;
-    }
-    if (lane == 0 && a.lse != nullptr) a.lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
 template <int NT, bool F32>
@@ -490,7 +365,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
 #pragma unroll
         for (int w = 0; w < kAttnWarps; ++w) add_part(x, sum, *reinterpret_cast<const float4*>(&s_o(w, r, 4 * lane)), ml[w], top);
         if (whole) {
-            store_row<F32>(a, out_row(pl.w, c.kv_heads, a.group, head, q.row0 + r), x, top, sum);
+            store_row<F32>(a.out, a.lse, out_row(pl.w, c.kv_heads, a.group, head, q.row0 + r), x, top, sum);
         } else {
             __stcg(reinterpret_cast<float4*>(a.part_o + (part * R + r) * kKvDim + 4 * lane), x);
             if (lane == 0) __stcg(a.part_ml + part * R + r, make_float2(top, sum));
@@ -567,7 +442,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv4_attention_join_kernel(con
 #pragma unroll
             for (int w = 0; w < kJoinWarps; ++w) add_part(x, sum, s_x[w][lane], s_ml[w], top);
         }
-        store_row<F32>(a, out_row(pl.w, c.kv_heads, a.group, head, row0 + r), x, top, sum);
+        store_row<F32>(a.out, a.lse, out_row(pl.w, c.kv_heads, a.group, head, row0 + r), x, top, sum);
     }
 }
 

@@ -29,6 +29,29 @@ struct Kv4AttentionPlan {
 };
 Kv4AttentionPlan kv4_attention_plan(int num_tokens, int num_seqs, int q_heads, int kv_heads);
 int kv4_attention(Kv4AttentionArgs a, int q_heads, bool f32, void* workspace, cudaStream_t stream);
+// The form for many query rows and an fp16 result (kv4_attention_tc.cu).
+struct Kv4ChunkArgs {
+    Kv4View c;
+    const __half* q;
+    __half* out;
+    float* lse;              // may be null
+    float* part_o;           // splits: unnormalised sums [tile][head][split][row][128] ...
+    float2* part_ml;         // ... and maximum (base 2) and sum of weights
+    float scale;
+    int group, q_stride, splits;
+};
+struct Kv4ChunkPlan {
+    int splits;
+    long long tile_heads, ml_offset, bytes;
+};
+Kv4ChunkPlan kv4_chunk_plan(int num_tokens, int num_seqs, int q_heads, int kv_heads);
+int kv4_chunk_attention(Kv4ChunkArgs a, int q_heads, void* workspace, cudaStream_t stream);
+int kv4_chunk_set_attributes();
+int kv4_chunk_timeouts(unsigned int* out);
+// Which form a call takes: the tensor-memory kernel for fp16 results of at least 64 query rows a sequence and head.
+inline bool kv4_takes_chunk(int num_tokens, int num_seqs, int q_heads, int kv_heads, bool f32) {
+    return !f32 && static_cast<long long>(q_heads / kv_heads) * num_tokens >= 64ll * num_seqs;
+}
 int kv4_add_key_weights(const Kv4WeightArgs& a, cudaStream_t stream);
 
 struct Kv4AppendArgs {

@@ -79,7 +79,7 @@ def spans(lens, new):
         first += n
 
 
-def attention(pool, table, lens, new, q, scale):
+def attention(pool, table, lens, new, q, scale, fp16_rows=False):
     """q [tokens, heads, 128] -> out, lse, and bounds of the 32-bit result's error: the tokens' outputs and lse.
 
     Score error: a sum of 128 exact products in 32 bits, whatever its order and with truncation, is off by at most 128 * 2^-23
@@ -96,6 +96,7 @@ def attention(pool, table, lens, new, q, scale):
         for h in range(pool.kv):
             k, there = pool.rows(table[b], h, top, 0)
             v, _ = pool.rows(table[b], h, top, 1)
+            step = 2.0 ** -11 if fp16_rows else 0.0
             for i in range(n):
                 see = there & (np.arange(top) <= L - n + i)
                 if not see.any():
@@ -109,8 +110,8 @@ def attention(pool, table, lens, new, q, scale):
                     out[first + i, h * group + g] = p @ vv / p.sum()
                     lse[first + i, h * group + g] = m + np.log(p.sum())
                     size = (np.abs(kk) @ np.abs(x) + 2 * np.abs(kk).max(1) * np.abs(x).sum()).max() * scale
-                    d = (128 * 2.0 ** -23 + 4 * 2.0 ** -24) * size + 2.0 ** -22 * max(1, np.abs(s).max())
-                    eout[first + i, h * group + g] = (4 * d + 2.0 ** -20 + see.sum() * 2.0 ** -27) * np.abs(vv).max() * 3
+                    d = (128 * 2.0 ** -23 + 4 * 2.0 ** -24) * size + 2.0 ** -22 * max(1, np.abs(s).max()) + step * (np.abs(kk) @ np.abs(x)).max() * scale
+                    eout[first + i, h * group + g] = (4 * d + 2 * step + 2.0 ** -20 + see.sum() * 2.0 ** -27) * np.abs(vv).max() * 3
                     else_[first + i, h * group + g] = 2 * d + 2.0 ** -21 + 2.0 ** -22 * abs(lse[first + i, h * group + g])
     return out, lse, eout, else_
 
