@@ -727,7 +727,7 @@ int w4a16_kv4_add_key_weights(const w4a16_kv4_cache* cache, const w4a16_kv4_batc
     if (int st = kv4_heads(c, num_q_heads, &q_stride, num_q_heads)) return st;
     if (misaligned(q, 16) || misaligned(lse, 4)) return W4A16_ERR_ALIGNMENT;
     if (int st = ensure_device_ready(nullptr)) return st;
-    return kv4_add_key_weights(Kv4WeightArgs{c, H(q), lse, softmax_scale, num_q_heads / c.kv_heads, q_stride}, S(stream));
+    return kv4_add_key_weights(Kv4WeightArgs{c, H(q), lse, softmax_scale, num_q_heads / c.kv_heads, q_stride, 0}, S(stream));
 }
 
 int w4a16_kv4_evict(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, const int32_t* dst_block_table, int32_t* new_seq_lens,

@@ -448,74 +448,104 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv4_attention_join_kernel(con
 
 // ---- attention weight of the cached positions ------------------------------------------------------------------
 
-// A warp owns 32 positions of a head and adds up, over all query rows of the sequence, exp(score - lse): no position is
-// another warp's, so nothing is atomic and the order of the sum is fixed.  The keys' codes are converted once and stay in
-// registers; the queries pass through shared memory in blocks of 64 rows, already in fragment order.
-constexpr int kWeightRows = 64, kWeightPositions = 32 * kAttnWarps;
+// A warp takes 32 positions of a head and adds up, over all query rows of the sequence, exp(score - lse): no position is
+// another warp's, so nothing is atomic and the order of the sum is fixed.  The queries pass through shared memory in blocks of up to
+// 128 rows, in fragment order, and stay there while the CTA walks over its positions; the codes of the next 32 are on their way
+// meanwhile.  What bounds it is the rate of mma.sync (with a block of rows staged for each 128 positions it was the staging: the last 32
+// tokens of two sequences of 32 000 and 20 000 positions, 32 heads on 8, took 111 us).
+constexpr int kWeightRows = 128, kWeightPositions = 32 * kAttnWarps;
 
-__global__ void __launch_bounds__(kAttnThreads) kv4_key_weight_kernel(const __grid_constant__ Kv4WeightArgs a) {
+__global__ void __launch_bounds__(kAttnThreads, 4) kv4_key_weight_kernel(const __grid_constant__ Kv4WeightArgs a) {
     __shared__ uint4 s_q[kWeightRows / 8][4][32];
-    __shared__ float s_qsum[kWeightRows], s_lse[kWeightRows];
+    __shared__ float2 s_row[kWeightRows];                    // sum of q, -lse, both in the exponent's units
     pdl_wait_prior_grids();
     pdl_release_dependents();
     const Kv4View& c = a.c;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int head = blockIdx.y, b = blockIdx.z;
+    const int head = blockIdx.y, b = blockIdx.z, ps = 1 << c.page_shift;
+    const int first = blockIdx.x * a.positions + warp * 32;
     const int2 mine = kv4_new_tokens(c, b);
-    const int len = max(__ldcg(c.lens + b), 0), seen = min(len, kv4_capacity(c)), past = len - mine.y;
-    const int rows = mine.y * a.group;
+    const int len = max(__ldcg(c.lens + b), 0), past = len - mine.y;
+    const int rows = mine.y * a.group, end = min(min(len, kv4_capacity(c)), (static_cast<int>(blockIdx.x) + 1) * a.positions);
     const float to_log2 = a.scale * kLog2e;
-    for (int base = blockIdx.x * kWeightPositions; base < seen && rows > 0; base += gridDim.x * kWeightPositions) {
-        const int at = base + warp * 32;
-        // codes of positions at + g + {0, 8, 16, 24}
-        uint32_t codes[2][4][2][4];
-        float ks[4], kz[4], got[4] = {};
-        bool ok[2];
-        int pages[2];
+    const int32_t* table = c.table + static_cast<size_t>(b) * c.max_pages;
+    if (blockIdx.x * a.positions >= end || rows <= 0) return;
+    // what the lane needs of 32 positions: rows at + g + {0, 8, 16, 24}
+    struct Raw {
+        uint4 w[4];
+        uint32_t params[4];
+        int page[2];
+    } raw;
+    auto pages = [&](int at, int (&p)[2]) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) p[u] = at + 16 * u < end ? __ldcg(table + ((at + 16 * u) >> c.page_shift)) : -1;
+    };
+    auto fetch = [&](int at) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int p = at + 16 * u;
-            pages[u] = p < seen ? kv4_page(c, b, p) : -1;
-            const uint32_t* record = kv4_record_of_page(c, pages[u], head);
-            ok[u] = record != nullptr;
+            const uint32_t* record = kv4_record_of_page(c, raw.page[u], head);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                uint4 w = make_uint4(0, 0, 0, 0);
-                uint32_t params = 0;
-                if (ok[u]) {
-                    const int ps = 1 << c.page_shift, s = (p & (ps - 1)) + g + 8 * i;
-                    w = __ldcg(reinterpret_cast<const uint4*>(record + s * kKvRowWords + 4 * t));
-                    params = __ldcg(record + 32 * ps + s);
+                raw.w[2 * u + i] = make_uint4(0, 0, 0, 0);
+                raw.params[2 * u + i] = 0;
+                if (record != nullptr) {
+                    const int s = ((at + 16 * u) & (ps - 1)) + g + 8 * i;
+                    raw.w[2 * u + i] = __ldcg(reinterpret_cast<const uint4*>(record + s * kKvRowWords + 4 * t));
+                    raw.params[2 * u + i] = __ldcg(record + 32 * ps + s);
                 }
-                ks[2 * u + i] = kv4_scale(params) * (to_log2 * kKvKeyUndo);
-                kz[2 * u + i] = fmaf(-8.0f, kv4_scale(params), kv4_zero(params));
-                kv4_key_codes(w.x, codes[u][0][i]);
-                kv4_key_codes(w.y, codes[u][1][i]);
-                kv4_key_codes(w.z, codes[u][2][i]);
-                kv4_key_codes(w.w, codes[u][3][i]);
             }
         }
-        for (int r0 = 0; r0 < rows; r0 += kWeightRows) {
-            __syncthreads();
-            // a row is 16 pieces of 16 bytes; half-warps take rows
-            for (int r = threadIdx.x >> 4; r < kWeightRows; r += kAttnThreads / 16) {
-                const int piece = threadIdx.x & 15, row = r0 + r;
-                uint4 w = make_uint4(0, 0, 0, 0);
-                float lse = INFINITY;
-                if (row < rows) {
-                    const int token = mine.x + row / a.group, h = head * a.group + row % a.group;
-                    w = __ldcg(reinterpret_cast<const uint4*>(a.q + static_cast<size_t>(token) * a.q_stride + h * kKvDim + 8 * piece));
-                    lse = __ldcg(a.lse + static_cast<size_t>(token) * c.kv_heads * a.group + h);
-                }
-                float s = sum_half8(w);
-#pragma unroll
-                for (int d = 8; d > 0; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
-                s_q[r >> 3][piece & 3][(r & 7) * 4 + (piece >> 2)] = query_words(w);
-                if (piece == 0) { s_qsum[r] = s * to_log2; s_lse[r] = lse * kLog2e; }
+    };
+    for (int r0 = 0; r0 < rows; r0 += kWeightRows) {
+        int next[2];
+        pages(first, raw.page);
+        // a row is 16 pieces of 16 bytes; half-warps take rows
+        const int staged = min((rows - r0 + 7) & ~7, kWeightRows);
+        __syncthreads();
+        for (int r = threadIdx.x >> 4; r < staged; r += kAttnThreads / 16) {
+            const int piece = threadIdx.x & 15, row = r0 + r;
+            uint4 w = make_uint4(0, 0, 0, 0);
+            float lse = INFINITY;
+            if (row < rows) {
+                const int token = mine.x + row / a.group, h = head * a.group + row % a.group;
+                w = __ldcg(reinterpret_cast<const uint4*>(a.q + static_cast<size_t>(token) * a.q_stride + h * kKvDim + 8 * piece));
+                lse = __ldcg(a.lse + static_cast<size_t>(token) * c.kv_heads * a.group + h);
             }
-            __syncthreads();
-            const int blocks = (min(rows - r0, kWeightRows) + 7) / 8;
-            for (int n = 0; n < blocks; ++n) {
+            float s = sum_half8(w);
+#pragma unroll
+            for (int d = 8; d > 0; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
+            s_q[r >> 3][piece & 3][(r & 7) * 4 + (piece >> 2)] = query_words(w);
+            if (piece == 0) s_row[r] = make_float2(s * to_log2, -lse * kLog2e);
+        }
+        fetch(first);
+        pages(first + kWeightPositions, next);
+        __syncthreads();
+        for (int at = first; at < end; at += kWeightPositions) {
+            uint32_t codes[2][4][2][4];
+            float ks[4], kz[4], got[4] = {}, old[4] = {};
+            float* weight[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                ks[k] = kv4_scale(raw.params[k]);
+                kz[k] = fmaf(-8.0f, ks[k], kv4_zero(raw.params[k]));
+                ks[k] *= to_log2 * kKvKeyUndo;
+                kv4_key_codes(raw.w[k].x, codes[k >> 1][0][k & 1]);
+                kv4_key_codes(raw.w[k].y, codes[k >> 1][1][k & 1]);
+                kv4_key_codes(raw.w[k].z, codes[k >> 1][2][k & 1]);
+                kv4_key_codes(raw.w[k].w, codes[k >> 1][3][k & 1]);
+                const int p = at + 8 * k + g;
+                weight[k] = nullptr;
+                if (t == 0 && p < end && static_cast<unsigned>(raw.page[k >> 1]) < static_cast<unsigned>(c.num_pages)) {
+                    weight[k] = c.key_weight + kv4_weight_index(c, raw.page[k >> 1], head, p);
+                    old[k] = __ldcg(weight[k]);
+                }
+            }
+            raw.page[0] = next[0];
+            raw.page[1] = next[1];
+            fetch(at + kWeightPositions);
+            pages(at + 2 * kWeightPositions, next);
+            const bool all_see = at + 32 <= past + r0 / a.group + 1;
+            for (int n = 0; n < staged / 8; ++n) {
                 float even[2][4] = {}, s[2][4] = {};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -528,29 +558,24 @@ __global__ void __launch_bounds__(kAttnThreads) kv4_key_weight_kernel(const __gr
                         mma_16816(s[u], a1, f.z, f.w);
                     }
                 }
+                const float4 row = *reinterpret_cast<const float4*>(&s_row[n * 8 + 2 * t]);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int r = n * 8 + 2 * t + e;
-                    const float qs = s_qsum[r], lse = s_lse[r];
-                    const int limit = r0 + r < rows ? past + (r0 + r) / a.group + 1 : 0;
+                    const float qs = e ? row.z : row.x, less = e ? row.w : row.y;
+                    const int r = r0 + n * 8 + 2 * t + e, limit = all_see ? 0x7FFFFFFF : r < rows ? past + r / a.group + 1 : 0;
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const float x = fmaf(kv4_key_sum(even[u][2 * i + e], s[u][2 * i + e]), ks[2 * u + i], kz[2 * u + i] * qs) - lse;
-                            if (at + 16 * u + 8 * i + g < limit) got[2 * u + i] += ex2(x);
-                        }
+                    for (int k = 0; k < 4; ++k) {
+                        const float x = fmaf(kv4_key_sum(even[k >> 1][2 * (k & 1) + e], s[k >> 1][2 * (k & 1) + e]), ks[k], fmaf(kz[k], qs, less));
+                        const float p = ex2(x);
+                        got[k] += all_see || at + 8 * k + g < limit ? p : 0.0f;
+                    }
                 }
             }
-        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            got[i] += __shfl_xor_sync(0xFFFFFFFFu, got[i], 1);
-            got[i] += __shfl_xor_sync(0xFFFFFFFFu, got[i], 2);
-            const int p = at + 8 * i + g;
-            if (t == 0 && p < seen && ok[i >> 1]) {
-                float* w = c.key_weight + kv4_weight_index(c, pages[i >> 1], head, p);
-                *w = __ldcg(w) + got[i];
+            for (int k = 0; k < 4; ++k) {
+                got[k] += __shfl_xor_sync(0xFFFFFFFFu, got[k], 1);
+                got[k] += __shfl_xor_sync(0xFFFFFFFFu, got[k], 2);
+                if (weight[k] != nullptr) __stcg(weight[k], old[k] + got[k]);
             }
         }
     }
@@ -589,10 +614,15 @@ int kv4_attention(Kv4AttentionArgs a, int q_heads, bool f32, void* workspace, cu
     return static_cast<int>(launch_kernel(join, split ? dim3(static_cast<unsigned>(p.tile_heads), 8 * p.nt) : dim3(ctas - 1), dim3(32 * kJoinWarps), 0, stream, pdl_enabled(), a, 8 * p.nt, ctas));
 }
 
-int kv4_add_key_weights(const Kv4WeightArgs& a, cudaStream_t stream) {
+int kv4_add_key_weights(Kv4WeightArgs a, cudaStream_t stream) {
     const Kv4View& c = a.c;
-    const long long blocks = ((static_cast<long long>(c.max_pages) << c.page_shift) + kWeightPositions - 1) / kWeightPositions;
-    const dim3 grid(static_cast<unsigned>(blocks < 4096 ? blocks : 4096), c.kv_heads, c.num_seqs);
+    // as many positions a CTA as leave each SM four CTAs where the tables are as long as the sequences; 128 at least, 2048 at most
+    const long long capacity = static_cast<long long>(c.max_pages) << c.page_shift;
+    const long long each = capacity * c.kv_heads * c.num_seqs / (148 * 4);
+    a.positions = static_cast<int>(each < kWeightPositions ? kWeightPositions : each > 2048 ? 2048 : each / kWeightPositions * kWeightPositions);
+    const long long blocks = (capacity + a.positions - 1) / a.positions;
+    if (blocks > 0x7FFFFFFFll / a.positions) return W4A16_ERR_TOO_LARGE;
+    const dim3 grid(static_cast<unsigned>(blocks), c.kv_heads, c.num_seqs);
     return static_cast<int>(launch_kernel(kv4_key_weight_kernel, grid, dim3(kAttnThreads), 0, stream, pdl_enabled(), a));
 }
 

@@ -21,6 +21,7 @@ struct Kv4WeightArgs {
     const float* lse;
     float scale;
     int group, q_stride;
+    int positions;           // of a CTA; the launch chooses
 };
 // How a call is cut; a function of its sizes alone, so that the workspace can be sized without a device.
 struct Kv4AttentionPlan {
@@ -52,7 +53,7 @@ int kv4_chunk_timeouts(unsigned int* out);
 inline bool kv4_takes_chunk(int num_tokens, int num_seqs, int q_heads, int kv_heads, bool f32) {
     return !f32 && static_cast<long long>(q_heads / kv_heads) * num_tokens >= 64ll * num_seqs;
 }
-int kv4_add_key_weights(const Kv4WeightArgs& a, cudaStream_t stream);
+int kv4_add_key_weights(Kv4WeightArgs a, cudaStream_t stream);
 
 struct Kv4AppendArgs {
     const __half *q, *k, *v, *q_bias, *k_bias, *v_bias;

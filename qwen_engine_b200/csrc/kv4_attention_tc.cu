@@ -3,7 +3,8 @@
 // A CTA has 256 query rows of one key/value head (token major, so the heads that share it lie side by side) as two tiles of 128,
 // and walks over the positions 128 at a time:
 //   S_i [128 rows x 128 positions] = Q_i . K^T      Q and K from shared memory
-//   P_i = 2^(S_i c - m), fp16, over S_i in tensor memory; m is the running maximum, renewed only where a score exceeds it by 2^8
+//   P_i = 2^(S_i c - m), fp16, over S_i in tensor memory; m follows the running maximum, for the next step where it falls 8 behind, at
+//       once (the step's weights are worked out again) where 15, as fp16 ends at 2^16
 //   O_i [128 rows x 128 dims] += P_i . V            P from tensor memory, V (transposed: positions contiguous) from shared memory
 // While the softmax warps of one tile work the tensor core has the other one.  Keys and values become fp16 once for both tiles:
 // value = (code - 8) * scale + zero by one fma behind an exact conversion, so with one rounding.
@@ -30,7 +31,15 @@ namespace w4 {
 namespace {
 
 constexpr int kTile = 128, kChunkRows = 2 * kTile, kChunkKeys = 128;
-constexpr int kSoftWarps = 8, kKeyWarp = 8, kValueWarp = 12, kMmaWarp = 16, kChunkThreads = 17 * 32;
+constexpr int kSoftWarps = 8, kKeyWarp = 8, kValueWarp = 12, kMmaWarp = 16, kChunkThreads = 20 * 32;
+// Registers: a launch of 20 warps has 96 a thread (61 440); the warpgroups share them as 128 (softmax, two), 80 (keys, values) and 64
+// (the issuing warp's): 256 * 128 + 256 * 80 + 128 * 64 = 61 440.
+constexpr int kSoftRegs = 128, kOperandRegs = 80, kIssueRegs = 64;
+static_assert(256 * kSoftRegs + 256 * kOperandRegs + 128 * kIssueRegs <= kChunkThreads * 96);
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 constexpr int kOperand = kTile * kKvDim * 2;              // bytes of a 128 x 128 operand: two panels of 64 columns, 128-byte swizzle
 constexpr int kPanel = kOperand / 2;
 constexpr int kValueStage = kChunkKeys * 64;
@@ -38,24 +47,136 @@ constexpr int kSmemK = 2 * kOperand, kSmemV = 4 * kOperand, kSmemStage = 6 * kOp
 constexpr int kChunkSmem = kSmemParam + 2 * kChunkKeys * 4;
 constexpr int kTmemO = 256;                               // S_0, S_1, O_0, O_1: 128 columns each
 
-__device__ __forceinline__ void tc_mma_f16_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+// The two products, with descriptors given by their low words (address): the high word is the same for every operand here, and as
+// 64-bit values the 64 of them that the unrolled loop uses were kept in registers, and spilled.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);      // rows of 128 bytes in groups of 8, 128-byte swizzle
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr) { return ((addr & 0x3FFFFu) >> 4) | (1u << 16); }
+__device__ __forceinline__ void mma_ss(uint32_t tmem_d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
         : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
-        "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]),
-          "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]),
-          "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]),
-          "=f"(r[31])
-        : "r"(taddr)
-        : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+                 : "r"(taddr)
+                 : "memory");
+}
+// Bounded waits that leave the issue slots to others: a try that parks the thread for up to 20 us, and the abort flag looked at
+// between tries only.  (With the short tries of mbar_wait, and its flag at each, waiting warps issued 6000 of a step's 14 000
+// instructions.)
+__device__ __forceinline__ bool park_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    if (mbar_test_wait(bar, parity)) return true;      // a try costs more even where the phase is complete (663 us without this, 615 with)
+    for (unsigned it = 0; it < (1u << 16); ++it) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity), "r"(20000u)
+            : "memory");
+        if (ok) return true;
+        if (*abort_flag) return false;
+    }
+    *abort_flag = 1;
+    atomicAdd(&g_tc_wait_timeouts, 1u);
+    return false;
+}
+// The whole warp waits, every lane by itself: all see what the barrier's arrivals announce.  (One lane's wait behind a branch made the
+// whole kernel a third slower, 817 us for 615: what follows it is no longer known to be converged.)
+__device__ __forceinline__ bool park_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    return __all_sync(0xFFFFFFFFu, park_wait(bar, parity, abort_flag));
+}
+// Two 32-bit operations in one instruction, the exponential and the conversion, all volatile: their order is the software pipeline
+// of softmax_pass.
+__device__ __forceinline__ void fma2(float& x, float& y, float2 b, float2 c) {
+    asm volatile("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tmov.b64 c, {%4, %5};\n\tfma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+                 : "+f"(x), "+f"(y) : "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+}
+__device__ __forceinline__ void add2(float2& s, float x, float y) {
+    asm volatile("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+                 : "+f"(s.x), "+f"(s.y) : "f"(x), "f"(y));
+}
+__device__ __forceinline__ void ex2_here(float& x) { asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(x)); }
+__device__ __forceinline__ uint32_t pack_here(float lo, float hi) {
+    uint32_t d;
+    asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+
+// Waits for the tensor-memory loads in flight and hands the values on: whatever uses them depends on the wait.
+__device__ __forceinline__ void tmem_take32(float (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15])
+                 :: "memory");
+    asm volatile("" : "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]), "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31]) :: "memory");
+}
+
+// A row of 128 scores to weights p = 2^(score * scale2 - mu), as fp16 pairs, their sum, and the largest exponent.  What bounds it is
+// the exponential, 8 cycles a warp; so it is one stream of them, with a pair's scaling eight pairs ahead of its exponential and its sum
+// and conversion three behind.  (As loops that the compiler orders a row took 2200 cycles alone on its scheduler.)  The wait for
+// tensor-memory loads is one for all that are in flight, so 32 columns are asked for behind the wait for the 32 before them and
+// have all of their exponentials' time; asked for in eighths, later, each wait stalled (2200 cycles again, 1300 without loads).
+// SIMPLE: the row sees every position; else `sees` and, of those, `bad` (weight NaN).
+template <bool SIMPLE>
+__device__ __forceinline__ float softmax_pass(uint32_t t_s, float2 scale2, float2 mu2, const uint32_t (&sees)[4], const uint32_t (&bad)[4], uint32_t (&p)[64], float* total) {
+    float s[2][32];
+    float2 sum[2] = {};
+    float top[2] = {-INFINITY, -INFINITY};
+    auto scale = [&](int c, int k) {
+        float &x = s[c & 1][2 * k], &y = s[c & 1][2 * k + 1];
+        fma2(x, y, scale2, mu2);
+        if (!SIMPLE) {
+            if (!(sees[c] >> (2 * k) & 1u)) x = -INFINITY;
+            if (!(sees[c] >> (2 * k) & 2u)) y = -INFINITY;
+        }
+        top[k & 1] = fmaxf(top[k & 1], fmaxf(x, y));
+    };
+    auto finish = [&](int c, int k) {
+        float &x = s[c & 1][2 * k], &y = s[c & 1][2 * k + 1];
+        if (!SIMPLE) {
+            if (bad[c] >> (2 * k) & 1u) x = __int_as_float(0x7FC00000);
+            if (bad[c] >> (2 * k) & 2u) y = __int_as_float(0x7FC00000);
+        }
+        add2(sum[k & 1], x, y);
+        p[16 * c + k] = pack_here(x, y);
+    };
+    constexpr int kAhead = 8, kBehind = 3;
+    tmem_ld32(t_s, s[0]);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        tmem_take32(s[c & 1]);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) scale(c, k);
+        if (c > 0) {
+#pragma unroll
+            for (int k = 16 - kBehind; k < 16; ++k) finish(c - 1, k);
+        }
+        if (c < 3) tmem_ld32(t_s + 32u * (c + 1), s[(c + 1) & 1]);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            ex2_here(s[c & 1][2 * k]);
+            ex2_here(s[c & 1][2 * k + 1]);
+            if (k + kAhead < 16) scale(c, k + kAhead);
+            if (k >= kBehind) finish(c, k - kBehind);
+        }
+    }
+#pragma unroll
+    for (int k = 16 - kBehind; k < 16; ++k) finish(3, k);
+    *total = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+    return fmaxf(top[0], top[1]);
 }
 
 // (scale, zero) of a row that becomes fp16 values: where rounding took its ends past 65504 both shrink a little, so that none is
@@ -161,7 +282,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;
+    constexpr uint32_t tmem = 0;        // all 512 columns are this CTA's, so they begin at 0; a constant keeps the issuing thread's operands uniform
     pdl_release_dependents();           // not before: a CTA of the next launch must not take this one's tensor memory
     const int seen = work ? chunk_seen(c, pl, a.group) : 0, steps_each = chunk_steps(seen, a.splits);
     const int k0 = split * steps_each * kChunkKeys, k1 = min(seen, k0 + steps_each * kChunkKeys);
@@ -172,6 +293,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
 
     if (warp < kSoftWarps) {
         // ================= softmax: thread = row = tensor-memory lane =================
+        more_registers<kSoftRegs>();
         const int i = warp >> 2, r = tid & 127, row = i * kTile + r;
         const bool mine = work && row < pl.rows;
         const size_t at_row = mine ? out_row(pl.w, c.kv_heads, a.group, pl.head, pl.row0 + row) : 0;
@@ -194,91 +316,75 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
         const float to_log2 = a.scale * kLog2e;
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t t_s = lanes + static_cast<uint32_t>(i * 128), t_o = lanes + static_cast<uint32_t>(kTmemO + i * 128);
-        float m = -INFINITY, mu = 0.0f, l = 0.0f;
+        // m: reference of the exponents, at most 15 below the row's largest so far and renewed where it is 8 below; grow: by how much, at
+        // the next step.  Rows that have seen nothing have -infinity.
+        float m = -INFINITY, l = 0.0f, grow = 0.0f;
         bool ok = true;
         for (int j = 0; j < (i < tiles ? steps : 0); ++j) {
-            ok = warp_wait(s_full(i), j & 1, s_abort, lane);
+            ok = park_warp(s_full(i), j & 1, s_abort);
             if (!ok) break;
             tc_fence_after();
             const int base = k0 + j * kChunkKeys;
-            const uint4 there = *reinterpret_cast<const uint4*>(s_mask[j & 3][0]), poison = *reinterpret_cast<const uint4*>(s_mask[j & 3][1]);
-            const uint32_t all = there.x & there.y & there.z & there.w, any = poison.x | poison.y | poison.z | poison.w;
-            const bool simple = __all_sync(0xFFFFFFFFu, base + kChunkKeys <= limit && all == ~0u && any == 0);
-            const uint32_t th[4] = {there.x, there.y, there.z, there.w}, po[4] = {poison.x, poison.y, poison.z, poison.w};
-            auto sees = [&](int q) -> uint32_t {        // the row's positions of quarter q
-                const int n = limit - base - 32 * q;
-                return th[q] & (n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u);
-            };
-            float x[2][32];
-            float top = -INFINITY;
-            tmem_ld32(t_s, x[0]);
+            uint32_t sees[4], bad[4];
+            bool simple;
+            {
+                const uint4 there = *reinterpret_cast<const uint4*>(s_mask[j & 3][0]), poison = *reinterpret_cast<const uint4*>(s_mask[j & 3][1]);
+                const uint32_t all = there.x & there.y & there.z & there.w, any = poison.x | poison.y | poison.z | poison.w;
+                simple = __all_sync(0xFFFFFFFFu, base + kChunkKeys <= limit && all == ~0u && any == 0);
+                const uint32_t th[4] = {there.x, there.y, there.z, there.w}, po[4] = {poison.x, poison.y, poison.z, poison.w};
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                tmem_ld_wait();
-                if (q < 3) tmem_ld32(t_s + 32u * (q + 1), x[(q + 1) & 1]);
-                float (&v)[32] = x[q & 1];
-                if (!simple) {
-                    const uint32_t bits = sees(q);
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) v[k] = bits >> k & 1u ? v[k] : -INFINITY;
+                for (int q = 0; q < 4; ++q) {
+                    const int n = limit - base - 32 * q;
+                    sees[q] = th[q] & (n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u);
+                    bad[q] = sees[q] & po[q];
                 }
-                float t4[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-                for (int k = 4; k < 32; ++k) t4[k & 3] = fmaxf(t4[k & 3], v[k]);
-                top = fmaxf(top, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
             }
-            top *= to_log2;
-            if (__any_sync(0xFFFFFFFFu, top > m + 8.0f)) {
-                const float fresh = fmaxf(m, top), f = fresh == m ? 1.0f : ex2(m - fresh);
-                m = fresh;
-                mu = fresh == -INFINITY ? 0.0f : fresh;
-                l *= f;
-                if (j > 0) {
-                    // the product of the step before is complete: s_full of this step was committed behind it
+            uint32_t p[64];
+            float sum;
+            for (int turns = 0; turns < 2; ++turns) {
+                if (__any_sync(0xFFFFFFFFu, grow > 0.0f)) {
+                    const float f = ex2(-grow);
+                    m += grow;
+                    l *= f;
+                    grow = 0.0f;
+                    if (j > 0) {
+                        // the product of the step before is complete: s_full of this step was committed behind it
 #pragma unroll 1
-                    for (int q = 0; q < 4; ++q) {
-                        tmem_ld32(t_o + 32u * q, x[0]);
-                        tmem_ld_wait();
-                        uint32_t y[2][16];
+                        for (int q = 0; q < 4; ++q) {
+                            float x[32];
+                            tmem_ld32(t_o + 32u * q, x);
+                            tmem_take32(x);
+                            uint32_t y[2][16];
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) y[k >> 4][k & 15] = __float_as_uint(x[0][k] * f);
-                        tmem_st16(t_o + 32u * q, y[0]);
-                        tmem_st16(t_o + 32u * q + 16u, y[1]);
+                            for (int k = 0; k < 32; ++k) y[k >> 4][k & 15] = __float_as_uint(x[k] * f);
+                            tmem_st16(t_o + 32u * q, y[0]);
+                            tmem_st16(t_o + 32u * q + 16u, y[1]);
+                        }
                     }
                 }
+                const float mu = m == -INFINITY ? 0.0f : m;
+                const float2 scale2 = make_float2(to_log2, to_log2), mu2 = make_float2(-mu, -mu);
+                const float top = simple ? softmax_pass<true>(t_s, scale2, mu2, sees, bad, p, &sum) : softmax_pass<false>(t_s, scale2, mu2, sees, bad, p, &sum);
+                // too large for fp16, or the row's first positions: again with the maximum known
+                const bool fresh = m == -INFINITY && top > -INFINITY, again = fresh || top > 15.0f;
+                if (fresh) m = top;
+                else if (top > 8.0f) grow = top;
+                if (!__any_sync(0xFFFFFFFFu, again)) break;
             }
-            float sum[4] = {};
-            tmem_ld32(t_s, x[0]);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                tmem_ld_wait();
-                if (q < 3) tmem_ld32(t_s + 32u * (q + 1), x[(q + 1) & 1]);
-                float (&v)[32] = x[q & 1];
-                uint32_t p[16];
-                if (simple) {
+                uint32_t y[16];
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) v[k] = ex2(fmaf(v[k], to_log2, -mu));
-                } else {
-                    const uint32_t bits = sees(q), bad = bits & po[q];
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        const float e = ex2(fmaf(v[k], to_log2, -mu));
-                        v[k] = bits >> k & 1u ? (bad >> k & 1u ? __int_as_float(0x7FC00000) : e) : 0.0f;
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < 32; ++k) sum[k & 3] += v[k];
-#pragma unroll
-                for (int k = 0; k < 16; ++k) p[k] = pack_half2(v[2 * k], v[2 * k + 1]);
-                tmem_st16(t_s + 16u * q, p);             // over the quarter before it, which has been read
+                for (int k = 0; k < 16; ++k) y[k] = p[16 * q + k];
+                tmem_st16(t_s + 16u * q, y);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            l += sum;
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full(i));
         }
-        if (ok && steps > 0 && i < tiles) ok = warp_wait(finished, 0, s_abort, lane);
+        if (ok && steps > 0 && i < tiles) ok = park_warp(finished, 0, s_abort);
         if (work && ok && i < tiles) {
             tc_fence_after();
             const bool whole = a.splits == 1;
@@ -289,7 +395,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
                 float x[32] = {};
                 if (steps > 0) {
                     tmem_ld32(t_o + 32u * q, x);
-                    tmem_ld_wait();
+                    tmem_take32(x);
                 }
                 if (!mine) continue;
                 if (whole) {
@@ -312,6 +418,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
         }
     } else if (warp < kValueWarp) {
         // ================= keys: thread = position = row of the operand =================
+        fewer_registers<kOperandRegs>();
         const int t = tid & 127;
         uint4 w[4];
         uint32_t kp = 0, vp = 0;
@@ -339,7 +446,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
         }
         for (int j = 0; j < steps; ++j) {
             const int slot = j & 1;
-            if (!warp_wait(k_empty(slot), ((j >> 1) & 1) ^ 1, s_abort, lane)) break;
+            if (!park_warp(k_empty(slot), ((j >> 1) & 1) ^ 1, s_abort)) break;
             const uint32_t p = finite_params(kp);
             const __half2 s = __half2half2(__ushort_as_half(static_cast<unsigned short>(p))), z = __half2half2(__ushort_as_half(static_cast<unsigned short>(p >> 16)));
             const uint32_t here = __ballot_sync(0xFFFFFFFFu, there), bad = __ballot_sync(0xFFFFFFFFu, nan_params(vp));
@@ -365,6 +472,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
         }
     } else if (warp < kMmaWarp) {
         // ================= values =================
+        fewer_registers<kOperandRegs>();
         const int t = tid & 127, word = (lane >> 3) + 4 * (warp - kValueWarp);
         uint32_t vp = 0;
         int page = -1;
@@ -398,7 +506,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
             params[t] = nan_params(vp) ? 0u : finite_params(vp);
             asm volatile("bar.sync 1, 128;" ::: "memory");        // every position's codes and parameters are there, and the step before has been read
             if (j + 1 < steps) fetch(j + 1);
-            if (!warp_wait(v_empty(slot), ((j >> 1) & 1) ^ 1, s_abort, lane)) break;
+            if (!park_warp(v_empty(slot), ((j >> 1) & 1) ^ 1, s_abort)) break;
             uint8_t* to = smem + kSmemV + slot * kOperand;
             const uint8_t* stage = smem + kSmemStage + slot * kValueStage;
 #pragma unroll
@@ -428,48 +536,54 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
             if (lane == 0) mbar_arrive(v_full(slot));
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
-    } else if (steps > 0) {
+    } else {
         // ================= MMA issue: one thread =================
-        if (elect_one()) {
-            const uint32_t idesc = make_idesc(kTile);
-            auto scores = [&](int i, int slot) {
-                const uint64_t qd = make_smem_desc(smem0 + static_cast<uint32_t>(i * kOperand)), kd = make_smem_desc(smem0 + static_cast<uint32_t>(kSmemK + slot * kOperand));
+        fewer_registers<kIssueRegs>();
+        if (warp == kMmaWarp && steps > 0 && elect_one()) {
+            constexpr uint32_t idesc = (1u << 4) | ((kTile >> 3) << 17) | ((kTile >> 4) << 24);      // D fp32, A and B fp16, both K-major
+            const uint32_t qd = desc_low(smem0), kd = desc_low(smem0 + kSmemK), vd = desc_low(smem0 + kSmemV);
+            constexpr uint32_t kNext = kOperand >> 4;
+            // tile and slot are constants, so that nothing but the loop's own counters is computed here
+            auto scores = [&]<int I, int SLOT>() {
 #pragma unroll
                 for (int ks = 0; ks < 8; ++ks) {
                     const uint32_t off = (ks >= 4 ? kPanel >> 4 : 0) + 2u * (ks & 3);
-                    tc_mma_f16_ss(tmem + static_cast<uint32_t>(i * 128), qd + off, kd + off, idesc, ks != 0);
+                    mma_ss(tmem + static_cast<uint32_t>(I * 128), qd + (I * kNext + off), kd + (SLOT * kNext + off), idesc, ks != 0);
                 }
-                tc_commit(s_full(i));
+                tc_commit(s_full(I));
             };
-            bool ok = mbar_wait(q_full, 0, s_abort) && mbar_wait(k_full(0), 0, s_abort);
+            bool ok = park_wait(q_full, 0, s_abort) && park_wait(k_full(0), 0, s_abort);
             if (ok) {
                 tc_fence_after();
-                for (int i = 0; i < tiles; ++i) scores(i, 0);
+                scores.template operator()<0, 0>();
+                if (tiles == 2) scores.template operator()<1, 0>();
                 tc_commit(k_empty(0));
             }
-            for (int j = 0; ok && j < steps; ++j) {
-                const int slot = j & 1, next = slot ^ 1;
-                ok = mbar_wait(v_full(slot), (j >> 1) & 1, s_abort);
-                for (int i = 0; ok && i < tiles; ++i) {
-                    ok = mbar_wait(p_full(i), j & 1, s_abort);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint64_t vd = make_smem_desc(smem0 + static_cast<uint32_t>(kSmemV + slot * kOperand));
+            auto outputs = [&]<int I, int SLOT>(int j) {
+                if (!park_wait(p_full(I), j & 1, s_abort)) return false;
+                tc_fence_after();
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks)
-                        tc_mma_f16_ts(tmem + static_cast<uint32_t>(kTmemO + i * 128), tmem + static_cast<uint32_t>(i * 128 + 8 * ks),
-                                      vd + ((ks >= 4 ? kPanel >> 4 : 0) + 2u * (ks & 3)), idesc, j != 0 || ks != 0);
-                    if (j + 1 < steps) {
-                        if (i == 0) {
-                            ok = mbar_wait(k_full(next), ((j + 1) >> 1) & 1, s_abort);
-                            if (!ok) break;
-                            tc_fence_after();
-                        }
-                        scores(i, next);
+                for (int ks = 0; ks < 8; ++ks)
+                    mma_ts(tmem + static_cast<uint32_t>(kTmemO + I * 128), tmem + static_cast<uint32_t>(I * 128 + 8 * ks),
+                                  vd + (SLOT * kNext + (ks >= 4 ? kPanel >> 4 : 0) + 2u * (ks & 3)), idesc, j != 0 || ks != 0);
+                if (j + 1 < steps) {
+                    if (I == 0) {
+                        if (!park_wait(k_full(SLOT ^ 1), ((j + 1) >> 1) & 1, s_abort)) return false;
+                        tc_fence_after();
                     }
+                    scores.template operator()<I, (SLOT ^ 1)>();
                 }
-                if (j + 1 < steps) tc_commit(k_empty(next));
-                tc_commit(v_empty(slot));
+                return true;
+            };
+            auto step = [&]<int SLOT>(int j) {
+                ok = park_wait(v_full(SLOT), (j >> 1) & 1, s_abort) && outputs.template operator()<0, SLOT>(j) &&
+                     (tiles == 1 || outputs.template operator()<1, SLOT>(j));
+                if (j + 1 < steps) tc_commit(k_empty(SLOT ^ 1));
+                tc_commit(v_empty(SLOT));
+            };
+            for (int j = 0; ok && j < steps; j += 2) {
+                step.template operator()<0>(j);
+                if (ok && j + 1 < steps) step.template operator()<1>(j + 1);
             }
             tc_commit(finished);
         }
@@ -478,7 +592,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
     tc_fence_before();
     __syncthreads();
     if (*s_abort) __nanosleep(500000);      // a bounded wait ran out: what is in flight lands before the memory goes
-    if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+    if (warp == kMmaWarp) tmem_dealloc(s_tmem, 512);
 }
 
 // The splits of a (tile, head) joined, a warp a row.
