@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv4_attention_join_kernel(con
 // tokens of two sequences of 32 000 and 20 000 positions, 32 heads on 8, took 111 us).
 constexpr int kWeightRows = 128, kWeightPositions = 32 * kAttnWarps;
 
-__global__ void __launch_bounds__(kAttnThreads, 4) kv4_key_weight_kernel(const __grid_constant__ Kv4WeightArgs a) {
+__global__ void __launch_bounds__(kAttnThreads, 3) kv4_key_weight_kernel(const __grid_constant__ Kv4WeightArgs a) {
     __shared__ uint4 s_q[kWeightRows / 8][4][32];
     __shared__ float2 s_row[kWeightRows];                    // sum of q, -lse, both in the exponent's units
     pdl_wait_prior_grids();
@@ -544,33 +544,40 @@ __global__ void __launch_bounds__(kAttnThreads, 4) kv4_key_weight_kernel(const _
             raw.page[1] = next[1];
             fetch(at + kWeightPositions);
             pages(at + 2 * kWeightPositions, next);
-            const bool all_see = at + 32 <= past + r0 / a.group + 1;
-            for (int n = 0; n < staged / 8; ++n) {
-                float even[2][4] = {}, s[2][4] = {};
+            auto add_rows = [&]<bool CUT>() {               // CUT: some row does not see some of these positions
+                for (int n = 0; n < staged / 8; ++n) {
+                    float even[2][4] = {}, s[2][4] = {};
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint4 f = s_q[n][j][lane];
+                    for (int j = 0; j < 4; ++j) {
+                        const uint4 f = s_q[n][j][lane];
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const uint32_t a0[4] = {codes[u][j][0][0], codes[u][j][1][0], codes[u][j][0][2], codes[u][j][1][2]};
-                        const uint32_t a1[4] = {codes[u][j][0][1], codes[u][j][1][1], codes[u][j][0][3], codes[u][j][1][3]};
-                        mma_16816(even[u], a0, f.x, f.y);
-                        mma_16816(s[u], a1, f.z, f.w);
+                        for (int u = 0; u < 2; ++u) {
+                            const uint32_t a0[4] = {codes[u][j][0][0], codes[u][j][1][0], codes[u][j][0][2], codes[u][j][1][2]};
+                            const uint32_t a1[4] = {codes[u][j][0][1], codes[u][j][1][1], codes[u][j][0][3], codes[u][j][1][3]};
+                            mma_16816(even[u], a0, f.x, f.y);
+                            mma_16816(s[u], a1, f.z, f.w);
+                        }
+                    }
+                    const float4 row = *reinterpret_cast<const float4*>(&s_row[n * 8 + 2 * t]);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float qs = e ? row.z : row.x, less = e ? row.w : row.y;
+                        int limit = 0;
+                        if constexpr (CUT) {
+                            const int r = r0 + n * 8 + 2 * t + e;
+                            limit = r < rows ? past + r / a.group + 1 : 0;
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float x = fmaf(kv4_key_sum(even[k >> 1][2 * (k & 1) + e], s[k >> 1][2 * (k & 1) + e]), ks[k], fmaf(kz[k], qs, less));
+                            const float p = ex2(x);
+                            if (!CUT || at + 8 * k + g < limit) got[k] += p;
+                        }
                     }
                 }
-                const float4 row = *reinterpret_cast<const float4*>(&s_row[n * 8 + 2 * t]);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float qs = e ? row.z : row.x, less = e ? row.w : row.y;
-                    const int r = r0 + n * 8 + 2 * t + e, limit = all_see ? 0x7FFFFFFF : r < rows ? past + r / a.group + 1 : 0;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float x = fmaf(kv4_key_sum(even[k >> 1][2 * (k & 1) + e], s[k >> 1][2 * (k & 1) + e]), ks[k], fmaf(kz[k], qs, less));
-                        const float p = ex2(x);
-                        got[k] += all_see || at + 8 * k + g < limit ? p : 0.0f;
-                    }
-                }
-            }
+            };
+            if (at + 32 <= past + r0 / a.group + 1) add_rows.template operator()<false>();
+            else add_rows.template operator()<true>();
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 got[k] += __shfl_xor_sync(0xFFFFFFFFu, got[k], 1);
@@ -616,9 +623,10 @@ int kv4_attention(Kv4AttentionArgs a, int q_heads, bool f32, void* workspace, cu
 
 int kv4_add_key_weights(Kv4WeightArgs a, cudaStream_t stream) {
     const Kv4View& c = a.c;
-    // as many positions a CTA as leave each SM four CTAs where the tables are as long as the sequences; 128 at least, 2048 at most
+    // as many positions a CTA as leave each SM six CTAs, two rounds of three, where the tables are as long as the sequences; 128 at
+    // least, 2048 at most
     const long long capacity = static_cast<long long>(c.max_pages) << c.page_shift;
-    const long long each = capacity * c.kv_heads * c.num_seqs / (148 * 4);
+    const long long each = capacity * c.kv_heads * c.num_seqs / (148 * 6);
     a.positions = static_cast<int>(each < kWeightPositions ? kWeightPositions : each > 2048 ? 2048 : each / kWeightPositions * kWeightPositions);
     const long long blocks = (capacity + a.positions - 1) / a.positions;
     if (blocks > 0x7FFFFFFFll / a.positions) return W4A16_ERR_TOO_LARGE;
