@@ -6,7 +6,7 @@
 namespace w4 {
 namespace {
 
-constexpr int kRowThreads = 16;          // a row is a half-warp's: 8 values a lane
+constexpr int kRowThreads = 16;          // a row is a half-warp's
 constexpr int kAppendThreads = 256;      // 16 rows a CTA
 
 struct AppendArgs {
@@ -18,14 +18,12 @@ struct AppendArgs {
     int q_heads, q_stride, kv_stride, blocks_per_token;
 };
 
-__device__ __forceinline__ void half8_to_float(const uint4& w, float (&x)[8]) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-        x[2 * i] = f.x;
-        x[2 * i + 1] = f.y;
-    }
+__device__ __forceinline__ void half4_to_float(uint2 w, float* x) {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+    x[0] = a.x;
+    x[1] = a.y;
+    x[2] = b.x;
+    x[3] = b.y;
 }
 __device__ __forceinline__ uint4 float_to_half8(const float (&x)[8]) {
     uint32_t u[4];
@@ -37,45 +35,59 @@ __device__ __forceinline__ uint4 float_to_half8(const float (&x)[8]) {
     return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
-// One row of 128 fp16 values, 8 a lane of a half-warp, to its code word and (scale, zero).  Both halves of a warp call it.
-// The codes are those of the formula in IEEE arithmetic: a product with the reciprocal is off by less than 1e-5 (|quotient|
-// < 11), so only where that lands nearer than this to a border between two codes is the division made.  A row with an infinity
-// or a NaN gets a NaN scale: it reads back as NaN instead of as finite values that it does not hold.
-__device__ __forceinline__ uint32_t kv4_quantise_lane(const float (&x)[8], uint32_t* params) {
-    float lo = x[0], hi = x[0];
-    bool finite = true;
+// A row of 128 fp16 values in a half-warp: lane hl has 4 hl .. 4 hl + 3 and the same + 64, so that both values of a rotated pair are its
+// own.  Returns the code word that the lane stores, number kv4_word_of(hl), and the row's (scale, zero).  Both halves of a warp call it.
+// The codes are those of the formula in IEEE arithmetic: a product with the reciprocal is off by less than 1e-5 (|quotient| < 11), so
+// only where one lands nearer than that to a border between two codes are the divisions made.  A row with an infinity or a NaN gets
+// a NaN scale: it reads back as NaN instead of as finite values that it does not hold.
+__device__ __forceinline__ int kv4_word_of(int hl) { return (hl & 1) * 8 + (hl >> 1); }
+__device__ __forceinline__ uint32_t kv4_quantise_lane(const __half2 (&h)[4], int hl, uint32_t* params) {
+    __half2 lo2 = __hmin2_nan(__hmin2_nan(h[0], h[1]), __hmin2_nan(h[2], h[3])), hi2 = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    // (smallest, minus the largest), so that one minimum reduces both
+    __half2 ends = __halves2half2(__hmin_nan(__low2half(lo2), __high2half(lo2)), __hneg(__hmax_nan(__low2half(hi2), __high2half(hi2))));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        lo = fminf(lo, x[j]);
-        hi = fmaxf(hi, x[j]);
-        finite = finite && fabsf(x[j]) <= 65504.0f;
-    }
-#pragma unroll
-    for (int m = 8; m > 0; m >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, m));
-        hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, m));
-    }
-    const uint32_t all = __ballot_sync(0xFFFFFFFFu, finite);
-    const bool row_finite = ((threadIdx.x & 16 ? all >> 16 : all) & 0xFFFFu) == 0xFFFFu;
+    for (int m = 8; m > 0; m >>= 1) ends = __hmin2_nan(ends, __shfl_xor_sync(0xFFFFFFFFu, ends, m));
+    const float lo = __low2float(ends), hi = -__high2float(ends);
+    const bool finite = lo >= -65504.0f && hi <= 65504.0f;                  // false for a NaN
     __half scale = __float2half_rn(__fdiv_rn(hi - lo, 15.0f));
     const float s = __half2float(scale);
     __half zero = __float2half_rn(__fadd_rn(lo, 8.0f * s));
     const float z = __half2float(zero);
-    uint32_t word = 0x88888888u;
-    constexpr int kShift[8] = {0, 8, 16, 24, 4, 12, 20, 28};
-    if (row_finite && s > 0.0f) {
-        word = 0;
+    uint32_t part[2] = {0x08080808u, 0x08080808u};
+    if (finite && s > 0.0f) {
         const float inv = __frcp_rn(s);
+        constexpr float kRound = 12582912.0f;                               // 1.5 * 2^23: adding it leaves the nearest integer in the low bits
+        float d[8], t[8], off = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 f = __half22float2(h[j]);
+            d[2 * j] = f.x - z;
+            d[2 * j + 1] = f.y - z;
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            float t = (x[j] - z) * inv;
-            if (fabsf(fabsf(t - rintf(t)) - 0.5f) < 2e-5f) t = __fdiv_rn(x[j] - z, s);
-            word |= static_cast<uint32_t>(min(max(__float2int_rn(t) + 8, 0), 15)) << kShift[j];
+            t[j] = d[j] * inv;
+            off = fmaxf(off, fabsf(t[j] - (__fadd_rn(t[j], kRound) - kRound)));
+        }
+        if (off > 0.5f - 2e-5f) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] = __fdiv_rn(d[j], s);
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            part[q] = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float r = fminf(fmaxf(t[4 * q + j], -8.0f), 7.0f);     // rounds to the same code as what it cuts off
+                part[q] |= (__float_as_uint(__fadd_rn(r, kRound + 8.0f)) & 15u) << (8 * j);
+            }
         }
     }
-    if (!row_finite) scale = zero = __ushort_as_half(0x7FFF);
+    if (!finite) scale = zero = __ushort_as_half(0x7FFF);
     *params = static_cast<uint32_t>(__half_as_ushort(scale)) | (static_cast<uint32_t>(__half_as_ushort(zero)) << 16);
-    return word;
+    // an even lane has elements 0..3 of its words, an odd one 4..7; the even one finishes the first word, the odd one the second
+    const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, hl & 1 ? part[0] : part[1], 1);
+    return hl & 1 ? (part[1] << 4) | other : part[0] | (other << 4);
 }
 
 // Where a token of the batch goes.
@@ -105,7 +117,7 @@ __device__ __forceinline__ Spot find_spot(const Kv4View& c, int token) {     // 
 // CTA instead of four 4 prompts of up to 4100 tokens took 79 us.
 template <int TOK>
 __global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(const __grid_constant__ AppendArgs a) {
-    __shared__ float2 s_turn[TOK][kKvDim / 2];
+    __shared__ __align__(16) float2 s_turn[TOK][kKvDim / 2];     // cosine, sine
     __shared__ Spot s_spot[TOK];
     __shared__ int s_pos[TOK];
     pdl_wait_prior_grids();
@@ -119,14 +131,19 @@ __global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(const __grid
     const int kind = row < n_q ? 0 : row < n_q + c.kv_heads ? 1 : 2;
     const int head = row - (kind == 0 ? 0 : kind == 1 ? n_q : n_q + c.kv_heads);
     const bool on = row < rows;
-    const __half* src = (kind == 0 ? a.q : kind == 1 ? a.k : a.v) + head * kKvDim + hl * 8;
+    const __half* src = (kind == 0 ? a.q : kind == 1 ? a.k : a.v) + head * kKvDim + hl * 4;
     const int stride = kind == 0 ? a.q_stride : a.kv_stride;
-    uint4 raw[TOK], bias = make_uint4(0, 0, 0, 0);
+    uint2 raw[TOK][2], bias[2] = {make_uint2(0, 0), make_uint2(0, 0)};
 #pragma unroll
     for (int i = 0; i < TOK; ++i)
-        raw[i] = on && token0 + i < c.num_tokens ? __ldcg(reinterpret_cast<const uint4*>(src + static_cast<size_t>(token0 + i) * stride)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+            raw[i][p] = on && token0 + i < c.num_tokens ? __ldcg(reinterpret_cast<const uint2*>(src + static_cast<size_t>(token0 + i) * stride + 64 * p)) : make_uint2(0, 0);
     const __half* b = kind == 0 ? a.q_bias : kind == 1 ? a.k_bias : a.v_bias;
-    if (on && b != nullptr) bias = __ldcg(reinterpret_cast<const uint4*>(b + head * kKvDim + hl * 8));
+    if (on && b != nullptr) {
+#pragma unroll
+        for (int p = 0; p < 2; ++p) bias[p] = __ldcg(reinterpret_cast<const uint2*>(b + head * kKvDim + hl * 4 + 64 * p));
+    }
     if (warp < TOK) {
         const int token = token0 + warp;
         int pos = 0;
@@ -148,37 +165,42 @@ __global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(const __grid
     }
     __syncthreads();
     float bf[8];
-    half8_to_float(bias, bf);
+    half4_to_float(bias[0], bf);
+    half4_to_float(bias[1], bf + 4);
     const int ps = 1 << c.page_shift, part = kind - 1;
 #pragma unroll
     for (int i = 0; i < TOK; ++i) {
         const Spot s = s_spot[i];
         if (s.seq < 0) continue;                                 // behind the last sequence: left as it is
-        float x[8];
-        half8_to_float(raw[i], x);
+        float x[8];                                              // four values and the four 64 behind them
+        half4_to_float(raw[i][0], x);
+        half4_to_float(raw[i][1], x + 4);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] += bf[j];
-        if (a.inv_freq != nullptr) {
-            // values d and d + 64 are a pair: lanes hl and hl ^ 8
+        if (a.inv_freq != nullptr && kind != 2) {
+            const float4 t01 = reinterpret_cast<const float4*>(s_turn[i])[2 * hl], t23 = reinterpret_cast<const float4*>(s_turn[i])[2 * hl + 1];
+            const float cs[4] = {t01.x, t01.z, t23.x, t23.z}, sn[4] = {t01.y, t01.w, t23.y, t23.w};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float other = __shfl_xor_sync(0xFFFFFFFFu, x[j], 8);
-                const float2 t = s_turn[i][(hl & 7) * 8 + j];
-                if (kind != 2) x[j] = hl < 8 ? x[j] * t.x - other * t.y : x[j] * t.x + other * t.y;
+            for (int j = 0; j < 4; ++j) {
+                const float u = x[j], v = x[j + 4];
+                x[j] = u * cs[j] - v * sn[j];
+                x[j + 4] = v * cs[j] + u * sn[j];
             }
         }
-        const uint4 rounded = float_to_half8(x);
-        if (on && kind == 0)
-            *reinterpret_cast<uint4*>(a.q_out + static_cast<size_t>(token0 + i) * a.q_stride + head * kKvDim + hl * 8) = rounded;
+        const __half2 h[4] = {__floats2half2_rn(x[0], x[1]), __floats2half2_rn(x[2], x[3]), __floats2half2_rn(x[4], x[5]), __floats2half2_rn(x[6], x[7])};
+        if (on && kind == 0) {
+            __half* out = a.q_out + static_cast<size_t>(token0 + i) * a.q_stride + head * kKvDim + hl * 4;
+            *reinterpret_cast<uint2*>(out) = make_uint2(*reinterpret_cast<const uint32_t*>(&h[0]), *reinterpret_cast<const uint32_t*>(&h[1]));
+            *reinterpret_cast<uint2*>(out + 64) = make_uint2(*reinterpret_cast<const uint32_t*>(&h[2]), *reinterpret_cast<const uint32_t*>(&h[3]));
+        }
         const bool stored = on && kind != 0 && s.page >= 0;
         if (__any_sync(0xFFFFFFFFu, stored)) {
-            half8_to_float(rounded, x);
             uint32_t params;
-            const uint32_t word = kv4_quantise_lane(x, &params);
+            const uint32_t word = kv4_quantise_lane(h, hl, &params);
             if (stored) {
                 uint32_t* record = kv4_record_of_page(c, s.page, head);
                 const int slot = s.at & (ps - 1);
-                record[(part * ps + slot) * kKvRowWords + hl] = word;
+                record[(part * ps + slot) * kKvRowWords + kv4_word_of(hl)] = word;
                 if (hl == 0) {
                     record[(32 + part) * ps + slot] = params;
                     if (kind == 1 && c.key_weight != nullptr) c.key_weight[kv4_weight_index(c, s.page, head, s.at)] = 0.0f;
