@@ -437,7 +437,8 @@ W4A16_API int w4a16_gemm_prefill_dual_gate_up_swiglu_w4a16(const uint32_t* gate_
  * The pool is uint32 [num_pages][num_kv_heads][34 * page_size]; a record is
  *   key codes [page_size][16] | value codes [page_size][16] | key (scale, zero) [page_size] | value (scale, zero) [page_size]
  * with code words packed as the weight words above and (scale, zero) an fp16 pair, scale in the low half.
- * page_size is a power of two from 16 to 4096.
+ * page_size is a power of two from 16 to 4096.  Sizes beyond 2^24 tokens, 2^30 query rows (tokens x heads), 65535 sequences or heads, or
+ * 2^30 positions a block table row give W4A16_ERR_TOO_LARGE.
  */
 typedef struct w4a16_kv4_cache {
     void* pages;               /* the pool, 16-byte aligned */
@@ -487,7 +488,10 @@ W4A16_API int w4a16_kv4_read(const w4a16_kv4_cache* cache, const w4a16_kv4_batch
  * w4a16_gemv_attn_heads_f32_w4a16 takes), [num_tokens][num_q_heads][128]; lse (may be NULL): fp32
  * [num_tokens][num_q_heads], the logarithm of the sum of exp(softmax_scale * q . key_j).  A token that sees nothing
  * gives zeros and -infinity.  workspace: w4a16_attention_kv4_workspace_bytes() of device memory that no other call in
- * flight uses (nothing is kept in it between calls); NULL where that is 0.
+ * flight uses, two replayed graphs that may run at the same time included (nothing is kept in it between calls).  out must
+ * not overlap q.
+ * Two forms: fp16 results of at least 64 query rows a sequence and head (tokens x shared heads, on average) run on tcgen05 with
+ * keys, values and weights rounded to fp16; all others keep keys and values exact, and 32-bit results weights too.
  */
 W4A16_API int64_t w4a16_attention_kv4_workspace_bytes(int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads);
 W4A16_API int w4a16_attention_kv4(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, const void* q, void* out,
@@ -506,9 +510,9 @@ W4A16_API int w4a16_kv4_add_key_weights(const w4a16_kv4_cache* cache, const w4a1
 /*
  * Cuts every sequence down to `budget` positions, each head by itself: its first num_sink, its last num_recent, and of
  * the rest those with the largest key_weight (the earlier of equal ones; a NaN is the smallest).  What stays keeps its
- * order and is copied, rows and weights, to the pages of dst_block_table [num_seqs][dst_max_pages_per_seq], which must not
- * hold pages of the sequences being cut; the old pages are left as they are, so pages shared with other sequences are
- * safe.  Sequences that fit are copied whole.  new_seq_lens [num_seqs] = min(length, budget);
+ * order and is copied, rows and weights, to the pages of dst_block_table [num_seqs][dst_max_pages_per_seq]: pages of their own, none
+ * twice and none of the sequences being cut; the old pages are left as they are, so pages shared with other sequences are
+ * safe.  Sequences that fit are copied whole.  new_seq_lens [num_seqs] = min(length, budget), another array than seq_lens;
  * kept int32 [num_seqs][num_kv_heads][budget]: the old positions in order, -1 behind the last.  num_tokens and query_start
  * of the batch are not used.
  */

@@ -99,6 +99,7 @@ int kv4_view(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, Kv4View
         misaligned(batch->query_start, 4))
         return W4A16_ERR_ALIGNMENT;
     if (cache->num_kv_heads > 65535 || batch->num_seqs > 65535 || batch->num_tokens > (1 << 24)) return W4A16_ERR_TOO_LARGE;
+    if (static_cast<long long>(batch->max_pages_per_seq) * ps > (1ll << 30)) return W4A16_ERR_TOO_LARGE;
     int shift = 4;
     while ((1 << shift) < ps) ++shift;
     *v = Kv4View{static_cast<uint32_t*>(cache->pages), cache->key_weight, batch->block_table, batch->seq_lens, batch->query_start,
@@ -736,7 +737,8 @@ int w4a16_kv4_evict(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, 
     if (int st = kv4_view(cache, batch, &c)) return st;
     if (!c.key_weight || !dst_block_table || !new_seq_lens || !kept || dst_max_pages_per_seq <= 0 || budget <= 0 || num_sink < 0 || num_recent < 0)
         return W4A16_ERR_INVALID_ARG;
-    if (dst_block_table == batch->block_table) return W4A16_ERR_INVALID_ARG;
+    // in place: heads still read what another one has written
+    if (dst_block_table == batch->block_table || new_seq_lens == batch->seq_lens) return W4A16_ERR_INVALID_ARG;
     if (static_cast<long long>(num_sink) + num_recent > budget) return W4A16_ERR_SHAPE;
     if (static_cast<long long>(dst_max_pages_per_seq) * cache->page_size < budget) return W4A16_ERR_SHAPE;
     if (misaligned(dst_block_table, 4) || misaligned(new_seq_lens, 4) || misaligned(kept, 4)) return W4A16_ERR_ALIGNMENT;

@@ -43,7 +43,7 @@ __device__ __forceinline__ int2 kv4_new_tokens(const Kv4View& c, int b) {
     return make_int2(first, end - first);
 }
 __device__ __forceinline__ int kv4_capacity(const Kv4View& c) {
-    return static_cast<int>(min(static_cast<long long>(c.max_pages) << c.page_shift, 0x7FFFFFF0ll));
+    return c.max_pages << c.page_shift;       // at most 2^30: the entry points see to it
 }
 // The record of position `at` of a sequence and head; null where the table has no page of the pool there.
 __device__ __forceinline__ uint32_t* kv4_record_of_page(const Kv4View& c, int page, int head) {

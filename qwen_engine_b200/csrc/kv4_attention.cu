@@ -629,7 +629,6 @@ int kv4_add_key_weights(Kv4WeightArgs a, cudaStream_t stream) {
     const long long each = capacity * c.kv_heads * c.num_seqs / (148 * 6);
     a.positions = static_cast<int>(each < kWeightPositions ? kWeightPositions : each > 2048 ? 2048 : each / kWeightPositions * kWeightPositions);
     const long long blocks = (capacity + a.positions - 1) / a.positions;
-    if (blocks > 0x7FFFFFFFll / a.positions) return W4A16_ERR_TOO_LARGE;
     const dim3 grid(static_cast<unsigned>(blocks), c.kv_heads, c.num_seqs);
     return static_cast<int>(launch_kernel(kv4_key_weight_kernel, grid, dim3(kAttnThreads), 0, stream, pdl_enabled(), a));
 }

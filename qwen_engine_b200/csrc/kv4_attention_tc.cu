@@ -619,6 +619,11 @@ __global__ void __launch_bounds__(32 * kChunkJoinWarps) kv4_chunk_join_kernel(co
 }  // namespace
 
 int kv4_chunk_set_attributes() {
+    // the warpgroups trade registers against what a launch has: with fewer than 96 a thread they would wait for each other
+    cudaFuncAttributes f{};
+    const cudaError_t e = cudaFuncGetAttributes(&f, kv4_chunk_kernel);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    if (f.numRegs != 96) return static_cast<int>(cudaErrorInvalidKernelImage);
     return static_cast<int>(cudaFuncSetAttribute(kv4_chunk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kChunkSmem + 1024));
 }
 int kv4_chunk_timeouts(unsigned int* out) { return static_cast<int>(cudaMemcpyFromSymbol(out, g_tc_wait_timeouts, sizeof(unsigned int))); }

@@ -59,6 +59,7 @@ __device__ __forceinline__ bool find_unit(const Kv4View& c, int group, int tile_
         n.x += tiles * w.units;
         n.y += tiles;
     };
+#pragma unroll 4
     for (int b = b0; b < b1; ++b) {
         w = seq_work(c, b, group, tile_rows);
         count(mine);

@@ -207,7 +207,7 @@ def check_attention(got, lse, want, T, f32):
     if lse is not None:
         empty = np.isneginf(wl)
         assert np.array_equal(np.isneginf(lse[:T]), empty) and (lse[T] == 7).all()
-        assert np.all(np.abs(lse[:T] - wl)[~empty] <= el[~empty])
+        assert np.all(np.abs(lse[:T][~empty] - wl[~empty]) <= el[~empty])
 
 
 @pytest.mark.parametrize("f32", [True, False])
@@ -422,3 +422,127 @@ def test_decode_steps_between_qkv_and_o(ops):
     assert np.all(np.abs(util.to_np(acc) - want[0]) <= want[2])
     for h_ in range(kv):
         assert util.to_np(kept)[0, h_].tolist() == ref.evict(got, util.to_np(table)[0], steps, h_, page, 2 * per, 20, 2, 6)
+
+
+@pytest.mark.parametrize("tokens,f32", [(3, True), (60, False)])
+def test_rows_behind_the_last_sequence_are_left_alone(ops, tokens, f32):
+    lens, new, kv, heads, page = [70, 30], [tokens, 5], 2, 8, 16
+    rng, pool, table, cache, batch = make(ops, 11, lens, new, kv, page)
+    T = sum(new)
+    batch.num_tokens = T + 9
+    q = np.full((T + 9, heads, 128), np.nan, BF)
+    q[:T] = rng.standard_normal((T, heads, 128))
+    got, lse = attend(ops, cache, batch, util.to_dev(q), heads, f32)
+    few = few_rows(batch, heads, cache, f32)
+    check_attention(np.concatenate([got[:T], got[-1:]]), np.concatenate([lse[:T], lse[-1:]]), ref.attention(pool, table, lens, new, q[:T], SCALE, not few), T, f32)
+    assert (got[T:] == 7).all() and (lse[T:] == 7).all()
+    before = util.to_np(cache.key_weight).copy()
+    ops.kv4_add_key_weights(cache, batch, util.to_dev(q), util.to_dev(lse), heads, SCALE)
+    add, rel = ref.key_weights(pool, table, lens, new, q[:T], lse[:T].astype(np.float64), SCALE)
+    after = util.to_np(cache.key_weight)
+    assert np.all(np.abs(after - before - add) <= add * 2 * (rel + 2.0 ** -9 * (not few)) + np.abs(after) * 2.0 ** -22)
+
+
+@pytest.mark.parametrize("rows", [63, 64, 65])
+def test_both_sides_of_the_border_between_the_forms(ops, rows):
+    """One key/value head and one query head a sequence: a token is a row."""
+    lens, new, kv, heads, page = [300], [rows], 1, 1, 16
+    rng, pool, table, cache, batch = make(ops, 12, lens, new, kv, page)
+    q = rng.standard_normal((rows, heads, 128)).astype(BF)
+    got, lse = attend(ops, cache, batch, util.to_dev(q), heads, False)
+    check_attention(got, lse, ref.attention(pool, table, lens, new, q, SCALE, rows >= 64), rows, False)
+
+
+@pytest.mark.parametrize("lens,new,kv,heads,f32", [([900, 40], [1, 1], 2, 12, True), ([900, 40], [1, 1], 2, 12, False), ([900, 400], [5, 4], 2, 12, True),
+                                                   ([900, 400], [200, 100], 2, 12, False)])
+def test_the_same_call_gives_the_same_bits(ops, lens, new, kv, heads, f32):
+    """Twice, with programmatic dependent launch off, and out of a graph that is replayed after the lengths have changed and come back."""
+    rng, pool, table, cache, batch = make(ops, 13, lens, new, kv, 16)
+    T = sum(new)
+    q = util.to_dev(rng.standard_normal((T, heads, 128)).astype(BF))
+    first = attend(ops, cache, batch, q, heads, f32)
+    again = attend(ops, cache, batch, q, heads, f32)
+    ops.set_pdl(False)
+    try:
+        plain = attend(ops, cache, batch, q, heads, f32)
+    finally:
+        ops.set_pdl(True)
+    for other in (again, plain):
+        assert np.array_equal(first[0], other[0]) and np.array_equal(first[1], other[1])
+    out = torch.empty(T, heads, 128, dtype=torch.float32 if f32 else torch.float16, device="cuda")
+    lse = torch.empty(T, heads, device="cuda")
+    n = ops.attention_kv4_workspace_bytes(T, len(lens), heads, kv)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        ops.attention_kv4(cache, batch, q, out, lse, ws, heads, n, f32, SCALE)
+        ops.kv4_add_key_weights(cache, batch, q, lse, heads, SCALE)
+    short = [max(L // 3, k) for L, k in zip(lens, new)]
+    batch.seq_lens.copy_(i32(short))
+    graph.replay()
+    want = ref.attention(pool, table, short, new, util.to_np(q), SCALE, not few_rows(batch, heads, cache, f32))
+    check_attention(np.concatenate([util.to_np(out), np.full((1, heads, 128), 7)]), np.concatenate([util.to_np(lse), np.full((1, heads), 7.0)]), want, T, f32)
+    batch.seq_lens.copy_(i32(lens))
+    graph.replay()
+    assert np.array_equal(util.to_np(out), first[0][:T]) and np.array_equal(util.to_np(lse), first[1][:T])
+
+
+def test_two_streams_with_a_workspace_each(ops):
+    lens, kv, heads = [3000], 2, 12
+    rng, pool, table, cache, batch = make(ops, 14, lens, [1], kv, 64)
+    chunk = ops.KV4Batch.of(batch.block_table, batch.seq_lens, i32([0, 300]), 300)
+    q1, q2 = (util.to_dev(rng.standard_normal((n, heads, 128)).astype(BF)) for n in (1, 300))
+    want1, want2 = attend(ops, cache, batch, q1, heads, True)[0], attend(ops, cache, chunk, q2, heads, False)[0]
+    n1, n2 = ops.attention_kv4_workspace_bytes(1, 1, heads, kv), ops.attention_kv4_workspace_bytes(300, 1, heads, kv)
+    w1, w2 = (torch.empty(n, dtype=torch.uint8, device="cuda") for n in (n1, n2))
+    o1, o2 = torch.empty(1, heads, 128, device="cuda"), torch.empty(300, heads, 128, dtype=torch.float16, device="cuda")
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        ops.attention_kv4(cache, batch, q1, o1, None, w1, heads, n1, True, SCALE, stream=s1)
+        ops.attention_kv4(cache, chunk, q2, o2, None, w2, heads, n2, False, SCALE, stream=s2)
+    torch.cuda.synchronize()
+    assert np.array_equal(util.to_np(o1)[0], want1[0]) and np.array_equal(util.to_np(o2), want2[:300])
+
+
+def test_a_pool_of_more_than_4_gib(ops):
+    """The same sequences on the last pages of a pool whose offsets pass 32 bits: the same bits from every operator."""
+    lens, new, kv, heads, page = [500, 130], [70, 64], 2, 8, 64
+    rng, pool, table, small, batch = make(ops, 15, lens, new, kv, page)
+    n = pool.num_pages
+    record = kv * 34 * page * 4
+    big_n = (4 << 30) // record + 2 * n
+    pages = torch.zeros(big_n, kv, 34 * page, dtype=torch.int32, device="cuda")
+    assert (big_n - n) * record > 1 << 32
+    pages[-n:] = small.pages
+    weight = torch.zeros(big_n, kv, page, device="cuda")
+    weight[-n:] = small.key_weight
+    big = ops.KV4Cache(pages, weight, big_n, kv, page)
+    moved = ops.KV4Batch.of(batch.block_table + (big_n - n), batch.seq_lens, batch.query_start, batch.num_tokens)
+    T = sum(new)
+    q, k, v = (util.to_dev(rng.standard_normal((T, w * 128)).astype(BF)) for w in (heads, kv, kv))
+    results = []
+    for cache, b in ((small, batch), (big, moved)):
+        ops.kv4_append(cache, b, None, k, v, None, None, None, None, None, None, heads)
+        kr, vr = (torch.empty(T, kv, 128, dtype=torch.float16, device="cuda") for _ in range(2))
+        ops.kv4_read(cache, b, kr, vr)
+        out = [kr.clone(), vr.clone(), cache.pages[-n:].clone()]
+        for f32 in (True, False):
+            o, l = attend(ops, cache, b, q, heads, f32)
+            out += [torch.from_numpy(o), torch.from_numpy(l)]
+        lse = util.to_dev(l[:T])
+        ops.kv4_add_key_weights(cache, b, q, lse, heads, SCALE)
+        out.append(cache.key_weight[-n:].clone())
+        spare = [p for p in range(n) if p not in set(table.reshape(-1).tolist())]
+        dst = i32([[spare[0] + cache.num_pages - n], [spare[1] + cache.num_pages - n]])
+        kept, new_lens = i32(np.zeros((2, kv, 40))), i32([0, 0])
+        ops.kv4_evict(cache, b, dst, new_lens, kept, 1, 40, 4, 8)
+        out += [kept, new_lens, cache.pages[-n:].clone(), cache.key_weight[-n:].clone()]
+        results.append([util.to_np(t) for t in out])
+    for a, b in zip(*results):
+        assert np.array_equal(a, b, equal_nan=a.dtype.kind == "f")
+
+
+def test_waits_of_the_chunk_form_did_not_run_out(ops):
+    assert ops.debug_counter(0) == 0

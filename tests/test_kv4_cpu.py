@@ -31,7 +31,7 @@ def calls(lib, **changes):
     c, b = views(**{k: v for k, v in changes.items() if k in (
         "pages", "key_weight", "num_pages", "num_kv_heads", "page_size", "block_table", "seq_lens", "query_start", "num_seqs", "max_pages_per_seq", "num_tokens")})
     a = dict(q=P, k=P, v=P, q_bias=None, k_bias=None, v_bias=None, positions=None, inv=None, q_out=P, heads=12, q_stride=0, kv_stride=0, out=P, lse=P, ws=P,
-             ws_bytes=1 << 40, f32=0, scale=0.088, dst=2 * P, new_lens=P, kept=P, dst_pages=2, budget=32, sink=4, recent=8)
+             ws_bytes=1 << 40, f32=0, scale=0.088, dst=2 * P, new_lens=2 * P, kept=P, dst_pages=2, budget=32, sink=4, recent=8)
     a.update({k: v for k, v in changes.items() if k in a})
     return {
         "append": lib.w4a16_kv4_append(c, b, a["q"], a["k"], a["v"], a["q_bias"], a["k_bias"], a["v_bias"], a["positions"], a["inv"], a["q_out"], a["heads"],
@@ -58,7 +58,7 @@ REFUSED = [
     (dict(out=None), -1, {"attention"}), (dict(scale=0.0), -1, {"attention", "weights"}), (dict(scale=float("nan")), -1, {"attention", "weights"}),
     (dict(scale=float("inf")), -1, {"attention", "weights"}), (dict(ws=None), -1, {"attention"}), (dict(ws_bytes=16), -1, {"attention"}),
     (dict(ws=P + 8), -3, {"attention"}), (dict(lse=None), -1, {"weights"}), (dict(key_weight=None), -1, {"weights", "evict"}),
-    (dict(dst=None), -1, {"evict"}), (dict(dst=P), -1, {"evict"}), (dict(kept=None), -1, {"evict"}), (dict(new_lens=None), -1, {"evict"}),
+    (dict(dst=None), -1, {"evict"}), (dict(dst=P), -1, {"evict"}), (dict(new_lens=P), -1, {"evict"}), (dict(max_pages_per_seq=1 << 27), -5, ALL), (dict(kept=None), -1, {"evict"}), (dict(new_lens=None), -1, {"evict"}),
     (dict(budget=0), -1, {"evict"}), (dict(sink=-1), -1, {"evict"}), (dict(sink=30), -2, {"evict"}), (dict(budget=33), -2, {"evict"}),
     (dict(sink=2147483647, recent=2147483647), -2, {"evict"}),
 ]
