@@ -491,7 +491,7 @@ W4A16_API int w4a16_kv4_read(const w4a16_kv4_cache* cache, const w4a16_kv4_batch
  * flight uses, two replayed graphs that may run at the same time included (nothing is kept in it between calls).  out must
  * not overlap q.
  * Two forms: fp16 results of at least 64 query rows a sequence and head (tokens x shared heads, on average) run on tcgen05 with
- * keys, values and weights rounded to fp16; all others keep keys and values exact, and 32-bit results weights too.
+ * values and weights rounded to fp16; all others keep the values exact, and 32-bit results the weights too.  Keys never are.
  */
 W4A16_API int64_t w4a16_attention_kv4_workspace_bytes(int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads);
 W4A16_API int w4a16_attention_kv4(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, const void* q, void* out,

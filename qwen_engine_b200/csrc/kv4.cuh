@@ -69,20 +69,24 @@ __device__ __forceinline__ int kv4_seq_of_token(const Kv4View& c, int token) {
 __device__ __forceinline__ float kv4_scale(uint32_t params) { return __half2float(__ushort_as_half(static_cast<unsigned short>(params))); }
 __device__ __forceinline__ float kv4_zero(uint32_t params) { return __half2float(__ushort_as_half(static_cast<unsigned short>(params >> 16))); }
 
-// Four pairs of codes out of a word as fp16 numbers for the tensor cores: pair n holds the nibbles at bits 4 n and 16 + 4 n.  In
-// the low bits of a half a nibble is a subnormal number already, code * 2^-24 (n even) or code * 2^-20 (n odd), so a mask is all
-// the conversion there is.  Pairs of one kind go to one product, and the two sums are put together in 32 bits.
-__device__ __forceinline__ void kv4_key_codes(uint32_t w, uint32_t (&out)[4]) {
+// Four pairs (code - 8) out of a word as fp16: pair n holds the nibbles at bits 4 n and 16 + 4 n.  0x6400 | c is 1024 + c and
+// 0x6400 | c << 4 is 1024 + 16 c, so one addition or one fma gives c - 8, exactly.  (In the low bits of a half a nibble is a subnormal
+// number already, and a mask would do for keys; but the tensor core lines products up by their exponents, a subnormal's has leading
+// zeros behind it, and 32-bit results were off by 2e-6 where they are now by 3e-7, for 3 % of a large batch's time.)
+__device__ __forceinline__ void kv4_centred_codes(uint32_t w, uint32_t (&out)[4]) {
+    const __half2 a = __float2half2_rn(-1032.0f), m = __float2half2_rn(0.0625f), b = __float2half2_rn(-72.0f);
     const uint32_t u = w >> 8;
-    out[0] = w & 0x000F000Fu;
-    out[1] = w & 0x00F000F0u;
-    out[2] = u & 0x000F000Fu;
-    out[3] = u & 0x00F000F0u;
+    uint32_t r[4];
+    asm("lop3.b32 %0, %1, 0x000F000F, 0x64006400, 0xEA;" : "=r"(r[0]) : "r"(w));
+    asm("lop3.b32 %0, %1, 0x00F000F0, 0x64006400, 0xEA;" : "=r"(r[1]) : "r"(w));
+    asm("lop3.b32 %0, %1, 0x000F000F, 0x64006400, 0xEA;" : "=r"(r[2]) : "r"(u));
+    asm("lop3.b32 %0, %1, 0x00F000F0, 0x64006400, 0xEA;" : "=r"(r[3]) : "r"(u));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 c = *reinterpret_cast<const __half2*>(&r[i]), v = i & 1 ? __hfma2(c, m, b) : __hadd2(c, a);
+        out[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
 }
-// score = scale * sum(q code) + (zero - 8 scale) * sum(q), from the sums over the two kinds of pairs.
-__device__ __forceinline__ float kv4_key_sum(float even, float odd) { return fmaf(even, 16.0f, odd); }
-constexpr float kKvKeyUndo = 1048576.0f;      // 2^20, on the scale
-
 // The same for values, whose nibble places are different rows of A: pair n holds (code - 7.5) times 2^-9 (n even) or 2^-5
 // (n odd), which the row's sums carry to the end.  One fma takes the subnormal numbers there; codes taken around 7.5, their mean, leave sums that do not grow with the number of positions, where the
 // tensor core's truncation would all go one way (at 131 001 positions the output's error against 64 bits fell from 6.5e-6).

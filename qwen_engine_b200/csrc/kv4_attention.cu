@@ -6,8 +6,8 @@
 // head has query heads, and these, not the positions, are what is padded.  The rows of a head (token major) are cut into tiles
 // of 8 or 16; a tile's positions are split over CTAs, a CTA's over its four warps, 16 positions at a time.
 //
-//   scores^T [16 positions x 8 queries] = codes [16 x 128] . q^T;  then scale * score + (zero - 8 scale) * (sum of q), because a
-//       row is (code - 8) * scale + zero: the codes are exact in fp16 and no key is ever rounded.
+//   scores^T [16 positions x 8 queries] = codes [16 x 128] . q^T;  then scale * score + zero * (sum of q), because a row is
+//       (code - 8) * scale + zero: the codes are exact in fp16 and no key is ever rounded.
 //   out^T [128 x 8] += codes^T [128 x 16] . (p * value scale)^T: for a 32-bit result the weight enters as two fp16 numbers
 //       whose sum has 22 bits, for an fp16 result as one (2^-12 of a weight is less than the result's own rounding, and
 //       the weights' roundings average out); zeros enter as one 32-bit sum a query.
@@ -84,17 +84,6 @@ struct TileCopy {
 __device__ __forceinline__ uint4 query_words(const uint4& w) {
     return make_uint4(__byte_perm(w.x, w.y, 0x5410), __byte_perm(w.x, w.y, 0x7632), __byte_perm(w.z, w.w, 0x5410), __byte_perm(w.z, w.w, 0x7632));
 }
-__device__ __forceinline__ float sum_half8(const uint4& w) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-        s += f.x + f.y;
-    }
-    return s;
-}
-
 template <int NT, bool F32>
 __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_kernel(const __grid_constant__ Kv4AttentionArgs a) {
     constexpr int R = 8 * NT, kPitch = kKvDim + 4;
@@ -179,18 +168,18 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) r.v[i] = *reinterpret_cast<const uint2*>(st + value_from + 256 * i);
-        float even[NT][4] = {}, s[NT][4] = {};
+        float s[NT][4] = {};
         const uint32_t kw0[4] = {r.k[0].x, r.k[0].y, r.k[0].z, r.k[0].w}, kw1[4] = {r.k[1].x, r.k[1].y, r.k[1].z, r.k[1].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             uint32_t lo[4], hi[4];
-            kv4_key_codes(kw0[j], lo);
-            kv4_key_codes(kw1[j], hi);
+            kv4_centred_codes(kw0[j], lo);
+            kv4_centred_codes(kw1[j], hi);
             const uint32_t a0[4] = {lo[0], hi[0], lo[2], hi[2]}, a1[4] = {lo[1], hi[1], lo[3], hi[3]};
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const uint4 b = s_q[n][j][lane];
-                mma_16816(even[n], a0, b.x, b.y);
+                mma_16816(s[n], a0, b.x, b.y);
                 mma_16816(s[n], a1, b.z, b.w);
             }
         }
@@ -198,8 +187,8 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             ks[i] = kv4_scale(r.kp[i]);
-            kz[i] = fmaf(-8.0f, ks[i], kv4_zero(r.kp[i]));
-            ks[i] *= to_log2 * kKvKeyUndo;
+            kz[i] = kv4_zero(r.kp[i]);
+            ks[i] *= to_log2;
             vs[i] = kv4_scale(r.vp[i]);
             vz[i] = fmaf(-0.5f, vs[i], kv4_zero(r.vp[i]));  // codes are taken around 7.5
         }
@@ -207,7 +196,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = fmaf(kv4_key_sum(even[n][e], s[n][e]), ks[e >> 1], kz[e >> 1] * qsum[n][e & 1]);
+            for (int e = 0; e < 4; ++e) s[n][e] = fmaf(s[n][e], ks[e >> 1], kz[e >> 1] * qsum[n][e & 1]);
         if constexpr (CUT) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -527,12 +516,12 @@ __global__ void __launch_bounds__(kAttnThreads, 3) kv4_key_weight_kernel(const _
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 ks[k] = kv4_scale(raw.params[k]);
-                kz[k] = fmaf(-8.0f, ks[k], kv4_zero(raw.params[k]));
-                ks[k] *= to_log2 * kKvKeyUndo;
-                kv4_key_codes(raw.w[k].x, codes[k >> 1][0][k & 1]);
-                kv4_key_codes(raw.w[k].y, codes[k >> 1][1][k & 1]);
-                kv4_key_codes(raw.w[k].z, codes[k >> 1][2][k & 1]);
-                kv4_key_codes(raw.w[k].w, codes[k >> 1][3][k & 1]);
+                kz[k] = kv4_zero(raw.params[k]);
+                ks[k] *= to_log2;
+                kv4_centred_codes(raw.w[k].x, codes[k >> 1][0][k & 1]);
+                kv4_centred_codes(raw.w[k].y, codes[k >> 1][1][k & 1]);
+                kv4_centred_codes(raw.w[k].z, codes[k >> 1][2][k & 1]);
+                kv4_centred_codes(raw.w[k].w, codes[k >> 1][3][k & 1]);
                 const int p = at + 8 * k + g;
                 weight[k] = nullptr;
                 if (t == 0 && p < end && static_cast<unsigned>(raw.page[k >> 1]) < static_cast<unsigned>(c.num_pages)) {
@@ -546,7 +535,7 @@ __global__ void __launch_bounds__(kAttnThreads, 3) kv4_key_weight_kernel(const _
             pages(at + 2 * kWeightPositions, next);
             auto add_rows = [&]<bool CUT>() {               // CUT: some row does not see some of these positions
                 for (int n = 0; n < staged / 8; ++n) {
-                    float even[2][4] = {}, s[2][4] = {};
+                    float s[2][4] = {};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const uint4 f = s_q[n][j][lane];
@@ -554,7 +543,7 @@ __global__ void __launch_bounds__(kAttnThreads, 3) kv4_key_weight_kernel(const _
                         for (int u = 0; u < 2; ++u) {
                             const uint32_t a0[4] = {codes[u][j][0][0], codes[u][j][1][0], codes[u][j][0][2], codes[u][j][1][2]};
                             const uint32_t a1[4] = {codes[u][j][0][1], codes[u][j][1][1], codes[u][j][0][3], codes[u][j][1][3]};
-                            mma_16816(even[u], a0, f.x, f.y);
+                            mma_16816(s[u], a0, f.x, f.y);
                             mma_16816(s[u], a1, f.z, f.w);
                         }
                     }
@@ -569,7 +558,7 @@ __global__ void __launch_bounds__(kAttnThreads, 3) kv4_key_weight_kernel(const _
                         }
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            const float x = fmaf(kv4_key_sum(even[k >> 1][2 * (k & 1) + e], s[k >> 1][2 * (k & 1) + e]), ks[k], fmaf(kz[k], qs, less));
+                            const float x = fmaf(s[k >> 1][2 * (k & 1) + e], ks[k], fmaf(kz[k], qs, less));
                             const float p = ex2(x);
                             if (!CUT || at + 8 * k + g < limit) got[k] += p;
                         }

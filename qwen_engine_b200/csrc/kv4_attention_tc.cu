@@ -2,18 +2,22 @@
 //
 // A CTA has 256 query rows of one key/value head (token major, so the heads that share it lie side by side) as two tiles of 128,
 // and walks over the positions 128 at a time:
-//   S_i [128 rows x 128 positions] = Q_i . K^T      Q and K from shared memory
+//   S_i [128 rows x 128 positions] = Q_i . K^T      both from shared memory
 //   P_i = 2^(S_i c - m), fp16, over S_i in tensor memory; m follows the running maximum, for the next step where it falls 8 behind, at
 //       once (the step's weights are worked out again) where 15, as fp16 ends at 2^16
 //   O_i [128 rows x 128 dims] += P_i . V            P from tensor memory, V (transposed: positions contiguous) from shared memory
-// While the softmax warps of one tile work the tensor core has the other one.  Keys and values become fp16 once for both tiles:
-// value = (code - 8) * scale + zero by one fma behind an exact conversion, so with one rounding.
+// While the softmax warps of one tile work the tensor core has the other one.  Keys and values become fp16 once for both tiles.  A
+// value is (code - 8) * scale + zero by one fma behind an exact conversion, so has one rounding.  A key has none: (code - 8) * scale
+// has 15 bits at most and is the sum of two fp16 numbers, the product and what its rounding left (one fma), which are two operands;
+// its zero comes in as 16 more columns that all hold it, against the sum of q in two parts, an eighth in each of eight columns.
+// (Keys rounded to fp16 left 4e-4 in the lse of short sequences.  Exact codes as the operand and scale and zero in the softmax need two
+// numbers a position in every thread: from shared memory they took 200 of 910 us, through the same queue as the exponentials.)
 //
 // What bounds it: the exponentials (16 a cycle and SM: 2048 cycles for 256 x 128) and the tensor core (2048 cycles) alike, and
 // behind them the issue slots of the softmax.
 //
 //   warps 0..3, 4..7 : softmax of tile 0 and 1, a thread a row; at the end they store O
-//   warps 8..11      : keys, a thread a position: its row from global memory a step ahead in registers, to shared memory as fp16
+//   warps 8..11      : keys, a thread a position: its row from global memory a step ahead in registers, to shared memory in two parts
 //   warps 12..15     : values: codes through a staging buffer, then a thread takes 8 dims x 8 positions twice and stores them as
 //                      rows of 8 positions.  Every access of both is free of bank conflicts (chunks of 16 bytes are xor-ed).
 //   warp 16          : tensor memory; one thread issues the MMAs
@@ -43,20 +47,25 @@ __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec
 constexpr int kOperand = kTile * kKvDim * 2;              // bytes of a 128 x 128 operand: two panels of 64 columns, 128-byte swizzle
 constexpr int kPanel = kOperand / 2;
 constexpr int kValueStage = kChunkKeys * 64;
-constexpr int kSmemK = 2 * kOperand, kSmemV = 4 * kOperand, kSmemStage = 6 * kOperand, kSmemParam = kSmemStage + 2 * kValueStage;
-constexpr int kChunkSmem = kSmemParam + 2 * kChunkKeys * 4;
+constexpr int kExtra = kTile * 32;                        // 16 more columns, 32-byte swizzle
+// queries of both tiles; keys, first and second part; values, two slots; the extra columns of queries and keys; values' codes and parameters
+constexpr int kSmemK = 2 * kOperand, kSmemV = 4 * kOperand, kSmemQx = 6 * kOperand, kSmemKx = kSmemQx + 2 * kExtra, kSmemStage = kSmemKx + kExtra,
+              kSmemParam = kSmemStage + 2 * kValueStage, kChunkSmem = kSmemParam + 2 * kChunkKeys * 4;
+static_assert(kChunkSmem + 1024 + 2048 <= 227 * 1024);
 constexpr int kTmemO = 256;                               // S_0, S_1, O_0, O_1: 128 columns each
 
 // The two products, with descriptors given by their low words (address): the high word is the same for every operand here, and as
 // 64-bit values the 64 of them that the unrolled loop uses were kept in registers, and spilled.
 constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);      // rows of 128 bytes in groups of 8, 128-byte swizzle
+constexpr uint32_t kDescHighExtra = (256u >> 4) | (1u << 14) | (6u << 29);  // rows of 32 bytes in groups of 8, 32-byte swizzle
 __device__ __forceinline__ uint32_t desc_low(uint32_t addr) { return ((addr & 0x3FFFFu) >> 4) | (1u << 16); }
+template <uint32_t HIGH = kDescHigh>
 __device__ __forceinline__ void mma_ss(uint32_t tmem_d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
         "setp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
-        ::"r"(tmem_d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
+        ::"r"(tmem_d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(HIGH)
         : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
@@ -192,17 +201,10 @@ __device__ __forceinline__ bool nan_params(uint32_t p) { return kv4_scale(p) != 
 
 // Four pairs of values of a word's nibbles (bits 4 n and 16 + 4 n) with their scales and zeros.
 __device__ __forceinline__ void dequantise(uint32_t w, __half2 s, __half2 z, uint32_t (&out)[4]) {
-    const __half2 a = __float2half2_rn(-1032.0f), m = __float2half2_rn(0.0625f), b = __float2half2_rn(-72.0f);
-    const uint32_t u = w >> 8;
-    uint32_t r[4];
-    asm("lop3.b32 %0, %1, 0x000F000F, 0x64006400, 0xEA;" : "=r"(r[0]) : "r"(w));      // 1024 + code
-    asm("lop3.b32 %0, %1, 0x00F000F0, 0x64006400, 0xEA;" : "=r"(r[1]) : "r"(w));      // 1024 + 16 code
-    asm("lop3.b32 %0, %1, 0x000F000F, 0x64006400, 0xEA;" : "=r"(r[2]) : "r"(u));
-    asm("lop3.b32 %0, %1, 0x00F000F0, 0x64006400, 0xEA;" : "=r"(r[3]) : "r"(u));
+    kv4_centred_codes(w, out);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const __half2 c = *reinterpret_cast<const __half2*>(&r[i]);
-        const __half2 v = __hfma2(i & 1 ? __hfma2(c, m, b) : __hadd2(c, a), s, z);
+        const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&out[i]), s, z);
         out[i] = *reinterpret_cast<const uint32_t*>(&v);
     }
 }
@@ -212,6 +214,8 @@ __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_ca
 __device__ __forceinline__ uint32_t operand_at(int row, int chunk) {
     return static_cast<uint32_t>((chunk >> 3) * kPanel + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
 }
+
+__device__ __forceinline__ uint32_t extra_at(int row, int chunk) { return static_cast<uint32_t>(row * 32 + ((chunk ^ ((row >> 2) & 1)) << 4)); }
 
 // The (tile, head) of a CTA: long ones first, which are the last ones of a sequence.
 struct ChunkPlace {
@@ -247,8 +251,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
     volatile int* s_abort = &s_abort_word;
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t smem0 = smem_u32(smem), bar0 = smem_u32(s_bar);
-    auto k_full = [&](int i) { return bar0 + 8u * i; };
-    auto k_empty = [&](int i) { return bar0 + 8u * (2 + i); };
+    const uint32_t k_full = bar0, k_empty = bar0 + 8u * 2;
     auto v_full = [&](int i) { return bar0 + 8u * (4 + i); };
     auto v_empty = [&](int i) { return bar0 + 8u * (6 + i); };
     auto s_full = [&](int i) { return bar0 + 8u * (8 + i); };
@@ -257,14 +260,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (warp == kMmaWarp) {
         if (lane < 2) {
-            mbar_init(k_full(lane), 4);
-            mbar_init(k_empty(lane), 1);
             mbar_init(v_full(lane), 4);
             mbar_init(v_empty(lane), 1);
             mbar_init(s_full(lane), 1);
             mbar_init(p_full(lane), 4);
         }
         if (lane == 0) {
+            mbar_init(k_full, 4);
+            mbar_init(k_empty, 1);
             mbar_init(q_full, kSoftWarps);
             mbar_init(finished, 1);
             *s_abort = 0;
@@ -300,6 +303,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
         const int limit = mine ? pl.w.past + (pl.row0 + row) / a.group + 1 : 0x7FFFFFFF;
         if (steps > 0 && i < tiles) {
             uint4 w[16];
+            float qsum = 0.0f;
             const __half* src = a.q;
             if (mine) src += static_cast<size_t>(pl.w.first + (pl.row0 + row) / a.group) * a.q_stride + (pl.head * a.group + (pl.row0 + row) % a.group) * kKvDim;
 #pragma unroll
@@ -309,6 +313,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
                 *reinterpret_cast<uint4*>(smem + i * kOperand + operand_at(r, k)) =
                     make_uint4(__byte_perm(w[k].x, w[k].y, 0x5410), __byte_perm(w[k].z, w[k].w, 0x5410), __byte_perm(w[k].x, w[k].y, 0x7632),
                                __byte_perm(w[k].z, w[k].w, 0x7632));
+#pragma unroll
+            for (int k = 0; k < 16; ++k) qsum += sum_half8(w[k]);
+            const __half part = __float2half_rn(qsum * 0.125f), rest = __float2half_rn(fmaf(qsum, 0.125f, -__half2float(part)));
+            const uint32_t pp = pack_half2(__half2float(part), __half2float(part)), rr = pack_half2(__half2float(rest), __half2float(rest));
+            *reinterpret_cast<uint4*>(smem + kSmemQx + i * kExtra + extra_at(r, 0)) = make_uint4(pp, pp, pp, pp);
+            *reinterpret_cast<uint4*>(smem + kSmemQx + i * kExtra + extra_at(r, 1)) = make_uint4(rr, rr, rr, rr);
             fence_proxy_async_smem();
         }
         __syncwarp();
@@ -445,30 +455,39 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
             fetch(0);
         }
         for (int j = 0; j < steps; ++j) {
-            const int slot = j & 1;
-            if (!park_warp(k_empty(slot), ((j >> 1) & 1) ^ 1, s_abort)) break;
-            const uint32_t p = finite_params(kp);
-            const __half2 s = __half2half2(__ushort_as_half(static_cast<unsigned short>(p))), z = __half2half2(__ushort_as_half(static_cast<unsigned short>(p >> 16)));
+            if (!park_warp(k_empty, (j & 1) ^ 1, s_abort)) break;
             const uint32_t here = __ballot_sync(0xFFFFFFFFu, there), bad = __ballot_sync(0xFFFFFFFFu, nan_params(vp));
             if (lane == 0) {
                 s_mask[j & 3][0][warp - kKeyWarp] = here;
                 s_mask[j & 3][1][warp - kKeyWarp] = bad;
             }
-            uint8_t* to = smem + kSmemK + slot * kOperand;
+            // 8 * scale has to be finite: rows that span more than 122 820 lose up to 6 % of that
+            const __half2 s = __hmin2_nan(__half2half2(__ushort_as_half(static_cast<unsigned short>(kp))), __float2half2_rn(8188.0f));
+            const uint32_t zero = __byte_perm(kp, kp, 0x3232);
+            *reinterpret_cast<uint4*>(smem + kSmemKx + t * 32) = make_uint4(zero, zero, zero, zero);
+            *reinterpret_cast<uint4*>(smem + kSmemKx + t * 32 + 16) = make_uint4(zero, zero, zero, zero);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const uint32_t words[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    uint32_t o[4];
-                    dequantise(words[e], s, z, o);          // pairs (0, 2), (4, 6), (1, 3), (5, 7)
-                    *reinterpret_cast<uint4*>(to + operand_at(t, 4 * k + e)) = make_uint4(o[0], o[1], o[2], o[3]);
+                    uint32_t o[4], hi[4], lo[4];
+                    kv4_centred_codes(words[e], o);         // pairs (0, 2), (4, 6), (1, 3), (5, 7)
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        const __half2 h = __hmul2(as_half2(o[n]), s), l = __hfma2(as_half2(o[n]), s, __hneg2(h));
+                        hi[n] = *reinterpret_cast<const uint32_t*>(&h);
+                        lo[n] = *reinterpret_cast<const uint32_t*>(&l);
+                    }
+                    uint8_t* to = smem + kSmemK + operand_at(t, 4 * k + e);
+                    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(to + kOperand) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
             }
             if (j + 1 < steps) fetch(j + 1);
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(k_full(slot));
+            if (lane == 0) mbar_arrive(k_full);
         }
     } else if (warp < kMmaWarp) {
         // ================= values =================
@@ -541,23 +560,26 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
         fewer_registers<kIssueRegs>();
         if (warp == kMmaWarp && steps > 0 && elect_one()) {
             constexpr uint32_t idesc = (1u << 4) | ((kTile >> 3) << 17) | ((kTile >> 4) << 24);      // D fp32, A and B fp16, both K-major
-            const uint32_t qd = desc_low(smem0), kd = desc_low(smem0 + kSmemK), vd = desc_low(smem0 + kSmemV);
-            constexpr uint32_t kNext = kOperand >> 4;
+            const uint32_t qd = desc_low(smem0), kd = desc_low(smem0 + kSmemK), vd = desc_low(smem0 + kSmemV), qx = desc_low(smem0 + kSmemQx), kx = desc_low(smem0 + kSmemKx);
+            constexpr uint32_t kNext = kOperand >> 4, kPanelNext = kPanel >> 4, kExtraNext = kExtra >> 4;
             // tile and slot are constants, so that nothing but the loop's own counters is computed here
-            auto scores = [&]<int I, int SLOT>() {
+            auto scores = [&]<int I>() {
+                mma_ss<kDescHighExtra>(tmem + static_cast<uint32_t>(I * 128), qx + I * kExtraNext, kx, idesc, 0);
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
-                    const uint32_t off = (ks >= 4 ? kPanel >> 4 : 0) + 2u * (ks & 3);
-                    mma_ss(tmem + static_cast<uint32_t>(I * 128), qd + (I * kNext + off), kd + (SLOT * kNext + off), idesc, ks != 0);
-                }
+                for (int part = 0; part < 2; ++part)
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) {
+                        const uint32_t off = (ks >= 4 ? kPanelNext : 0) + 2u * (ks & 3);
+                        mma_ss(tmem + static_cast<uint32_t>(I * 128), qd + (I * kNext + off), kd + (part * kNext + off), idesc, 1);
+                    }
                 tc_commit(s_full(I));
             };
-            bool ok = park_wait(q_full, 0, s_abort) && park_wait(k_full(0), 0, s_abort);
+            bool ok = park_wait(q_full, 0, s_abort) && park_wait(k_full, 0, s_abort);
             if (ok) {
                 tc_fence_after();
-                scores.template operator()<0, 0>();
-                if (tiles == 2) scores.template operator()<1, 0>();
-                tc_commit(k_empty(0));
+                scores.template operator()<0>();
+                if (tiles == 2) scores.template operator()<1>();
+                tc_commit(k_empty);
             }
             auto outputs = [&]<int I, int SLOT>(int j) {
                 if (!park_wait(p_full(I), j & 1, s_abort)) return false;
@@ -565,20 +587,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
 #pragma unroll
                 for (int ks = 0; ks < 8; ++ks)
                     mma_ts(tmem + static_cast<uint32_t>(kTmemO + I * 128), tmem + static_cast<uint32_t>(I * 128 + 8 * ks),
-                                  vd + (SLOT * kNext + (ks >= 4 ? kPanel >> 4 : 0) + 2u * (ks & 3)), idesc, j != 0 || ks != 0);
+                           vd + (SLOT * kNext + (ks >= 4 ? kPanelNext : 0) + 2u * (ks & 3)), idesc, j != 0 || ks != 0);
                 if (j + 1 < steps) {
                     if (I == 0) {
-                        if (!park_wait(k_full(SLOT ^ 1), ((j + 1) >> 1) & 1, s_abort)) return false;
+                        if (!park_wait(k_full, (j + 1) & 1, s_abort)) return false;
                         tc_fence_after();
                     }
-                    scores.template operator()<I, (SLOT ^ 1)>();
+                    scores.template operator()<I>();
                 }
                 return true;
             };
             auto step = [&]<int SLOT>(int j) {
                 ok = park_wait(v_full(SLOT), (j >> 1) & 1, s_abort) && outputs.template operator()<0, SLOT>(j) &&
                      (tiles == 1 || outputs.template operator()<1, SLOT>(j));
-                if (j + 1 < steps) tc_commit(k_empty(SLOT ^ 1));
+                if (j + 1 < steps) tc_commit(k_empty);
                 tc_commit(v_empty(SLOT));
             };
             for (int j = 0; ok && j < steps; j += 2) {

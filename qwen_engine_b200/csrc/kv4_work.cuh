@@ -110,6 +110,16 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ float sum_half8(const uint4& w) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        s += f.x + f.y;
+    }
+    return s;
+}
 // One part's four dimensions, with its maximum and sum, into a sum around `top` (the largest maximum).  A part without any
 // position has maximum -infinity and sum 0; where all parts are such, the factor is 1 and what is added is 0.
 __device__ __forceinline__ void add_part(float4& x, float& sum, const float4& p, float2 ml, float top) {

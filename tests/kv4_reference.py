@@ -86,7 +86,8 @@ def attention(pool, table, lens, new, q, scale, fp16_rows=False):
     times the sum of the magnitudes; the zero's part and the scaling add four roundings.  With scores off by at most d, weights
     are off by a factor of at most 1 + 2 d, as is their sum, so the output by 4 d * max|v|; the weights' two fp16 parts, the
     exponential (2 ulp) and the sums of up to L terms in 32 bits add (2^-21 + 2^-21 + L * 2^-23 / 16) * max|v|, as the tensor
-    core adds 16 terms at a time.  lse: d and the logarithm's rounding."""
+    core adds 16 terms at a time.  lse: d and the logarithm's rounding.  fp16_rows: values and weights are rounded to fp16 on the
+    way, 2^-11 each."""
     tokens, heads, _ = q.shape
     group = heads // pool.kv
     out, lse = np.zeros((tokens, heads, 128)), np.full((tokens, heads), -np.inf)
@@ -110,7 +111,7 @@ def attention(pool, table, lens, new, q, scale, fp16_rows=False):
                     out[first + i, h * group + g] = p @ vv / p.sum()
                     lse[first + i, h * group + g] = m + np.log(p.sum())
                     size = (np.abs(kk) @ np.abs(x) + 2 * np.abs(kk).max(1) * np.abs(x).sum()).max() * scale
-                    d = (128 * 2.0 ** -23 + 4 * 2.0 ** -24) * size + 2.0 ** -22 * max(1, np.abs(s).max()) + step * (np.abs(kk) @ np.abs(x)).max() * scale
+                    d = (128 * 2.0 ** -23 + 4 * 2.0 ** -24) * size + 2.0 ** -22 * max(1, np.abs(s).max())
                     eout[first + i, h * group + g] = (4 * d + 2 * step + 2.0 ** -20 + see.sum() * 2.0 ** -27) * np.abs(vv).max() * 3
                     else_[first + i, h * group + g] = 2 * d + 2.0 ** -21 + 2.0 ** -22 * abs(lse[first + i, h * group + g])
     return out, lse, eout, else_
