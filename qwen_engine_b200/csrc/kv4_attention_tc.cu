@@ -17,9 +17,10 @@
 // behind them the issue slots of the softmax.
 //
 //   warps 0..3, 4..7 : softmax of tile 0 and 1, a thread a row; at the end they store O
-//   warps 8..11      : keys, a thread a position: its row from global memory a step ahead in registers, to shared memory in two parts
-//   warps 12..15     : values: codes through a staging buffer, then a thread takes 8 dims x 8 positions twice and stores them as
-//                      rows of 8 positions.  Every access of both is free of bank conflicts (chunks of 16 bytes are xor-ed).
+//   warps 8..15      : operands.  Keys, half a row a thread, from global memory by way of registers, a step ahead; values' codes through a
+//                      staging buffer, then a thread takes 8 dims x 8 positions and stores them as rows of 8 positions.  Every access
+//                      of both is free of bank conflicts (chunks of 16 bytes are xor-ed).  Keys have one slot, so the next step's wait
+//                      for the scores of this one and come first (four warps for keys and four for values: 880 us)
 //   warp 16          : tensor memory; one thread issues the MMAs
 // Within a word the elements come out as 0 2 4 6 1 3 5 7; the queries are put into the same order once.
 //
@@ -35,7 +36,7 @@ namespace w4 {
 namespace {
 
 constexpr int kTile = 128, kChunkRows = 2 * kTile, kChunkKeys = 128;
-constexpr int kSoftWarps = 8, kKeyWarp = 8, kValueWarp = 12, kMmaWarp = 16, kChunkThreads = 20 * 32;
+constexpr int kSoftWarps = 8, kOperandWarp = 8, kMmaWarp = 16, kChunkThreads = 20 * 32;
 // Registers: a launch of 20 warps has 96 a thread (61 440); the warpgroups share them as 128 (softmax, two), 80 (keys, values) and 64
 // (the issuing warp's): 256 * 128 + 256 * 80 + 128 * 64 = 61 440.
 constexpr int kSoftRegs = 128, kOperandRegs = 80, kIssueRegs = 64;
@@ -260,13 +261,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (warp == kMmaWarp) {
         if (lane < 2) {
-            mbar_init(v_full(lane), 4);
+            mbar_init(v_full(lane), 8);
             mbar_init(v_empty(lane), 1);
             mbar_init(s_full(lane), 1);
             mbar_init(p_full(lane), 4);
         }
         if (lane == 0) {
-            mbar_init(k_full, 4);
+            mbar_init(k_full, 8);
             mbar_init(k_empty, 1);
             mbar_init(q_full, kSoftWarps);
             mbar_init(finished, 1);
@@ -426,90 +427,35 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
             if (mine && whole && a.lse != nullptr) a.lse[at_row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
             if (mine && !whole) __stcg(a.part_ml + part, make_float2(m, l));
         }
-    } else if (warp < kValueWarp) {
-        // ================= keys: thread = position = row of the operand =================
+    } else if (warp < kMmaWarp) {
+        // ================= operands: two threads a position =================
         fewer_registers<kOperandRegs>();
-        const int t = tid & 127;
-        uint4 w[4];
+        const int t = tid & 127, part = (warp - kOperandWarp) >> 2;      // keys: words 8 part ..; values: positions 64 part ..
+        const int word = (lane >> 3) + 4 * (warp & 3), oct = t >> 3;
+        uint4 w[2];
         uint32_t kp = 0, vp = 0;
         bool there = false;
         int page = -1;
         auto page_of = [&](int j) { const int at = k0 + j * kChunkKeys + t; return j < steps && at < k1 ? __ldcg(table + (at >> c.page_shift)) : -1; };
+        // position t's key codes and parameters into registers, its value codes into the staging buffer
+        const uint32_t stage_to = smem0 + static_cast<uint32_t>(kSmemStage + (t ^ ((oct >> 2) & 1)) * 64);
         auto fetch = [&](int j) {
             const uint32_t* record = kv4_record_of_page(c, page, pl.head);
             there = record != nullptr;
             kp = vp = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = make_uint4(0, 0, 0, 0);
+            w[0] = w[1] = make_uint4(0, 0, 0, 0);
             if (there) {
                 const int slot = (k0 + j * kChunkKeys + t) & (ps - 1);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) w[k] = __ldcg(reinterpret_cast<const uint4*>(record + slot * kKvRowWords) + k);
+                const uint32_t* keys = record + slot * kKvRowWords + 8 * part;
+                w[0] = __ldcg(reinterpret_cast<const uint4*>(keys));
+                w[1] = __ldcg(reinterpret_cast<const uint4*>(keys) + 1);
                 kp = __ldcg(record + 32 * ps + slot);
                 vp = __ldcg(record + 33 * ps + slot);
-            }
-            page = page_of(j + 1);
-        };
-        if (steps > 0) {
-            page = page_of(0);
-            fetch(0);
-        }
-        for (int j = 0; j < steps; ++j) {
-            if (!park_warp(k_empty, (j & 1) ^ 1, s_abort)) break;
-            const uint32_t here = __ballot_sync(0xFFFFFFFFu, there), bad = __ballot_sync(0xFFFFFFFFu, nan_params(vp));
-            if (lane == 0) {
-                s_mask[j & 3][0][warp - kKeyWarp] = here;
-                s_mask[j & 3][1][warp - kKeyWarp] = bad;
-            }
-            // 8 * scale has to be finite: rows that span more than 122 820 lose up to 6 % of that
-            const __half2 s = __hmin2_nan(__half2half2(__ushort_as_half(static_cast<unsigned short>(kp))), __float2half2_rn(8188.0f));
-            const uint32_t zero = __byte_perm(kp, kp, 0x3232);
-            *reinterpret_cast<uint4*>(smem + kSmemKx + t * 32) = make_uint4(zero, zero, zero, zero);
-            *reinterpret_cast<uint4*>(smem + kSmemKx + t * 32 + 16) = make_uint4(zero, zero, zero, zero);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t words[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    uint32_t o[4], hi[4], lo[4];
-                    kv4_centred_codes(words[e], o);         // pairs (0, 2), (4, 6), (1, 3), (5, 7)
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const __half2 h = __hmul2(as_half2(o[n]), s), l = __hfma2(as_half2(o[n]), s, __hneg2(h));
-                        hi[n] = *reinterpret_cast<const uint32_t*>(&h);
-                        lo[n] = *reinterpret_cast<const uint32_t*>(&l);
-                    }
-                    uint8_t* to = smem + kSmemK + operand_at(t, 4 * k + e);
-                    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4*>(to + kOperand) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                }
-            }
-            if (j + 1 < steps) fetch(j + 1);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(k_full);
-        }
-    } else if (warp < kMmaWarp) {
-        // ================= values =================
-        fewer_registers<kOperandRegs>();
-        const int t = tid & 127, word = (lane >> 3) + 4 * (warp - kValueWarp);
-        uint32_t vp = 0;
-        int page = -1;
-        auto page_of = [&](int j) { const int at = k0 + j * kChunkKeys + t; return j < steps && at < k1 ? __ldcg(table + (at >> c.page_shift)) : -1; };
-        // position t's codes into the staging buffer, its parameters into a register
-        const int oct = t >> 3;
-        const uint32_t stage_to = smem0 + static_cast<uint32_t>(kSmemStage + (t ^ ((oct >> 2) & 1)) * 64);
-        auto fetch = [&](int j) {
-            const uint32_t* record = kv4_record_of_page(c, page, pl.head);
-            vp = 0;
-            if (record != nullptr) {
-                const int slot = (k0 + j * kChunkKeys + t) & (ps - 1);
-                const uint32_t* codes = record + (ps + slot) * kKvRowWords;
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(stage_to + static_cast<uint32_t>((j & 1) * kValueStage + ((k ^ (oct & 3)) << 4))),
-                                 "l"(codes + 4 * k) : "memory");
-                vp = __ldcg(record + 33 * ps + slot);
+                for (int k = 0; k < 2; ++k)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                                 ::"r"(stage_to + static_cast<uint32_t>((j & 1) * kValueStage + (((2 * part + k) ^ (oct & 3)) << 4))),
+                                 "l"(keys + ps * kKvRowWords + 4 * k) : "memory");
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
             page = page_of(j + 1);
@@ -520,35 +466,67 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
         }
         for (int j = 0; j < steps; ++j) {
             const int slot = j & 1;
+            // ---- keys, first: the scores of the next step wait for them ----
+            if (!park_warp(k_empty, (j & 1) ^ 1, s_abort)) break;
+            const uint32_t here = __ballot_sync(0xFFFFFFFFu, there), bad = __ballot_sync(0xFFFFFFFFu, nan_params(vp));
+            if (part == 0 && lane == 0) {
+                s_mask[j & 3][0][warp & 3] = here;
+                s_mask[j & 3][1][warp & 3] = bad;
+            }
+            {
+                // 8 * scale has to be finite: rows that span more than 122 820 lose up to 6 % of that
+                const __half2 s = __hmin2_nan(__half2half2(__ushort_as_half(static_cast<unsigned short>(kp))), __float2half2_rn(8188.0f));
+                const uint32_t zero = __byte_perm(kp, kp, 0x3232);
+                *reinterpret_cast<uint4*>(smem + kSmemKx + t * 32 + 16 * part) = make_uint4(zero, zero, zero, zero);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t words[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t o[4], hi[4], lo[4];
+                        kv4_centred_codes(words[e], o);         // pairs (0, 2), (4, 6), (1, 3), (5, 7)
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            const __half2 h = __hmul2(as_half2(o[n]), s), l = __hfma2(as_half2(o[n]), s, __hneg2(h));
+                            hi[n] = *reinterpret_cast<const uint32_t*>(&h);
+                            lo[n] = *reinterpret_cast<const uint32_t*>(&l);
+                        }
+                        uint8_t* to = smem + kSmemK + operand_at(t, 8 * part + 4 * k + e);
+                        *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4*>(to + kOperand) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(k_full);
+            // ---- values ----
             asm volatile("cp.async.wait_group 0;" ::: "memory");
             uint32_t* params = reinterpret_cast<uint32_t*>(smem + kSmemParam) + slot * kChunkKeys;
-            params[t] = nan_params(vp) ? 0u : finite_params(vp);
-            asm volatile("bar.sync 1, 128;" ::: "memory");        // every position's codes and parameters are there, and the step before has been read
+            if (part == 0) params[t] = nan_params(vp) ? 0u : finite_params(vp);
+            asm volatile("bar.sync 1, 256;" ::: "memory");        // every position's codes and parameters are there, and the step before has been read
             if (j + 1 < steps) fetch(j + 1);
             if (!park_warp(v_empty(slot), ((j >> 1) & 1) ^ 1, s_abort)) break;
             uint8_t* to = smem + kSmemV + slot * kOperand;
             const uint8_t* stage = smem + kSmemStage + slot * kValueStage;
+            const int o8 = (lane & 7) + 8 * part;               // eight positions
+            const uint4 p0 = reinterpret_cast<const uint4*>(params)[2 * o8], p1 = reinterpret_cast<const uint4*>(params)[2 * o8 + 1];
+            const uint32_t pr[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
+            uint32_t vw[8];
 #pragma unroll
-            for (int job = 0; job < 2; ++job) {
-                const int o8 = (lane & 7) + 8 * job;               // eight positions
-                const uint4 p0 = reinterpret_cast<const uint4*>(params)[2 * o8], p1 = reinterpret_cast<const uint4*>(params)[2 * o8 + 1];
-                const uint32_t pr[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
-                uint32_t w[8];
+            for (int e = 0; e < 8; ++e)
+                vw[e] = *reinterpret_cast<const uint32_t*>(stage + ((8 * o8 + e) ^ ((o8 >> 2) & 1)) * 64 + (((word >> 2) ^ (o8 & 3)) << 4) + (word & 3) * 4);
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    w[e] = *reinterpret_cast<const uint32_t*>(stage + ((8 * o8 + e) ^ ((o8 >> 2) & 1)) * 64 + (((word >> 2) ^ (o8 & 3)) << 4) + (word & 3) * 4);
+            for (int half = 0; half < 2; ++half) {
+                uint32_t v[4][4];
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t v[4][4];
+                for (int e = 0; e < 4; ++e)
+                    dequantise(__byte_perm(vw[2 * e], vw[2 * e + 1], half ? 0x7632 : 0x5410), as_half2(__byte_perm(pr[2 * e], pr[2 * e + 1], 0x5410)),
+                               as_half2(__byte_perm(pr[2 * e], pr[2 * e + 1], 0x7632)), v[e]);
+                constexpr int kElement[2][4] = {{0, 4, 1, 5}, {2, 6, 3, 7}};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        dequantise(__byte_perm(w[2 * e], w[2 * e + 1], half ? 0x7632 : 0x5410), as_half2(__byte_perm(pr[2 * e], pr[2 * e + 1], 0x5410)),
-                                   as_half2(__byte_perm(pr[2 * e], pr[2 * e + 1], 0x7632)), v[e]);
-                    constexpr int kElement[2][4] = {{0, 4, 1, 5}, {2, 6, 3, 7}};
-#pragma unroll
-                    for (int n = 0; n < 4; ++n)
-                        *reinterpret_cast<uint4*>(to + operand_at(8 * word + kElement[half][n], o8)) = make_uint4(v[0][n], v[1][n], v[2][n], v[3][n]);
-                }
+                for (int n = 0; n < 4; ++n)
+                    *reinterpret_cast<uint4*>(to + operand_at(8 * word + kElement[half][n], o8)) = make_uint4(v[0][n], v[1][n], v[2][n], v[3][n]);
             }
             fence_proxy_async_smem();
             __syncwarp();
