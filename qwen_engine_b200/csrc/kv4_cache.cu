@@ -116,7 +116,7 @@ __device__ __forceinline__ Spot find_spot(const Kv4View& c, int token) {     // 
 // there (a 32-bit angle of position 100 000 is off by 0.004 rad).  What bounds a prompt are those round trips: with one token a
 // CTA instead of four 4 prompts of up to 4100 tokens took 79 us.
 template <int TOK>
-__global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 6) kv4_append_kernel(const __grid_constant__ AppendArgs a) {
     __shared__ __align__(16) float2 s_turn[TOK][kKvDim / 2];     // cosine, sine
     __shared__ Spot s_spot[TOK];
     __shared__ int s_pos[TOK];
