@@ -585,6 +585,28 @@ W4A16_API int64_t w4a16_sweep_workspace_bytes(int hidden_size, int intermediate_
 W4A16_API int w4a16_sweep_create(const w4a16_sweep_desc* desc, w4a16_stream_t stream, w4a16_sweep** out);
 W4A16_API int w4a16_sweep_destroy(w4a16_sweep* sweep);
 
+/*
+ * The sweep with attention over 4-bit caches in place of the stand-in: per layer
+ *   QKV GEMV -> w4a16_kv4_append (biases, rotary position) -> w4a16_attention_kv4 (fp32 heads) -> O GEMV from the heads (+h)
+ * and, with add_key_weights, w4a16_kv4_add_key_weights behind the attention.  A run is the decode step of one sequence: its
+ * seq_lens entry, in device memory, counts the step's token when the graph runs (the caller adds one before each).  batch has one
+ * sequence and one token.  Creating the sweep stores nothing in the caches.  head_dim must be 128; W4A16_SWEEP_PERSISTENT is
+ * not combined with it (W4A16_ERR_SHAPE).  Device arrays stay the caller's; host arrays are copied.
+ */
+typedef struct w4a16_sweep_kv4 {
+    const w4a16_kv4_cache* caches;                 /* host array [num_layers]; num_kv_heads as in the sweep's description */
+    w4a16_kv4_batch batch;
+    const struct w4a16_qwenbin_biases* biases;     /* host array [num_layers], entries may hold NULL; NULL: none */
+    const int32_t* position;                       /* device [1] rotary position; NULL: the cached position */
+    const float* rope_inv_freq;                    /* device [64]; NULL: no rotation */
+    void* workspace;                               /* device, w4a16_sweep_kv4_workspace_bytes(), 256-byte aligned */
+    float softmax_scale;
+    int add_key_weights;                           /* nonzero: every cache needs key_weight */
+} w4a16_sweep_kv4;
+W4A16_API int64_t w4a16_sweep_kv4_workspace_bytes(int num_q_heads, int num_kv_heads);
+W4A16_API int w4a16_sweep_create_kv4(const w4a16_sweep_desc* desc, const w4a16_sweep_kv4* kv, w4a16_stream_t stream,
+                                     w4a16_sweep** out);
+
 /* Kernels launched per w4a16_sweep_run_* call. */
 W4A16_API int w4a16_sweep_launches(const w4a16_sweep* sweep);
 

@@ -55,6 +55,12 @@ class KV4BatchView(ctypes.Structure):
         (n, c_int) for n in ("num_seqs", "max_pages_per_seq", "num_tokens")]
 
 
+class SweepKV4(ctypes.Structure):
+    """Mirror of w4a16_sweep_kv4."""
+    _fields_ = [("caches", POINTER(KV4CacheView)), ("batch", KV4BatchView), ("biases", POINTER(QwenBinBiases)), ("position", c_void_p),
+                ("rope_inv_freq", c_void_p), ("workspace", c_void_p), ("softmax_scale", ctypes.c_float), ("add_key_weights", c_int)]
+
+
 class SweepDesc(ctypes.Structure):
     """Mirror of w4a16_sweep_desc."""
     _fields_ = [("num_layers", c_int), ("hidden_size", c_int), ("intermediate_size", c_int),
@@ -134,6 +140,8 @@ SIGNATURES = {
     "w4a16_debug_counter": [c_int, POINTER(ctypes.c_uint)],
     "w4a16_sweep_workspace_bytes": [c_int, c_int, c_int, c_int, c_int],
     "w4a16_sweep_create": [POINTER(SweepDesc), c_void_p, POINTER(c_void_p)],
+    "w4a16_sweep_kv4_workspace_bytes": [c_int, c_int],
+    "w4a16_sweep_create_kv4": [POINTER(SweepDesc), POINTER(SweepKV4), c_void_p, POINTER(c_void_p)],
     "w4a16_sweep_destroy": [c_void_p],
     "w4a16_sweep_launches": [c_void_p],
     "w4a16_sweep_run_device": [c_void_p, c_void_p, c_void_p, c_void_p],
@@ -142,6 +150,7 @@ SIGNATURES = {
     "w4a16_sweep_status": [c_void_p, POINTER(c_int)],
 }
 RESTYPES = {"w4a16_sweep_workspace_bytes": ctypes.c_int64, "w4a16_kv4_page_bytes": ctypes.c_int64,
+            "w4a16_sweep_kv4_workspace_bytes": ctypes.c_int64,
             "w4a16_attention_kv4_workspace_bytes": ctypes.c_int64, "w4a16_sweep_buffer": c_void_p}
 
 _lib = None

@@ -37,6 +37,16 @@ struct w4a16_sweep {
     uint32_t epoch = 0;
     uint32_t launch_count = 0;
     int sm_count = 0;
+    // attention over 4-bit caches instead of the stand-in
+    bool has_kv4 = false;
+    w4a16_sweep_kv4 kv4{};
+    std::vector<w4a16_kv4_cache> kv4_caches;
+    std::vector<w4a16_qwenbin_biases> kv4_biases;
+    float* heads = nullptr;              // fp32 [nq*128]
+    float* lse = nullptr;                // [nq]
+    void* kv4_work = nullptr;
+    int64_t kv4_work_bytes = 0;
+    int32_t* no_tokens = nullptr;        // [1], zero: the length that the pass at creation sees
     uint8_t* exchange_begin = nullptr;   // tagged exchange buffers, status word and arrival counters: one range
     size_t exchange_bytes = 0;
 };
@@ -85,8 +95,52 @@ Carve carve(int hidden, int inter, int nq, int nkv, int hd) {
     return c;
 }
 
+struct Kv4Carve {
+    size_t heads, lse, no_tokens, work, total;
+};
+Kv4Carve carve_kv4(int nq, int nkv) {
+    Kv4Carve c{};
+    size_t off = 0;
+    c.heads = off; off += align_up(static_cast<size_t>(nq) * 128 * sizeof(float));
+    c.lse = off; off += align_up(static_cast<size_t>(nq) * sizeof(float));
+    c.no_tokens = off; off += kAlign;
+    c.work = off; off += align_up(static_cast<size_t>(w4a16_attention_kv4_workspace_bytes(1, 1, nq, nkv)));
+    c.total = off;
+    return c;
+}
+
+// The launches between the QKV and the O projection of layer l.  `eager`: the pass at creation, for a sequence without positions.
+int issue_kv4(w4a16_sweep* s, size_t l, bool eager, cudaStream_t stream) {
+    const w4a16_sweep_kv4& kv = s->kv4;
+    w4a16_kv4_batch batch = kv.batch;
+    if (eager) batch.seq_lens = s->no_tokens;
+    const w4a16_kv4_cache* cache = &s->kv4_caches[l];
+    const w4a16_qwenbin_biases b = s->kv4_biases.empty() ? w4a16_qwenbin_biases{} : s->kv4_biases[l];
+    const int nq = s->desc.num_q_heads;
+    w4a16_stream_t st = reinterpret_cast<w4a16_stream_t>(stream);
+    if (int e = w4a16_kv4_append(cache, &batch, s->q, s->k, s->v, b.q_bias, b.k_bias, b.v_bias, kv.position, kv.rope_inv_freq, s->q, nq, 0, 0, st)) return e;
+    if (int e = w4a16_attention_kv4(cache, &batch, s->q, s->heads, s->lse, s->kv4_work, nq, s->kv4_work_bytes, 1, kv.softmax_scale, 0, st)) return e;
+    return kv.add_key_weights ? w4a16_kv4_add_key_weights(cache, &batch, s->q, s->lse, nq, kv.softmax_scale, 0, st) : 0;
+}
+
+// The attention is one launch or two, so a graph with caches is asked for its kernels.
+cudaError_t count_kernels(cudaGraph_t graph, int* launches) {
+    size_t n = 0;
+    cudaError_t e = cudaGraphGetNodes(graph, nullptr, &n);
+    if (e != cudaSuccess) return e;
+    std::vector<cudaGraphNode_t> nodes(n);
+    if ((e = cudaGraphGetNodes(graph, nodes.data(), &n)) != cudaSuccess) return e;
+    *launches = 0;
+    for (cudaGraphNode_t node : nodes) {
+        cudaGraphNodeType type;
+        if ((e = cudaGraphNodeGetType(node, &type)) != cudaSuccess) return e;
+        *launches += type == cudaGraphNodeTypeKernel;
+    }
+    return cudaSuccess;
+}
+
 // Issues the launches of one pass on `stream`; returns the first nonzero status.
-int issue_pass(w4a16_sweep* s, cudaStream_t stream, int* launches) {
+int issue_pass(w4a16_sweep* s, cudaStream_t stream, int* launches, bool eager) {
     const auto& d = s->desc;
     const int H = d.hidden_size, I = d.intermediate_size;
     const int qdim = d.num_q_heads * d.head_dim, kvdim = d.num_kv_heads * d.head_dim;
@@ -121,13 +175,17 @@ int issue_pass(w4a16_sweep* s, cudaStream_t stream, int* launches) {
         }
         if (int st = gemv_launch(kQkv, a, stream)) return st;
         ++n;
-        // attention stand-in: the q projection plays the attention output
+        if (s->has_kv4)
+            if (int st = issue_kv4(s, static_cast<size_t>(&L - s->layers.data()), eager, stream)) return st;
+        // without a cache the q projection plays the attention output
         GemvArgs o = {};
         o.qweight[0] = static_cast<const uint32_t*>(L.o_weight); o.scales[0] = static_cast<const __half*>(L.o_scale);
         o.out[0] = s->h; o.rows[0] = H; o.residual = s->h;
         o.K = qdim; o.units = H;
         if (pub_sums) o.sumsq_out = s->sumsq_attn;
-        if (publish || (flags & W4A16_SWEEP_FUSE_QUANT_O)) {
+        if (s->has_kv4) {
+            o.x_f32 = s->heads;
+        } else if (publish || (flags & W4A16_SWEEP_FUSE_QUANT_O)) {
             o.x_fp16 = s->q;
         } else {
             if (int st = quantize_fp16_to_q8_1(s->q, s->act_q8, s->act_scale, s->act_sum8, qdim, stream)) return st;
@@ -194,18 +252,7 @@ int run_pass(w4a16_sweep* s, cudaStream_t stream) {
     return w4::psweep_launch(s->pargs, s->sm_count, stream);
 }
 
-}  // namespace
-
-extern "C" {
-
-int64_t w4a16_sweep_workspace_bytes(int hidden_size, int intermediate_size, int num_q_heads, int num_kv_heads,
-                                    int head_dim) {
-    if (hidden_size <= 0 || intermediate_size <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0)
-        return W4A16_ERR_INVALID_ARG;
-    return static_cast<int64_t>(carve(hidden_size, intermediate_size, num_q_heads, num_kv_heads, head_dim).total);
-}
-
-int w4a16_sweep_create(const w4a16_sweep_desc* desc, w4a16_stream_t stream_, w4a16_sweep** out) {
+int create_sweep(const w4a16_sweep_desc* desc, const w4a16_sweep_kv4* kv, w4a16_stream_t stream_, w4a16_sweep** out) {
     if (!desc || !out || !desc->layers || !desc->workspace || desc->num_layers <= 0) return W4A16_ERR_INVALID_ARG;
     const int H = desc->hidden_size, I = desc->intermediate_size;
     const int qdim = desc->num_q_heads * desc->head_dim;
@@ -250,6 +297,20 @@ int w4a16_sweep_create(const w4a16_sweep_desc* desc, w4a16_stream_t stream_, w4a
     cudaError_t e = cudaMemsetAsync(s->h, 0, H * sizeof(__half), stream);
     if (e != cudaSuccess) return static_cast<int>(e);
 
+    if (kv != nullptr) {
+        const Kv4Carve k = carve_kv4(desc->num_q_heads, desc->num_kv_heads);
+        uint8_t* kbase = static_cast<uint8_t*>(kv->workspace);
+        s->has_kv4 = true;
+        s->kv4 = *kv;
+        s->kv4_caches.assign(kv->caches, kv->caches + desc->num_layers);
+        if (kv->biases) s->kv4_biases.assign(kv->biases, kv->biases + desc->num_layers);
+        s->heads = reinterpret_cast<float*>(kbase + k.heads);
+        s->lse = reinterpret_cast<float*>(kbase + k.lse);
+        s->no_tokens = reinterpret_cast<int32_t*>(kbase + k.no_tokens);
+        s->kv4_work = kbase + k.work;
+        s->kv4_work_bytes = static_cast<int64_t>(k.total - k.work);
+        if ((e = cudaMemsetAsync(s->no_tokens, 0, sizeof(int32_t), stream)) != cudaSuccess) return static_cast<int>(e);
+    }
     if (desc->flags & W4A16_SWEEP_PERSISTENT) {
         const int kvdim = desc->num_kv_heads * desc->head_dim;
         if (!w4::psweep_supported(H, I, qdim, kvdim) || static_cast<size_t>(desc->num_layers) > kMaxPersistentLayers)
@@ -303,7 +364,7 @@ int w4a16_sweep_create(const w4a16_sweep_desc* desc, w4a16_stream_t stream_, w4a
         return 0;
     }
     // one eager pass (sets kernel attributes, validates the launches), then capture
-    if (int st = issue_pass(s.get(), stream, &s->launches)) return st;
+    if (int st = issue_pass(s.get(), stream, &s->launches, true)) return st;
     if ((e = cudaStreamSynchronize(stream)) != cudaSuccess) return static_cast<int>(e);
     // capture on a stream of our own: the caller's may be the legacy default stream, which cannot capture
     cudaStream_t cap = nullptr;
@@ -312,7 +373,7 @@ int w4a16_sweep_create(const w4a16_sweep_desc* desc, w4a16_stream_t stream_, w4a
         cudaStreamDestroy(cap);
         return static_cast<int>(e);
     }
-    const int st = issue_pass(s.get(), cap, nullptr);
+    const int st = issue_pass(s.get(), cap, nullptr, false);
     e = cudaStreamEndCapture(cap, &s->graph);
     cudaStreamDestroy(cap);
     if (st) {
@@ -320,12 +381,49 @@ int w4a16_sweep_create(const w4a16_sweep_desc* desc, w4a16_stream_t stream_, w4a
         return st;
     }
     if (e != cudaSuccess) return static_cast<int>(e);
+    if (s->has_kv4 && (e = count_kernels(s->graph, &s->launches)) != cudaSuccess) {
+        cudaGraphDestroy(s->graph);
+        return static_cast<int>(e);
+    }
     if ((e = cudaGraphInstantiate(&s->exec, s->graph, 0)) != cudaSuccess) {
         cudaGraphDestroy(s->graph);
         return static_cast<int>(e);
     }
     *out = s.release();
     return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t w4a16_sweep_workspace_bytes(int hidden_size, int intermediate_size, int num_q_heads, int num_kv_heads,
+                                    int head_dim) {
+    if (hidden_size <= 0 || intermediate_size <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0)
+        return W4A16_ERR_INVALID_ARG;
+    return static_cast<int64_t>(carve(hidden_size, intermediate_size, num_q_heads, num_kv_heads, head_dim).total);
+}
+
+int64_t w4a16_sweep_kv4_workspace_bytes(int num_q_heads, int num_kv_heads) {
+    const int64_t n = w4a16_attention_kv4_workspace_bytes(1, 1, num_q_heads, num_kv_heads);
+    return n < 0 ? n : static_cast<int64_t>(carve_kv4(num_q_heads, num_kv_heads).total);
+}
+
+int w4a16_sweep_create(const w4a16_sweep_desc* desc, w4a16_stream_t stream, w4a16_sweep** out) { return create_sweep(desc, nullptr, stream, out); }
+
+int w4a16_sweep_create_kv4(const w4a16_sweep_desc* desc, const w4a16_sweep_kv4* kv, w4a16_stream_t stream, w4a16_sweep** out) {
+    if (!desc || !kv || !kv->caches || !kv->workspace) return W4A16_ERR_INVALID_ARG;
+    if (desc->head_dim != 128 || (desc->flags & W4A16_SWEEP_PERSISTENT)) return W4A16_ERR_SHAPE;
+    if (kv->batch.num_seqs != 1 || kv->batch.num_tokens != 1 || kv->batch.query_start) return W4A16_ERR_INVALID_ARG;
+    if (reinterpret_cast<uintptr_t>(kv->workspace) % kAlign) return W4A16_ERR_ALIGNMENT;
+    if (const int64_t n = w4a16_sweep_kv4_workspace_bytes(desc->num_q_heads, desc->num_kv_heads); n < 0) return static_cast<int>(n);
+    for (int l = 0; l < desc->num_layers; ++l) {
+        const w4a16_kv4_cache& c = kv->caches[l];
+        if (int st = w4::kv4_check_step(&c, &kv->batch, desc->num_q_heads, kv->softmax_scale, kv->position, kv->rope_inv_freq, kv->biases ? kv->biases + l : nullptr))
+            return st;
+        if (c.num_kv_heads != desc->num_kv_heads || (kv->add_key_weights && !c.key_weight)) return W4A16_ERR_INVALID_ARG;
+    }
+    return create_sweep(desc, kv, stream, out);
 }
 
 int w4a16_sweep_destroy(w4a16_sweep* s) {

@@ -13,7 +13,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import LayerWeights, QKVView, SweepDesc, W4A16Error, check, load  # noqa: F401
+from ._lib import KV4BatchView, KV4CacheView, LayerWeights, QKVView, QwenBinBiases, SweepDesc, SweepKV4, W4A16Error, check, load  # noqa: F401
 
 __all__ = [
     "QKVProjectionView", "W4A16Error", "init", "set_pdl", "load", "set_option", "get_option", "OPT_PDL",
@@ -26,7 +26,7 @@ __all__ = [
     "launch_gemm_prefill_dual_gate_up_swiglu_w4a16", "gemv_group_dots", "DecodeSweep",
     "launch_gemv_rmsnorm_w4a16", "launch_gemv_qkv_rmsnorm_w4a16", "launch_gemv_dual_gate_up_swiglu_rmsnorm_w4a16", "launch_gemv_dual_gate_up_swiglu_rmsnorm_w4a16_q8_1",
     "gemv_w4a8_peers", "gemm_prefill_w4a16_block", "make_sample_control", "launch_embed_lookup_w4a16", "read_sample_control", "launch_sample_and_advance", "sample_slots", "launch_gemv_w4a8_sample_candidates", "launch_sample_finish", "launch_gemv_w4a8_sample_one_launch", "gemv_w4a8_sample_candidates_peers", "gemv_w4a8_sample_candidates_signal", "sample_finish_after_signals", "gemv_w4a8_peers_signal", "gather_after_signals", "launch_gemv_w4a8_sample_and_advance", "SWEEP_SEPARATE", "SWEEP_FUSE_ALL", "SWEEP_PERSISTENT", "SWEEP_QUANT_IN_GATE_UP", "SWEEP_PUBLISH_SUMSQ", "SWEEP_PUBLISH_AMAX", "SWEEP_DEFAULT", "gemv_w4a16_static_scratch", "debug_counter",
-    "KV4Cache", "KV4Batch", "kv4_append", "kv4_read", "attention_kv4", "attention_kv4_workspace_bytes", "kv4_add_key_weights", "kv4_evict",
+    "KV4Cache", "KV4Batch", "SweepCache", "kv4_append", "kv4_read", "attention_kv4", "attention_kv4_workspace_bytes", "kv4_add_key_weights", "kv4_evict",
 ]
 
 # Qwen2.5-1.5B defaults of the reference's launchers (include/config.cuh:10-22)
@@ -297,6 +297,38 @@ SWEEP_PUBLISH_AMAX = 64
 SWEEP_DEFAULT = SWEEP_FUSE_NORM | SWEEP_FUSE_QUANT_O | SWEEP_PUBLISH_SUMSQ
 
 
+@dataclass
+class SweepCache:
+    """4-bit caches of a DecodeSweep (w4a16_sweep_kv4): one KV4Cache a layer, the KV4Batch of one sequence, and biases: per layer
+    (q_bias, k_bias, v_bias) or None, or a ready ctypes array of QwenBinBiases (QwenBin.bias_table)."""
+    caches: list
+    batch: KV4Batch
+    softmax_scale: float
+    biases: object = None
+    position: torch.Tensor | None = None
+    rope_inv_freq: torch.Tensor | None = None
+    add_key_weights: bool = False
+
+    def pod(self, num_layers: int, num_q_heads: int, num_kv_heads: int):
+        """The C struct with a workspace of its own, and what has to live as long as the sweep."""
+        if len(self.caches) != num_layers or (self.biases is not None and len(self.biases) != num_layers):
+            raise ValueError("one cache, and one entry of biases, a layer expected")
+        nbytes = load().w4a16_sweep_kv4_workspace_bytes(num_q_heads, num_kv_heads)
+        if nbytes < 0:
+            check("w4a16_sweep_kv4_workspace_bytes", int(nbytes))
+        ws = torch.empty(nbytes + 256, dtype=torch.uint8, device="cuda")
+        caches = (KV4CacheView * num_layers)(*[
+            KV4CacheView(_ptr(c.pages), _ptr(c.key_weight), c.num_pages, c.num_kv_heads, c.page_size) for c in self.caches])
+        biases = self.biases
+        if biases is not None and not isinstance(biases, ctypes.Array):
+            biases = (QwenBinBiases * num_layers)(*[QwenBinBiases(*[_ptr(t) for t in (row or (None,) * 3)]) for row in biases])
+        b = self.batch
+        view = KV4BatchView(_ptr(b.block_table), _ptr(b.seq_lens), _ptr(b.query_start), b.num_seqs, b.max_pages_per_seq, b.num_tokens)
+        keep = (ws, [(c.pages, c.key_weight) for c in self.caches], b.block_table, b.seq_lens, self.biases and list(self.biases), self.position, self.rope_inv_freq)
+        return SweepKV4(caches, view, biases, _ptr(self.position), _ptr(self.rope_inv_freq),
+                        (ws.data_ptr() + 255) // 256 * 256, self.softmax_scale, int(self.add_key_weights)), keep
+
+
 class DecodeSweep:
     """The W4 projections of one batch-1 decode pass as one CUDA graph (C ABI w4a16_sweep_*).
 
@@ -304,10 +336,13 @@ class DecodeSweep:
     entries are fp16 gamma tensors, the others (qweight, scales) tensor pairs -- or a ready ctypes array of
     LayerWeights (e.g. QwenBin.layer_table over an uploaded `.qwenbin` file; the caller keeps that memory alive).  The object keeps
     the tensors alive; the native sweep owns only its graph.
+
+    kv4 (a SweepCache): attention over 4-bit caches instead of the stand-in; a run is then the decode step of the one sequence of
+    its batch, whose seq_lens entry the caller has raised by one before.
     """
 
     def __init__(self, layers, hidden=HIDDEN_SIZE, inter=INTERMEDIATE_SIZE, num_q_heads=NUM_Q_HEADS,
-                 num_kv_heads=NUM_KV_HEADS, head_dim=HEAD_DIM, stream=None, flags=SWEEP_DEFAULT):
+                 num_kv_heads=NUM_KV_HEADS, head_dim=HEAD_DIM, stream=None, flags=SWEEP_DEFAULT, kv4=None):
         lib = load()
         self._layers = layers
         self.hidden = hidden
@@ -324,7 +359,11 @@ class DecodeSweep:
                 _ptr(L["gate_up"][0]), _ptr(L["gate_up"][1]), _ptr(L["down"][0]), _ptr(L["down"][1]))
         desc = SweepDesc(len(layers), hidden, inter, num_q_heads, num_kv_heads, head_dim, arr, ws_ptr, flags)
         handle = ctypes.c_void_p()
-        check("w4a16_sweep_create", lib.w4a16_sweep_create(ctypes.byref(desc), _stream(stream), ctypes.byref(handle)))
+        if kv4 is None:
+            check("w4a16_sweep_create", lib.w4a16_sweep_create(ctypes.byref(desc), _stream(stream), ctypes.byref(handle)))
+        else:
+            kv, self._kv4 = kv4.pod(len(layers), num_q_heads, num_kv_heads)
+            check("w4a16_sweep_create_kv4", lib.w4a16_sweep_create_kv4(ctypes.byref(desc), ctypes.byref(kv), _stream(stream), ctypes.byref(handle)))
         self._h = handle
         self._handle = handle.value
         self._run_device = _native("sweep_run_device")

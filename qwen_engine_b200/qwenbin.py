@@ -53,3 +53,11 @@ class QwenBin:
         check("w4a16_qwenbin_tensors", load().w4a16_qwenbin_tensors(
             self.bytes.ctypes.data, self.bytes.size, base, layers, n, None, None))
         return layers
+
+    def bias_table(self, base: int):
+        """The ctypes array of QwenBinBiases that a SweepCache takes."""
+        n = self.header.num_layers
+        layers, biases = (LayerWeights * n)(), (QwenBinBiases * n)()
+        check("w4a16_qwenbin_tensors", load().w4a16_qwenbin_tensors(
+            self.bytes.ctypes.data, self.bytes.size, base, layers, n, None, biases))
+        return biases

@@ -541,3 +541,93 @@ def test_a_pool_of_more_than_4_gib(ops):
 
 def test_waits_of_the_chunk_form_did_not_run_out(ops):
     assert ops.debug_counter(0) == 0
+
+
+# ---- the decode sweep with caches ----------------------------------------------------------------------------------------
+
+
+def sweep_case(ops, layers, heads, kv, page, length, flags, weights, seed=5):
+    """A small model with a cache of `length` positions a layer; everything a sweep and a sequence of separate calls need."""
+    from qwen_engine_b200 import synth
+    H, inter, qd, kd = 512, 1024, 128 * heads, 128 * kv
+    rng = np.random.default_rng(seed)
+    per = -(-(length + 8) // page)
+    table, lens = i32(rng.permutation(per + 2)[None, :per].copy()), i32([length])
+    L, caches, biases, words = [], [], [], []
+    for l in range(layers):
+        d = {n: (util.to_dev(synth.packed_weights(seed, f"{n}{l}", r, c)), util.to_dev(synth.scales(seed, f"{n}{l}", r, c)))
+             for n, r, c in (("q", qd, H), ("k", kd, H), ("v", kd, H), ("o", H, qd), ("gate_up", 2 * inter, H), ("down", H, inter))}
+        d["input_norm"] = d["post_norm"] = torch.full((H,), 0.05, dtype=torch.float16, device="cuda")
+        L.append(d)
+        pool = ref.Pool(per + 2, kv, page).fill_random(rng, 1.5, 0.7)
+        words.append(pool.words.copy())
+        caches.append(ops.KV4Cache(util.to_dev(pool.words), torch.zeros(per + 2, kv, page, device="cuda") if weights else None, per + 2, kv, page))
+        biases.append(tuple(util.to_dev(rng.standard_normal(n).astype(BF)) for n in (qd, kd, kd)) if l != 1 else None)
+    inv = torch.tensor(1e6 ** (-np.arange(64) / 64), dtype=torch.float32, device="cuda")
+    position = i32([length + 100])
+    cache = ops.SweepCache(caches, ops.KV4Batch.of(table, lens), SCALE, biases, position, inv, weights)
+    sweep = ops.DecodeSweep(L, hidden=H, inter=inter, num_q_heads=heads, num_kv_heads=kv, flags=flags, kv4=cache)
+    return H, inter, L, cache, sweep, words
+
+
+def separate_calls(ops, H, inter, L, cache, heads, h):
+    qd, kd = 128 * heads, 128 * cache.caches[0].num_kv_heads
+    f16 = lambda n: torch.empty(n, dtype=torch.float16, device="cuda")  # noqa: E731
+    n = ops.attention_kv4_workspace_bytes(1, 1, heads, kd // 128)
+    ws, acc, lse = torch.empty(n, dtype=torch.uint8, device="cuda"), torch.empty(heads, 128, device="cuda"), torch.empty(heads, device="cuda")
+    for d, c, b in zip(L, cache.caches, cache.biases):
+        q, k, v, o, mlp, out = f16(qd), f16(kd), f16(kd), f16(H), f16(inter), f16(H)
+        view = ops.QKVProjectionView(*d["q"], q, *d["k"], k, *d["v"], v)
+        ops.launch_gemv_qkv_rmsnorm_w4a16(view, h, d["input_norm"], in_features=H, num_q_heads=heads, num_kv_heads=kd // 128)
+        ops.kv4_append(c, cache.batch, q, k, v, *(b or (None,) * 3), cache.position, cache.rope_inv_freq, q, heads)
+        ops.attention_kv4(c, cache.batch, q, acc, lse, ws, heads, n, True, SCALE)
+        if cache.add_key_weights:
+            ops.kv4_add_key_weights(c, cache.batch, q, lse, heads, SCALE)
+        ops.gemv_attn_heads_f32_w4a16(*d["o"], acc, h, o, H, qd)
+        ops.launch_gemv_dual_gate_up_swiglu_rmsnorm_w4a16(*d["gate_up"], o, d["post_norm"], mlp, H, inter)
+        ops.launch_gemv_w4a16(*d["down"], mlp, o, out, H, inter)
+        h = out
+    return h
+
+
+@pytest.mark.parametrize("flags", ["SWEEP_DEFAULT", "SWEEP_SEPARATE", "SWEEP_FUSE_ALL", "SWEEP_PUBLISH_AMAX"])
+@pytest.mark.parametrize("heads,kv,page,length,weights", [(12, 2, 16, 0, True), (4, 1, 32, 20, False), (8, 8, 16, 700, True)])
+def test_decode_sweep_with_caches_is_the_separate_calls(ops, heads, kv, page, length, weights, flags):
+    """Six steps on a growing sequence: hidden state, pages and weights bit for bit; making the sweep stores nothing."""
+    H, inter, L, cache, sweep, words = sweep_case(ops, 3, heads, kv, page, length, getattr(ops, flags), weights)
+    first = [c.pages.clone() for c in cache.caches]
+    other = ops.SweepCache([ops.KV4Cache(c.pages.clone(), None if c.key_weight is None else c.key_weight.clone(), c.num_pages, kv, page) for c in cache.caches],
+                           cache.batch, SCALE, cache.biases, cache.position, cache.rope_inv_freq, weights)
+    torch.cuda.synchronize()
+    assert all(np.array_equal(words_of(c), w) and (not weights or not c.key_weight.any()) for c, w in zip(cache.caches, words))
+    h = util.to_dev(np.random.default_rng(3).standard_normal(H).astype(BF))
+    for step in range(6):
+        cache.batch.seq_lens.add_(1)
+        cache.position.add_(1)
+        out = torch.empty_like(h)
+        sweep.run_device(h, out)
+        want = separate_calls(ops, H, inter, L, other, heads, h)
+        assert torch.equal(out, want), step
+        assert torch.isfinite(out).all()
+        for a, b, f in zip(cache.caches, other.caches, first):
+            assert torch.equal(a.pages, b.pages) and not torch.equal(a.pages, f)
+            if weights:
+                assert torch.equal(a.key_weight, b.key_weight) and a.key_weight.sum().item() > 0
+        h = out
+    sweep.close()
+
+
+def test_two_sweeps_from_one_cache_object_keep_their_workspaces(ops):
+    """Two graphs made from one SweepCache, run in turn, give what each gives alone."""
+    H, inter, L, cache, one, _ = sweep_case(ops, 2, 4, 2, 16, 40, ops.SWEEP_DEFAULT, False)
+    two = ops.DecodeSweep(L, hidden=H, inter=inter, num_q_heads=4, num_kv_heads=2, kv4=cache)
+    cache.batch.seq_lens.add_(1)
+    h = util.to_dev(np.random.default_rng(3).standard_normal(H).astype(BF))
+    a, b, c = (torch.empty_like(h) for _ in range(3))
+    one.run_device(h, a)
+    two.run_device(h, b)
+    one.run_device(h, c)
+    assert torch.equal(a, b) and torch.equal(a, c)
+    # 3 launches a layer more than the sweep without caches: append, attention, its join
+    plain = ops.DecodeSweep(L, hidden=H, inter=inter, num_q_heads=4, num_kv_heads=2)
+    assert one.launches == plain.launches + 2 * 3

@@ -126,3 +126,50 @@ def test_arguments_of_the_python_functions(lib):
         ops.kv4_read(SimpleNamespace(pages=torch.zeros(1), key_weight=None, num_pages=8, num_kv_heads=2, page_size=16), batch, d, d, stream=0)
     with pytest.raises(OverflowError):
         ops.attention_kv4(cache, batch, d, d, None, None, 12, 1 << 70, True, 0.1, stream=0)
+
+
+def sweep_create(lib, desc_changes=(), **changes):
+    from qwen_engine_b200._lib import KV4BatchView, KV4CacheView, LayerWeights, QwenBinBiases, SweepDesc, SweepKV4
+    layers = (LayerWeights * 2)(*[LayerWeights(*[P] * 14)] * 2)
+    c = dict(pages=P, key_weight=P, num_pages=8, num_kv_heads=2, page_size=16)
+    b = dict(block_table=P, seq_lens=P, query_start=None, num_seqs=1, max_pages_per_seq=4, num_tokens=1)
+    kv = dict(position=P, rope_inv_freq=P, workspace=P, softmax_scale=0.088, add_key_weights=1)
+    d = dict(num_layers=2, hidden=512, inter=512, q_heads=4, kv_heads=2, head_dim=128, layers=layers, workspace=P, flags=37)
+    bias = changes.pop("bias", P)
+    for k, v in changes.items():
+        next(x for x in (c, b, kv) if k in x)[k] = v
+    d.update(desc_changes)
+    good = KV4CacheView(P, P, 8, 2, 16)
+    caches = (KV4CacheView * 2)(good, KV4CacheView(*c.values()))       # the last layer's is the bad one
+    biases = (QwenBinBiases * 2)(QwenBinBiases(None, None, None), QwenBinBiases(P, bias, P))
+    pod = SweepKV4(caches, KV4BatchView(*b.values()), biases, *kv.values())
+    out = ctypes.c_void_p()
+    status = lib.w4a16_sweep_create_kv4(ctypes.byref(SweepDesc(*d.values())), ctypes.byref(pod), None, ctypes.byref(out))
+    assert not out.value
+    return status
+
+
+@pytest.mark.parametrize("desc,changes,status", [
+    ({}, dict(pages=None), -1), ({}, dict(num_kv_heads=4), -1), ({}, dict(key_weight=None), -1), ({}, dict(page_size=24), -2),
+    ({}, dict(num_seqs=2, num_tokens=2), -1), ({}, dict(num_tokens=2), -1), ({}, dict(query_start=P), -1), ({}, dict(seq_lens=None), -1),
+    ({}, dict(workspace=None), -1), ({}, dict(workspace=P + 16), -3), ({}, dict(softmax_scale=0.0), -1), ({}, dict(softmax_scale=float("nan")), -1),
+    ({}, dict(position=P + 2), -3), ({}, dict(rope_inv_freq=P + 2), -3), ({}, dict(bias=P + 8), -3), (dict(head_dim=64), {}, -2),
+    (dict(flags=8), {}, -2), (dict(q_heads=5), {}, -2), (dict(num_layers=0), {}, -1), (dict(q_heads=0), {}, -1), (dict(q_heads=1 << 20), {}, -5)],
+    ids=str)
+def test_a_sweep_with_caches_refuses(lib, desc, changes, status):
+    assert sweep_create(lib, desc, **changes) == status
+
+
+def test_workspace_of_a_sweep_with_caches(lib):
+    f = lib.w4a16_sweep_kv4_workspace_bytes
+    assert f(12, 2) >= lib.w4a16_attention_kv4_workspace_bytes(1, 1, 12, 2) + 12 * 129 * 4 and f(12, 2) % 256 == 0
+    assert f(0, 1) == -1 and f(3, 2) == -2
+
+
+def test_a_sweep_cache_asks_for_one_cache_a_layer():
+    from qwen_engine_b200 import KV4Batch, KV4Cache, SweepCache
+    cache = KV4Cache.allocate(4, device="cpu")
+    batch = KV4Batch.of(torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32))
+    for bad in (SweepCache([cache], batch, 0.1), SweepCache([cache] * 2, batch, 0.1, biases=[None])):
+        with pytest.raises(ValueError, match="a layer"):
+            bad.pod(2, 4, 2)
