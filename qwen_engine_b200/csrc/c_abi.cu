@@ -125,12 +125,11 @@ namespace w4 {
 
 // What a decode step asks of its cache before anything is launched.
 int kv4_check_step(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, int num_q_heads, float softmax_scale, const int32_t* position,
-                   const float* inv_freq, const w4a16_qwenbin_biases* b) {
-    Kv4View c;
+                   const float* inv_freq, const w4a16_qwenbin_biases* b, Kv4View* view) {
     int stride = 0;
-    if (int st = kv4_view(cache, batch, &c)) return st;
+    if (int st = kv4_view(cache, batch, view)) return st;
     if (!std::isfinite(softmax_scale) || softmax_scale <= 0.0f) return W4A16_ERR_INVALID_ARG;
-    if (int st = kv4_heads(c, num_q_heads, &stride, num_q_heads)) return st;
+    if (int st = kv4_heads(*view, num_q_heads, &stride, num_q_heads)) return st;
     if (misaligned(position, 4) || misaligned(inv_freq, 4)) return W4A16_ERR_ALIGNMENT;
     return b && (misaligned(b->q_bias, 16) || misaligned(b->k_bias, 16) || misaligned(b->v_bias, 16)) ? W4A16_ERR_ALIGNMENT : 0;
 }

@@ -6,6 +6,7 @@
 #include <new>
 #include <vector>
 
+#include "kv4_attention.hpp"
 #include "w4a16_internal.hpp"
 
 struct w4a16_sweep {
@@ -40,12 +41,11 @@ struct w4a16_sweep {
     // attention over 4-bit caches instead of the stand-in
     bool has_kv4 = false;
     w4a16_sweep_kv4 kv4{};
-    std::vector<w4a16_kv4_cache> kv4_caches;
+    std::vector<w4::Kv4View> kv4_views;
     std::vector<w4a16_qwenbin_biases> kv4_biases;
     float* heads = nullptr;              // fp32 [nq*128]
     float* lse = nullptr;                // [nq]
     void* kv4_work = nullptr;
-    int64_t kv4_work_bytes = 0;
     int32_t* no_tokens = nullptr;        // [1], zero: the length that the pass at creation sees
     uint8_t* exchange_begin = nullptr;   // tagged exchange buffers, status word and arrival counters: one range
     size_t exchange_bytes = 0;
@@ -112,15 +112,15 @@ Kv4Carve carve_kv4(int nq, int nkv) {
 // The launches between the QKV and the O projection of layer l.  `eager`: the pass at creation, for a sequence without positions.
 int issue_kv4(w4a16_sweep* s, size_t l, bool eager, cudaStream_t stream) {
     const w4a16_sweep_kv4& kv = s->kv4;
-    w4a16_kv4_batch batch = kv.batch;
-    if (eager) batch.seq_lens = s->no_tokens;
-    const w4a16_kv4_cache* cache = &s->kv4_caches[l];
+    Kv4View c = s->kv4_views[l];
+    if (eager) c.lens = s->no_tokens;
     const w4a16_qwenbin_biases b = s->kv4_biases.empty() ? w4a16_qwenbin_biases{} : s->kv4_biases[l];
-    const int nq = s->desc.num_q_heads;
-    w4a16_stream_t st = reinterpret_cast<w4a16_stream_t>(stream);
-    if (int e = w4a16_kv4_append(cache, &batch, s->q, s->k, s->v, b.q_bias, b.k_bias, b.v_bias, kv.position, kv.rope_inv_freq, s->q, nq, 0, 0, st)) return e;
-    if (int e = w4a16_attention_kv4(cache, &batch, s->q, s->heads, s->lse, s->kv4_work, nq, s->kv4_work_bytes, 1, kv.softmax_scale, 0, st)) return e;
-    return kv.add_key_weights ? w4a16_kv4_add_key_weights(cache, &batch, s->q, s->lse, nq, kv.softmax_scale, 0, st) : 0;
+    auto h = [](const void* p) { return static_cast<const __half*>(p); };
+    const int nq = s->desc.num_q_heads, q_stride = nq * kKvDim, kv_stride = c.kv_heads * kKvDim, group = nq / c.kv_heads;
+    if (int e = kv4_append(c, Kv4AppendArgs{s->q, s->k, s->v, h(b.q_bias), h(b.k_bias), h(b.v_bias), s->q, kv.position, kv.rope_inv_freq, nq, q_stride, kv_stride}, stream))
+        return e;
+    if (int e = kv4_attention(Kv4AttentionArgs{c, s->q, s->heads, s->lse, nullptr, nullptr, kv.softmax_scale, group, q_stride}, nq, true, s->kv4_work, stream)) return e;
+    return kv.add_key_weights ? kv4_add_key_weights(Kv4WeightArgs{c, s->q, s->lse, kv.softmax_scale, group, q_stride, 0}, stream) : 0;
 }
 
 // The attention is one launch or two, so a graph with caches is asked for its kernels.
@@ -252,7 +252,7 @@ int run_pass(w4a16_sweep* s, cudaStream_t stream) {
     return w4::psweep_launch(s->pargs, s->sm_count, stream);
 }
 
-int create_sweep(const w4a16_sweep_desc* desc, const w4a16_sweep_kv4* kv, w4a16_stream_t stream_, w4a16_sweep** out) {
+int create_sweep(const w4a16_sweep_desc* desc, const w4a16_sweep_kv4* kv, const std::vector<Kv4View>* views, w4a16_stream_t stream_, w4a16_sweep** out) {
     if (!desc || !out || !desc->layers || !desc->workspace || desc->num_layers <= 0) return W4A16_ERR_INVALID_ARG;
     const int H = desc->hidden_size, I = desc->intermediate_size;
     const int qdim = desc->num_q_heads * desc->head_dim;
@@ -302,13 +302,12 @@ int create_sweep(const w4a16_sweep_desc* desc, const w4a16_sweep_kv4* kv, w4a16_
         uint8_t* kbase = static_cast<uint8_t*>(kv->workspace);
         s->has_kv4 = true;
         s->kv4 = *kv;
-        s->kv4_caches.assign(kv->caches, kv->caches + desc->num_layers);
+        s->kv4_views = *views;
         if (kv->biases) s->kv4_biases.assign(kv->biases, kv->biases + desc->num_layers);
         s->heads = reinterpret_cast<float*>(kbase + k.heads);
         s->lse = reinterpret_cast<float*>(kbase + k.lse);
         s->no_tokens = reinterpret_cast<int32_t*>(kbase + k.no_tokens);
         s->kv4_work = kbase + k.work;
-        s->kv4_work_bytes = static_cast<int64_t>(k.total - k.work);
         if ((e = cudaMemsetAsync(s->no_tokens, 0, sizeof(int32_t), stream)) != cudaSuccess) return static_cast<int>(e);
     }
     if (desc->flags & W4A16_SWEEP_PERSISTENT) {
@@ -409,7 +408,7 @@ int64_t w4a16_sweep_kv4_workspace_bytes(int num_q_heads, int num_kv_heads) {
     return n < 0 ? n : static_cast<int64_t>(carve_kv4(num_q_heads, num_kv_heads).total);
 }
 
-int w4a16_sweep_create(const w4a16_sweep_desc* desc, w4a16_stream_t stream, w4a16_sweep** out) { return create_sweep(desc, nullptr, stream, out); }
+int w4a16_sweep_create(const w4a16_sweep_desc* desc, w4a16_stream_t stream, w4a16_sweep** out) { return create_sweep(desc, nullptr, nullptr, stream, out); }
 
 int w4a16_sweep_create_kv4(const w4a16_sweep_desc* desc, const w4a16_sweep_kv4* kv, w4a16_stream_t stream, w4a16_sweep** out) {
     if (!desc || !kv || !kv->caches || !kv->workspace) return W4A16_ERR_INVALID_ARG;
@@ -417,13 +416,15 @@ int w4a16_sweep_create_kv4(const w4a16_sweep_desc* desc, const w4a16_sweep_kv4* 
     if (kv->batch.num_seqs != 1 || kv->batch.num_tokens != 1 || kv->batch.query_start) return W4A16_ERR_INVALID_ARG;
     if (reinterpret_cast<uintptr_t>(kv->workspace) % kAlign) return W4A16_ERR_ALIGNMENT;
     if (const int64_t n = w4a16_sweep_kv4_workspace_bytes(desc->num_q_heads, desc->num_kv_heads); n < 0) return static_cast<int>(n);
+    std::vector<w4::Kv4View> views(desc->num_layers > 0 ? static_cast<size_t>(desc->num_layers) : 0);
     for (int l = 0; l < desc->num_layers; ++l) {
         const w4a16_kv4_cache& c = kv->caches[l];
-        if (int st = w4::kv4_check_step(&c, &kv->batch, desc->num_q_heads, kv->softmax_scale, kv->position, kv->rope_inv_freq, kv->biases ? kv->biases + l : nullptr))
+        if (int st = w4::kv4_check_step(&c, &kv->batch, desc->num_q_heads, kv->softmax_scale, kv->position, kv->rope_inv_freq, kv->biases ? kv->biases + l : nullptr, &views[l]))
             return st;
         if (c.num_kv_heads != desc->num_kv_heads || (kv->add_key_weights && !c.key_weight)) return W4A16_ERR_INVALID_ARG;
+        views[l].settled = true;
     }
-    return create_sweep(desc, kv, stream, out);
+    return create_sweep(desc, kv, &views, stream, out);
 }
 
 int w4a16_sweep_destroy(w4a16_sweep* s) {

@@ -33,6 +33,10 @@ struct Kv4View {
     const int32_t* lens;                 // [num_seqs]
     const int32_t* qstart;               // [num_seqs + 1] or null: one token a sequence
     int num_pages, kv_heads, page_shift, num_seqs, max_pages, num_tokens;
+    // No launch that may still run when this one starts writes table, lens, qstart or the positions of the call: they are read before
+    // the wait for the launches in front.  The decode sweep can promise it (its graph writes none of them), a single call cannot: a
+    // sampler that counts a position on may be two early launches ahead.
+    bool settled = false;
 };
 
 // New tokens of sequence b: first row of the batch and count, both inside the batch whatever the array holds.

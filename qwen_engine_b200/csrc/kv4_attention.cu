@@ -93,13 +93,15 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
     __shared__ FindScratch<kAttnThreads> s_find;
     static_assert(R * kPitch * 4 <= kStages * kStageBytes);
     auto s_o = [&](int w, int r, int d) -> float& { return reinterpret_cast<float*>(s_ring[w])[r * kPitch + d]; };
-    pdl_wait_prior_grids();
-    pdl_release_dependents();
     const Kv4View& c = a.c;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     long long per, all;
     Place pl;
-    if (!find_unit<kAttnThreads>(c, a.group, R, blockIdx.x, gridDim.x, s_find, &per, &all, &pl)) return;
+    if (!c.settled) pdl_wait_prior_grids();
+    const bool work = find_unit<kAttnThreads>(c, a.group, R, blockIdx.x, gridDim.x, s_find, &per, &all, &pl);
+    if (c.settled) pdl_wait_prior_grids();
+    pdl_release_dependents();               // the join reads lengths before its own wait, so not before this one's
+    if (!work) return;
     long long left = min(per, all - per * blockIdx.x);
     for (bool first_part = true; left > 0; first_part = false) {
     while (pl.in_seq >= static_cast<long long>(pl.w.tiles) * c.kv_heads * pl.w.units) {      // past the sequence: the next one with work
@@ -373,14 +375,16 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv4_attention_join_kernel(con
     __shared__ FindScratch<32 * kJoinWarps> s_find;
     __shared__ float4 s_x[kJoinWarps][32];
     __shared__ float2 s_ml[kJoinWarps];
-    pdl_wait_prior_grids();
-    pdl_release_dependents();
     const Kv4View& c = a.c;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     long long per, all;
     Place pl;
     const int boundary = blockIdx.x + 1;
-    if (!find_unit<32 * kJoinWarps, SPLIT>(c, a.group, tile_rows, SPLIT ? blockIdx.x : boundary, parts, s_find, &per, &all, &pl)) return;
+    // the attention in front releases this launch behind its own wait: what it read of the lengths is settled
+    const bool work = find_unit<32 * kJoinWarps, SPLIT>(c, a.group, tile_rows, SPLIT ? blockIdx.x : boundary, parts, s_find, &per, &all, &pl);
+    pdl_wait_prior_grids();
+    pdl_release_dependents();
+    if (!work) return;
     const int tile_head = static_cast<int>(SPLIT ? pl.in_seq : pl.in_seq / pl.w.units);
     const long long unit0 = pl.units_before + static_cast<long long>(tile_head) * pl.w.units;
     if (!SPLIT && (unit0 == per * boundary || unit0 < per * (boundary - 1))) return;
@@ -447,10 +451,9 @@ constexpr int kWeightRows = 128, kWeightPositions = 32 * kAttnWarps;
 __global__ void __launch_bounds__(kAttnThreads, 3) kv4_key_weight_kernel(const __grid_constant__ Kv4WeightArgs a) {
     __shared__ uint4 s_q[kWeightRows / 8][4][32];
     __shared__ float2 s_row[kWeightRows];                    // sum of q, -lse, both in the exponent's units
-    pdl_wait_prior_grids();
-    pdl_release_dependents();
     const Kv4View& c = a.c;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    if (!c.settled) pdl_wait_prior_grids();
     const int head = blockIdx.y, b = blockIdx.z, ps = 1 << c.page_shift;
     const int first = blockIdx.x * a.positions + warp * 32;
     const int2 mine = kv4_new_tokens(c, b);
@@ -458,6 +461,8 @@ __global__ void __launch_bounds__(kAttnThreads, 3) kv4_key_weight_kernel(const _
     const int rows = mine.y * a.group, end = min(min(len, kv4_capacity(c)), (static_cast<int>(blockIdx.x) + 1) * a.positions);
     const float to_log2 = a.scale * kLog2e;
     const int32_t* table = c.table + static_cast<size_t>(b) * c.max_pages;
+    if (c.settled) pdl_wait_prior_grids();
+    pdl_release_dependents();
     if (blockIdx.x * a.positions >= end || rows <= 0) return;
     // what the lane needs of 32 positions: rows at + g + {0, 8, 16, 24}
     struct Raw {

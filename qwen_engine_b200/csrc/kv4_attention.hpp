@@ -1,6 +1,7 @@
 // Arguments and launch plan of attention over the 4-bit key/value cache.
 #pragma once
 
+#include "../../include/w4a16_b200.h"
 #include "kv4.cuh"
 
 namespace w4 {
@@ -53,6 +54,8 @@ int kv4_chunk_timeouts(unsigned int* out);
 inline bool kv4_takes_chunk(int num_tokens, int num_seqs, int q_heads, int kv_heads, bool f32) {
     return !f32 && static_cast<long long>(q_heads / kv_heads) * num_tokens >= 64ll * num_seqs;
 }
+int kv4_check_step(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, int num_q_heads, float softmax_scale, const int32_t* position,
+                   const float* inv_freq, const w4a16_qwenbin_biases* biases, Kv4View* view);
 int kv4_add_key_weights(Kv4WeightArgs a, cudaStream_t stream);
 
 struct Kv4AppendArgs {

@@ -599,11 +599,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
 constexpr int kChunkJoinWarps = 8;
 __global__ void __launch_bounds__(32 * kChunkJoinWarps) kv4_chunk_join_kernel(const __grid_constant__ Kv4ChunkArgs a) {
     __shared__ FindScratch<32 * kChunkJoinWarps> s_find;
-    pdl_wait_prior_grids();
-    pdl_release_dependents();
     const int lane = threadIdx.x & 31, row = blockIdx.y * kChunkJoinWarps + (threadIdx.x >> 5);
     ChunkPlace pl;
-    if (!find_chunk<32 * kChunkJoinWarps>(a.c, a.group, blockIdx.x, s_find, &pl) || row >= pl.rows) return;
+    // released behind the wait of the launch in front, as the other form's join
+    const bool work = find_chunk<32 * kChunkJoinWarps>(a.c, a.group, blockIdx.x, s_find, &pl);
+    pdl_wait_prior_grids();
+    pdl_release_dependents();
+    if (!work || row >= pl.rows) return;
     const int seen = chunk_seen(a.c, pl, a.group), each = chunk_steps(seen, a.splits) * kChunkKeys;
     const int used = each > 0 ? (seen + each - 1) / each : 0;
     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);

@@ -120,8 +120,6 @@ __global__ void __launch_bounds__(kAppendThreads, 6) kv4_append_kernel(const __g
     __shared__ __align__(16) float2 s_turn[TOK][kKvDim / 2];     // cosine, sine
     __shared__ Spot s_spot[TOK];
     __shared__ int s_pos[TOK];
-    pdl_wait_prior_grids();
-    pdl_release_dependents();
     const Kv4View& c = a.c;
     const int token0 = blockIdx.x / a.blocks_per_token * TOK;
     const int row = (blockIdx.x % a.blocks_per_token) * (kAppendThreads / kRowThreads) + (threadIdx.x >> 4);
@@ -134,16 +132,22 @@ __global__ void __launch_bounds__(kAppendThreads, 6) kv4_append_kernel(const __g
     const __half* src = (kind == 0 ? a.q : kind == 1 ? a.k : a.v) + head * kKvDim + hl * 4;
     const int stride = kind == 0 ? a.q_stride : a.kv_stride;
     uint2 raw[TOK][2], bias[2] = {make_uint2(0, 0), make_uint2(0, 0)};
+    auto fetch = [&]() {
+        pdl_wait_prior_grids();
+        pdl_release_dependents();
 #pragma unroll
-    for (int i = 0; i < TOK; ++i)
+        for (int i = 0; i < TOK; ++i)
 #pragma unroll
-        for (int p = 0; p < 2; ++p)
-            raw[i][p] = on && token0 + i < c.num_tokens ? __ldcg(reinterpret_cast<const uint2*>(src + static_cast<size_t>(token0 + i) * stride + 64 * p)) : make_uint2(0, 0);
-    const __half* b = kind == 0 ? a.q_bias : kind == 1 ? a.k_bias : a.v_bias;
-    if (on && b != nullptr) {
+            for (int p = 0; p < 2; ++p)
+                raw[i][p] = on && token0 + i < c.num_tokens ? __ldcg(reinterpret_cast<const uint2*>(src + static_cast<size_t>(token0 + i) * stride + 64 * p)) : make_uint2(0, 0);
+        const __half* b = kind == 0 ? a.q_bias : kind == 1 ? a.k_bias : a.v_bias;
+        if (on && b != nullptr) {
 #pragma unroll
-        for (int p = 0; p < 2; ++p) bias[p] = __ldcg(reinterpret_cast<const uint2*>(b + head * kKvDim + hl * 4 + 64 * p));
-    }
+            for (int p = 0; p < 2; ++p) bias[p] = __ldcg(reinterpret_cast<const uint2*>(b + head * kKvDim + hl * 4 + 64 * p));
+        }
+    };
+    const bool late = TOK == 1 && c.settled;                     // a decode step: place and angles in front of the wait
+    if (!late) fetch();
     if (warp < TOK) {
         const int token = token0 + warp;
         int pos = 0;
@@ -163,6 +167,7 @@ __global__ void __launch_bounds__(kAppendThreads, 6) kv4_append_kernel(const __g
             s_turn[i >> 6][i & 63] = make_float2(cs, sn);
         }
     }
+    if (late) fetch();
     __syncthreads();
     float bf[8];
     half4_to_float(bias[0], bf);

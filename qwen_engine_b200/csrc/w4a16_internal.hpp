@@ -20,8 +20,6 @@ struct DeviceInfo {
     int cc_major = 0;
     bool ready = false;
 };
-int kv4_check_step(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, int num_q_heads, float softmax_scale, const int32_t* position,
-                   const float* inv_freq, const w4a16_qwenbin_biases* biases);
 int ensure_device_ready(const DeviceInfo** out);  // lazy per-device set-up; returns a status
 bool pdl_enabled();
 int option(int which);                             // current value of a W4A16_OPT_* run-time option
