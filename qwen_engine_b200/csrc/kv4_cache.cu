@@ -113,7 +113,9 @@ __device__ __forceinline__ Spot find_spot(const Kv4View& c, int token) {     // 
 // The rows of TOK tokens: q_heads of q (rotated into q_out), kv_heads of k (rotated, quantised), kv_heads of v (quantised).
 // A CTA takes 16 of a token's rows; all its rows are requested first, then a warp a token finds its place (three dependent
 // round trips), then the threads share the tokens' 64 angles.  Angles are position * inv_freq in 64 bits, reduced to a turn
-// there (a 32-bit angle of position 100 000 is off by 0.004 rad).  What bounds a prompt are those round trips: with one token a
+// there (a 32-bit angle of position 100 000 is off by 0.004 rad), and so are their sines; the products round one by one.  A rotated value is
+// then the 32-bit formula's bit for bit, and no code of a key beside a border between two codes depends on how it was computed (32-bit
+// sines and fused products moved one key in some millions by a whole step of its row; they cost 1 us less of 52).  What bounds a prompt are those round trips: with one token a
 // CTA instead of four 4 prompts of up to 4100 tokens took 79 us.
 template <int TOK>
 __global__ void __launch_bounds__(kAppendThreads, 6) kv4_append_kernel(const __grid_constant__ AppendArgs a) {
@@ -162,9 +164,9 @@ __global__ void __launch_bounds__(kAppendThreads, 6) kv4_append_kernel(const __g
     if (a.inv_freq != nullptr) {
         for (int i = threadIdx.x; i < TOK * kKvDim / 2; i += kAppendThreads) {
             const double turns = static_cast<double>(s_pos[i >> 6]) * static_cast<double>(__ldcg(a.inv_freq + (i & 63))) * 0.15915494309189533577;
-            float sn, cs;
-            sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sn, &cs);
-            s_turn[i >> 6][i & 63] = make_float2(cs, sn);
+            double sn, cs;
+            sincospi(2.0 * (turns - rint(turns)), &sn, &cs);
+            s_turn[i >> 6][i & 63] = make_float2(static_cast<float>(cs), static_cast<float>(sn));
         }
     }
     if (late) fetch();
@@ -188,8 +190,8 @@ __global__ void __launch_bounds__(kAppendThreads, 6) kv4_append_kernel(const __g
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float u = x[j], v = x[j + 4];
-                x[j] = u * cs[j] - v * sn[j];
-                x[j + 4] = v * cs[j] + u * sn[j];
+                x[j] = __fsub_rn(__fmul_rn(u, cs[j]), __fmul_rn(v, sn[j]));
+                x[j + 4] = __fadd_rn(__fmul_rn(v, cs[j]), __fmul_rn(u, sn[j]));
             }
         }
         const __half2 h[4] = {__floats2half2_rn(x[0], x[1]), __floats2half2_rn(x[2], x[3]), __floats2half2_rn(x[4], x[5]), __floats2half2_rn(x[6], x[7])};
