@@ -109,6 +109,12 @@ __device__ __forceinline__ bool park_wait(uint32_t bar, uint32_t parity, volatil
 __device__ __forceinline__ bool park_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
     return __all_sync(0xFFFFFFFFu, park_wait(bar, parity, abort_flag));
 }
+// Barrier of the operand warps: whether all of them are well.  A warp whose wait ran out comes here too, so none is left waiting.
+__device__ __forceinline__ bool all_of_256(bool ok) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"(static_cast<uint32_t>(ok)) : "memory");
+    return r != 0;
+}
 // Two 32-bit operations in one instruction, the exponential and the conversion, all volatile: their order is the software pipeline
 // of softmax_pass.
 __device__ __forceinline__ void fma2(float& x, float& y, float2 b, float2 c) {
@@ -218,7 +224,9 @@ __device__ __forceinline__ uint32_t operand_at(int row, int chunk) {
 
 __device__ __forceinline__ uint32_t extra_at(int row, int chunk) { return static_cast<uint32_t>(row * 32 + ((chunk ^ ((row >> 2) & 1)) << 4)); }
 
-// The (tile, head) of a CTA: long ones first, which are the last ones of a sequence.
+// The (tile, head) of a CTA.  (All steps of the batch shared evenly by 148 persistent CTAs took 780 us where this takes 765 and 102 where it
+// takes 57, for all that 20 and 50 of the SMs have nothing to do here: a piece costs 14 us beside its steps, for queries, first scores,
+// the second pass over the first step and its parts.)  Long ones first, which are the last ones of a sequence.
 struct ChunkPlace {
     SeqWork w;
     int seq, head, row0, rows;
@@ -464,10 +472,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
             page = page_of(0);
             fetch(0);
         }
+        bool ok = true;
         for (int j = 0; j < steps; ++j) {
             const int slot = j & 1;
             // ---- keys, first: the scores of the next step wait for them ----
-            if (!park_warp(k_empty, (j & 1) ^ 1, s_abort)) break;
+            ok = ok && park_warp(k_empty, (j & 1) ^ 1, s_abort);
             const uint32_t here = __ballot_sync(0xFFFFFFFFu, there), bad = __ballot_sync(0xFFFFFFFFu, nan_params(vp));
             if (part == 0 && lane == 0) {
                 s_mask[j & 3][0][warp & 3] = here;
@@ -504,9 +513,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
             asm volatile("cp.async.wait_group 0;" ::: "memory");
             uint32_t* params = reinterpret_cast<uint32_t*>(smem + kSmemParam) + slot * kChunkKeys;
             if (part == 0) params[t] = nan_params(vp) ? 0u : finite_params(vp);
-            asm volatile("bar.sync 1, 256;" ::: "memory");        // every position's codes and parameters are there, and the step before has been read
+            if (!all_of_256(ok)) break;         // every position's codes and parameters are there, and the step before has been read
             if (j + 1 < steps) fetch(j + 1);
-            if (!park_warp(v_empty(slot), ((j >> 1) & 1) ^ 1, s_abort)) break;
+            ok = park_warp(v_empty(slot), ((j >> 1) & 1) ^ 1, s_abort);
+            if (!ok) continue;
             uint8_t* to = smem + kSmemV + slot * kOperand;
             const uint8_t* stage = smem + kSmemStage + slot * kValueStage;
             const int o8 = (lane & 7) + 8 * part;               // eight positions
