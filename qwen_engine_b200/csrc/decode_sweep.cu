@@ -2,6 +2,7 @@
 // the reference engine's order (reference src/engine.cu:361-451), captured once into a CUDA
 // graph like the engine's decode graph (src/engine.cu:453-470).  Host C++ only; the kernels
 // are the library's ordinary launchers.
+#include <exception>
 #include <memory>
 #include <new>
 #include <vector>
@@ -408,9 +409,13 @@ int64_t w4a16_sweep_kv4_workspace_bytes(int num_q_heads, int num_kv_heads) {
     return n < 0 ? n : static_cast<int64_t>(carve_kv4(num_q_heads, num_kv_heads).total);
 }
 
-int w4a16_sweep_create(const w4a16_sweep_desc* desc, w4a16_stream_t stream, w4a16_sweep** out) { return create_sweep(desc, nullptr, nullptr, stream, out); }
+int w4a16_sweep_create(const w4a16_sweep_desc* desc, w4a16_stream_t stream, w4a16_sweep** out) try {
+    return create_sweep(desc, nullptr, nullptr, stream, out);
+} catch (const std::exception&) {
+    return static_cast<int>(cudaErrorMemoryAllocation);      // the copies of the host arrays
+}
 
-int w4a16_sweep_create_kv4(const w4a16_sweep_desc* desc, const w4a16_sweep_kv4* kv, w4a16_stream_t stream, w4a16_sweep** out) {
+int w4a16_sweep_create_kv4(const w4a16_sweep_desc* desc, const w4a16_sweep_kv4* kv, w4a16_stream_t stream, w4a16_sweep** out) try {
     if (!desc || !kv || !kv->caches || !kv->workspace) return W4A16_ERR_INVALID_ARG;
     if (desc->head_dim != 128 || (desc->flags & W4A16_SWEEP_PERSISTENT)) return W4A16_ERR_SHAPE;
     if (kv->batch.num_seqs != 1 || kv->batch.num_tokens != 1 || kv->batch.query_start) return W4A16_ERR_INVALID_ARG;
@@ -425,6 +430,8 @@ int w4a16_sweep_create_kv4(const w4a16_sweep_desc* desc, const w4a16_sweep_kv4* 
         views[l].settled = true;
     }
     return create_sweep(desc, kv, &views, stream, out);
+} catch (const std::exception&) {
+    return static_cast<int>(cudaErrorMemoryAllocation);
 }
 
 int w4a16_sweep_destroy(w4a16_sweep* s) {

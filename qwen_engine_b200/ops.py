@@ -313,6 +313,9 @@ class SweepCache:
         """The C struct with a workspace of its own, and what has to live as long as the sweep."""
         if len(self.caches) != num_layers or (self.biases is not None and len(self.biases) != num_layers):
             raise ValueError("one cache, and one entry of biases, a layer expected")
+        for name, t, dtype, n in (("position", self.position, torch.int32, 1), ("rope_inv_freq", self.rope_inv_freq, torch.float32, 64)):
+            if t is not None and (t.dtype != dtype or t.numel() != n or not t.is_contiguous()):
+                raise ValueError(f"{name}: {n} contiguous values of {dtype} expected")
         nbytes = load().w4a16_sweep_kv4_workspace_bytes(num_q_heads, num_kv_heads)
         if nbytes < 0:
             check("w4a16_sweep_kv4_workspace_bytes", int(nbytes))

@@ -173,3 +173,17 @@ def test_a_sweep_cache_asks_for_one_cache_a_layer():
     for bad in (SweepCache([cache], batch, 0.1), SweepCache([cache] * 2, batch, 0.1, biases=[None])):
         with pytest.raises(ValueError, match="a layer"):
             bad.pod(2, 4, 2)
+    for bad in (dict(position=torch.zeros(1)), dict(position=torch.zeros(2, dtype=torch.int32)), dict(rope_inv_freq=torch.zeros(128)[::2])):
+        with pytest.raises(ValueError, match="contiguous values"):
+            SweepCache([cache] * 2, batch, 0.1, **bad).pod(2, 4, 2)
+
+
+@pytest.mark.parametrize("version", [1, 2])
+def test_the_bias_table_is_the_file_s(lib, version):
+    import pathlib
+    from qwen_engine_b200.qwenbin import QwenBin
+    qb = QwenBin(pathlib.Path(__file__).parent / "golden" / f"tiny_w4a16_v{version}.qwenbin")
+    table, (_, _, want) = qb.bias_table(qb.host_base()), qb.tensors(qb.host_base())
+    assert [{n: getattr(b, n) for n, _ in b._fields_} for b in table] == want
+    heads = qb.dims()["num_q_heads"] * 128
+    assert all(b["q_bias"] is None or qb.host_base() <= b["q_bias"] <= qb.host_base() + qb.bytes.size - 2 * heads for b in want)
