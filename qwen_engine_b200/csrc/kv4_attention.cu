@@ -118,20 +118,67 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
     const int seen = min(max(q.past + (q.row0 + q.rows - 1) / a.group + 1, 0), kv4_capacity(c));
     const int k0 = unit0 * kUnit, k1 = min(k0 + units * kUnit, seen);
 
+    // A page outside the pool is a step without copies.
+    const uint8_t* ring = s_ring[warp];
+    const TileCopy copy(c, head, lane, static_cast<uint32_t>(__cvta_generic_to_shared(ring)));
+    const int32_t* table = c.table + static_cast<size_t>(q.seq) * c.max_pages;
+    const int first_at = k0 + warp * kKvTile, steps = first_at < k1 ? (k1 - first_at + kUnit - 1) / kUnit : 0;
+    auto page_of = [&](int step) { return step < steps ? __ldcg(table + ((first_at + step * kUnit) >> c.page_shift)) : -1; };
+    auto start = [&](int step, int page) {
+        const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(c.num_pages);
+        if (ok) copy.issue(static_cast<uint32_t>(step % kStages) * kStageBytes, page, first_at + step * kUnit, lane);
+        return ok;
+    };
+    // EARLY: page numbers of the first steps at once, all queries, and the rows on their way before the queries are used, instead of five
+    // to nine round trips one behind the other: 8 sequences of 3 to 5 tokens 24.0 -> 20.6 us, 64 sequences 103 -> 100.6.  Eight
+    // 32-bit rows have all registers in use, and what follows gets slower by more: one sequence of 131 001 positions 26.3 us
+    // instead of 25.7, of 32 000 in the decode sweep 866 instead of 814 (of 1021: 610 instead of 620).
+    constexpr bool EARLY = NT == 2 || !F32;
+    static_assert(kStages == 4);
+    int page[kStages] = {page_of(0), -1, -1, -1};
+    if constexpr (EARLY) {
+#pragma unroll
+        for (int i = 1; i < kStages; ++i) page[i] = page_of(i);
+    }
+
     // queries: B fragments of rows g (+ 8), and for the lane's columns 2 t, 2 t + 1 the sum of q and how far the row sees
     float qsum[NT][2];
     int limit[NT][2];
     const float to_log2 = a.scale * kLog2e;
+    [[maybe_unused]] uint4 qw[NT][4];
+    if constexpr (EARLY) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = n * 8 + g, row = q.row0 + r, token = q.first_token + row / a.group, h = head * a.group + row % a.group;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                qw[n][j] = r < q.rows ? __ldcg(reinterpret_cast<const uint4*>(a.q + static_cast<size_t>(token) * a.q_stride + h * kKvDim + 32 * t + 8 * j))
+                                      : make_uint4(0, 0, 0, 0);
+        }
+    }
+    uint32_t there = 0;                                     // bit i: the step i from now has rows
+    auto begin = [&](int i) {
+        if (start(i, page[i])) there |= 1u << i;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if constexpr (EARLY) {
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) begin(i);
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int r = n * 8 + g, row = q.row0 + r;
         float s = 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             uint4 w = make_uint4(0, 0, 0, 0);
-            if (r < q.rows) {
-                const int token = q.first_token + row / a.group, h = head * a.group + row % a.group;
-                w = __ldcg(reinterpret_cast<const uint4*>(a.q + static_cast<size_t>(token) * a.q_stride + h * kKvDim + 32 * t + 8 * j));
+            if constexpr (EARLY) {
+                w = qw[n][j];
+            } else {
+                const int r = n * 8 + g, row = q.row0 + r;
+                if (r < q.rows) {
+                    const int token = q.first_token + row / a.group, h = head * a.group + row % a.group;
+                    w = __ldcg(reinterpret_cast<const uint4*>(a.q + static_cast<size_t>(token) * a.q_stride + h * kKvDim + 32 * t + 8 * j));
+                }
             }
             s += sum_half8(w);
             if (j == warp) s_q[n][j][lane] = query_words(w);
@@ -154,9 +201,6 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
 
     float mu[NT][2];                                        // m, or 0 where nothing has been seen
     for (int n = 0; n < NT; ++n) mu[n][0] = mu[n][1] = 0.0f;
-    const uint8_t* ring = s_ring[warp];
-    const TileCopy copy(c, head, lane, static_cast<uint32_t>(__cvta_generic_to_shared(ring)));
-    const int32_t* table = c.table + static_cast<size_t>(q.seq) * c.max_pages;
     const int pos = key_position(g);                        // positions of rows g and g + 8 of A: pos and pos + 8
     const int value_from = kStageValues + 64 * t + ((8 * g) ^ (16 * (t & 2)));
     // CUT: some row does not see some of these positions
@@ -245,7 +289,8 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
         }
         vs[0] *= pw;
         vs[1] *= pw;
-        uint32_t ph[NT][2], pl[NT][2];                      // p * value scale in one or two fp16 parts, columns = positions
+        uint32_t ph[NT][2];
+        [[maybe_unused]] uint32_t pl[NT][2];                      // p * value scale in one or two fp16 parts, columns = positions
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             float x[4];
@@ -289,10 +334,15 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
         }
     };
 
-    // a page number is fetched one step before the copies that need it; a page outside the pool is a step without copies
-    const int first_at = k0 + warp * kKvTile, steps = first_at < k1 ? (k1 - first_at + kUnit - 1) / kUnit : 0;
-    uint32_t there = 0;                                     // bit i: the step i from now has rows
-    int next_page = steps > 0 ? __ldcg(table + (first_at >> c.page_shift)) : -1;
+    if constexpr (!EARLY) {
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) {
+            begin(i);
+            page[i + 1] = page_of(i + 1);
+        }
+    }
+    int next_page = page[kStages - 1];
+    // a page number is fetched one step before the copies that need it
     auto ahead = [&](int step) {
         const bool ok = step < steps && static_cast<unsigned>(next_page) < static_cast<unsigned>(c.num_pages);
         if (ok) copy.issue(static_cast<uint32_t>(step % kStages) * kStageBytes, next_page, first_at + step * kUnit, lane);
@@ -300,11 +350,6 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
         if (step + 1 < steps) next_page = __ldcg(table + ((first_at + (step + 1) * kUnit) >> c.page_shift));
         there |= (ok ? 1u : 0u) << (kStages - 1);
     };
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) {
-        ahead(i);
-        there >>= 1;
-    }
     for (int i = 0; i < steps; ++i) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
         __syncwarp();                                       // every lane's copies are there, and the slot of the step before has been read
