@@ -501,7 +501,8 @@ W4A16_API int w4a16_attention_kv4(const w4a16_kv4_cache* cache, const w4a16_kv4_
 /*
  * key_weight[position] += sum over the batch's tokens that see it and over the query heads of its group of
  * exp(softmax_scale * q . key - lse): how much attention each cached position got from these tokens.  q and lse are those
- * of the attention call; passing only the last tokens of each sequence adds up an observation window.
+ * of the attention call; passing only the last tokens of each sequence adds up an observation window.  Sequences may
+ * share pages: each adds its part (the order, so the last bits, may then differ from run to run).
  */
 W4A16_API int w4a16_kv4_add_key_weights(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, const void* q,
                                         const float* lse, int num_q_heads, float softmax_scale, int q_stride,

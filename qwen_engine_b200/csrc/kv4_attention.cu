@@ -486,8 +486,9 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv4_attention_join_kernel(con
 
 // ---- attention weight of the cached positions ------------------------------------------------------------------
 
-// A warp takes 32 positions of a head and adds up, over all query rows of the sequence, exp(score - lse): no position is
-// another warp's, so nothing is atomic and the order of the sum is fixed.  The queries pass through shared memory in blocks of up to
+// A warp takes 32 positions of a head and adds up, over all query rows of the sequence, exp(score - lse), and
+// adds that to the position's weight: one addition in memory for each block of rows, atomic because sequences may share pages (a common
+// prefix).  Positions of one sequence alone get the same bits every time, as one thread makes all their additions.  The queries pass through shared memory in blocks of up to
 // 128 rows, in fragment order, and stay there while the CTA walks over its positions; the codes of the next 32 are on their way
 // meanwhile.  What bounds it is the rate of mma.sync (with a block of rows staged for each 128 positions it was the staging: the last 32
 // tokens of two sequences of 32 000 and 20 000 positions, 32 heads on 8, took 111 us).
@@ -561,8 +562,7 @@ __global__ void __launch_bounds__(kAttnThreads, 3) kv4_key_weight_kernel(const _
         __syncthreads();
         for (int at = first; at < end; at += kWeightPositions) {
             uint32_t codes[2][4][2][4];
-            float ks[4], kz[4], got[4] = {}, old[4] = {};
-            float* weight[4];
+            float ks[4], kz[4], got[4] = {};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 ks[k] = kv4_scale(raw.params[k]);
@@ -572,13 +572,11 @@ __global__ void __launch_bounds__(kAttnThreads, 3) kv4_key_weight_kernel(const _
                 kv4_centred_codes(raw.w[k].y, codes[k >> 1][1][k & 1]);
                 kv4_centred_codes(raw.w[k].z, codes[k >> 1][2][k & 1]);
                 kv4_centred_codes(raw.w[k].w, codes[k >> 1][3][k & 1]);
-                const int p = at + 8 * k + g;
-                weight[k] = nullptr;
-                if (t == 0 && p < end && static_cast<unsigned>(raw.page[k >> 1]) < static_cast<unsigned>(c.num_pages)) {
-                    weight[k] = c.key_weight + kv4_weight_index(c, raw.page[k >> 1], head, p);
-                    old[k] = __ldcg(weight[k]);
-                }
             }
+            // the lane's position in the end: 8 t + g, so that a warp's additions are one instruction on 128 bytes
+            const int mine_at = at + 8 * t + g, mine_page = t < 2 ? raw.page[0] : raw.page[1];
+            float* weight = nullptr;
+            if (mine_at < end && static_cast<unsigned>(mine_page) < static_cast<unsigned>(c.num_pages)) weight = c.key_weight + kv4_weight_index(c, mine_page, head, mine_at);
             raw.page[0] = next[0];
             raw.page[1] = next[1];
             fetch(at + kWeightPositions);
@@ -621,8 +619,9 @@ __global__ void __launch_bounds__(kAttnThreads, 3) kv4_key_weight_kernel(const _
             for (int k = 0; k < 4; ++k) {
                 got[k] += __shfl_xor_sync(0xFFFFFFFFu, got[k], 1);
                 got[k] += __shfl_xor_sync(0xFFFFFFFFu, got[k], 2);
-                if (weight[k] != nullptr) __stcg(weight[k], old[k] + got[k]);
             }
+            const float sum = t < 2 ? (t == 0 ? got[0] : got[1]) : t == 2 ? got[2] : got[3];
+            if (weight != nullptr && sum != 0.0f) atomicAdd(weight, sum);
         }
     }
 }

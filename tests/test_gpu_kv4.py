@@ -631,3 +631,21 @@ def test_two_sweeps_from_one_cache_object_keep_their_workspaces(ops):
     # 3 launches a layer more than the sweep without caches: append, attention, its join
     plain = ops.DecodeSweep(L, hidden=H, inter=inter, num_q_heads=4, num_kv_heads=2)
     assert one.launches == plain.launches + 2 * 3
+
+
+def test_key_weights_of_pages_that_sequences_share(ops):
+    """Forty sequences over one prefix (their tables begin with the same pages): a position's weight is the sum over all of them.
+    Every addition may be off by half a step of the total on top of what each sequence's own sum may be off."""
+    seqs, kv, heads, page, shared = 40, 2, 4, 16, 6
+    lens = [page * shared + 3 + b % 11 for b in range(seqs)]
+    rng, pool, table, cache, batch = make(ops, 21, lens, [1] * seqs, kv, page)
+    table[:, :shared] = table[0, :shared]
+    batch = ops.KV4Batch.of(i32(table), batch.seq_lens)
+    q = (1.2 * rng.standard_normal((seqs, heads, 128))).astype(BF)
+    lse = ref.attention(pool, table, lens, [1] * seqs, q, SCALE)[1].astype(np.float32)
+    add, rel = ref.key_weights(pool, table, lens, [1] * seqs, q, lse.astype(np.float64), SCALE)
+    ops.kv4_add_key_weights(cache, batch, util.to_dev(q), util.to_dev(lse), heads, SCALE)
+    want = pool.weight + add
+    got = util.to_np(cache.key_weight)
+    assert np.all(np.abs(got - want) <= add * rel + seqs * np.abs(want) * 2.0 ** -24)
+    assert np.array_equal(got[add == 0], pool.weight[add == 0])
