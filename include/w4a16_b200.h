@@ -600,7 +600,7 @@ typedef struct w4a16_sweep_kv4 {
     const struct w4a16_qwenbin_biases* biases;     /* host array [num_layers], entries may hold NULL; NULL: none */
     const int32_t* position;                       /* device [1] rotary position; NULL: the cached position */
     const float* rope_inv_freq;                    /* device [64]; NULL: no rotation */
-    void* workspace;                               /* device, w4a16_sweep_kv4_workspace_bytes(), 256-byte aligned */
+    void* workspace;                               /* device, w4a16_sweep_kv4_workspace_bytes(), 256-byte aligned, no other sweep's */
     float softmax_scale;
     int add_key_weights;                           /* nonzero: every cache needs key_weight */
 } w4a16_sweep_kv4;

@@ -649,3 +649,31 @@ def test_key_weights_of_pages_that_sequences_share(ops):
     got = util.to_np(cache.key_weight)
     assert np.all(np.abs(got - want) <= add * rel + seqs * np.abs(want) * 2.0 ** -24)
     assert np.array_equal(got[add == 0], pool.weight[add == 0])
+
+
+def test_decode_sweep_goes_on_after_an_eviction(ops):
+    """Three steps, every layer's cache cut to 16 positions on a fresh page, table and lengths copied into the sweep's arrays, three more
+    steps: hidden state, pages and weights as the separate calls leave them."""
+    heads, kv, page, length = 4, 1, 32, 20
+    H, inter, L, cache, sweep, _ = sweep_case(ops, 3, heads, kv, page, length, ops.SWEEP_DEFAULT, True)
+    other = ops.SweepCache([ops.KV4Cache(c.pages.clone(), c.key_weight.clone(), c.num_pages, kv, page) for c in cache.caches],
+                           cache.batch, SCALE, cache.biases, cache.position, cache.rope_inv_freq, True)
+    h = util.to_dev(np.random.default_rng(4).standard_normal(H).astype(BF))
+    table, lens = cache.batch.block_table, cache.batch.seq_lens
+    for step in range(6):
+        if step == 3:
+            fresh = i32([[next(p for p in range(3) if p != table.item())]])
+            new_lens, kept = i32([0]), i32(np.zeros((1, kv, 16)))
+            for c in cache.caches + other.caches:
+                ops.kv4_evict(c, cache.batch, fresh, new_lens, kept, 1, 16, 4, 6)
+            table.copy_(fresh), lens.copy_(new_lens)
+            assert lens.item() == 16
+        lens.add_(1)
+        cache.position.add_(1)
+        out = torch.empty_like(h)
+        sweep.run_device(h, out)
+        assert torch.equal(out, separate_calls(ops, H, inter, L, other, heads, h)) and torch.isfinite(out).all(), step
+        for a, b in zip(cache.caches, other.caches):
+            assert torch.equal(a.pages, b.pages) and torch.equal(a.key_weight, b.key_weight), step
+        h = out
+    sweep.close()
