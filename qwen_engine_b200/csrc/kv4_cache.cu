@@ -1,6 +1,7 @@
 // The 4-bit key/value cache: rows in (bias, rotary position, quantisation), rows back as numbers, and eviction to fresh pages.
 #include "kv4.cuh"
 #include "kv4_attention.hpp"
+#include "kv4_select.hpp"
 #include "w4a16_internal.hpp"
 
 namespace w4 {
@@ -290,11 +291,9 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 //   5. the rows copied, shared out evenly over the cluster, eight lanes a position (16 bytes each), four positions in flight.
 // Integer counts and a fixed order throughout, so equal weights fall the same way every time.
 constexpr int kEvictThreads = 1024, kEvictWarps = kEvictThreads / 32;
-constexpr int kEvictBins = 2048, kEvictCoarse = kEvictBins / 32;
+constexpr int kEvictCoarse = kEvictBins / 32;
 constexpr int kEvictCached = 16384;      // keys of a slice in shared memory
 constexpr int kEvictMaxCluster = 8;
-constexpr uint32_t kEvictFirst = 0xAF800000u;     // key of 2^-32
-constexpr int kEvictFirstShift = 18;
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -344,7 +343,8 @@ __global__ void __launch_bounds__(kEvictThreads, 1) kv4_evict_kernel(const __gri
     };
     auto key_at = [&](int i) -> uint32_t { return cached ? s_keys[i - s0] : key_from(i); };
     const int m0 = max(s0, lo), m1 = min(s1, hi);                                      // this CTA's share of the middle
-    uint32_t first = kEvictFirst, last = kEvictFirst + (static_cast<uint32_t>(kEvictBins) << kEvictFirstShift) - 1, need = want;
+    KeyRange range;
+    uint32_t need = want;
     if (want > 0) {
         if (cached) {
             // quads lie in one page, and a page's weights are there whatever the length is
@@ -368,15 +368,13 @@ __global__ void __launch_bounds__(kEvictThreads, 1) kv4_evict_kernel(const __gri
                             make_uint4(weight_key(w[d].x), weight_key(w[d].y), weight_key(w[d].z), weight_key(w[d].w));
             }
         }
-        int shift = kEvictFirstShift;
-        bool clamp = true;                                       // the first round counts every key, the ends' bins all beyond them
         while (true) {
             for (int i = tid; i < kEvictBins; i += kEvictThreads) s_hist[i] = 0;
             __syncthreads();
             for (int i = m0 + tid; i < m1; i += kEvictThreads) {
                 uint32_t k = key_at(i);
-                if (clamp) k = min(max(k, first), last);
-                if (k >= first && k <= last) atomicAdd(&s_hist[(k - first) >> shift], 1u);
+                if (range.clamp) k = min(max(k, range.first), range.last);
+                if (k >= range.first && k <= range.last) atomicAdd(&s_hist[(k - range.first) >> range.shift], 1u);
             }
             __syncthreads();
             for (int k = warp; k < kEvictCoarse; k += kEvictWarps) {
@@ -420,17 +418,12 @@ __global__ void __launch_bounds__(kEvictThreads, 1) kv4_evict_kernel(const __gri
             barrier();                                           // and the histograms may be cleared
             const uint32_t bin = s_found[0];
             need = s_found[1];
-            const uint32_t base = first;
-            first = clamp && bin == 0 ? 0u : base + (bin << shift);
-            last = clamp && bin == kEvictBins - 1 ? ~0u : base + (bin << shift) + ((1u << shift) - 1u);
-            if (first == last) break;
-            const int bits = 32 - __clz(last - first);
-            shift = max(bits - 11, 0);
-            clamp = false;
+            range = narrowed(range, bin);
+            if (range.first == range.last) break;
             __syncthreads();                                     // s_found has been read
         }
     }
-    const uint32_t prefix = first;
+    const uint32_t prefix = range.first;
     // what stays: outside the middle, keys above `prefix`, and the first `need` of those equal to it
     const int run = ((s1 - s0 + kEvictWarps - 1) / kEvictWarps + 31) & ~31;
     const int r0 = min(s0 + warp * run, s1), r1 = min(r0 + run, s1);

@@ -342,6 +342,48 @@ def test_eviction(ops, lens, kv, page, budget, sink, recent, kind):
                     assert weight[dst[b, j // page], h, slot] == 9
 
 
+def check_eviction(ops, lens, kv, page, budget, sink, recent, weight_of, stale=0x7FFFFFFF):
+    """An eviction of sequences on pages of the pool, whole records compared.  `stale`: what the list of kept positions holds before."""
+    rng = np.random.default_rng(30)
+    B, per, dst_per = len(lens), -(-max(lens) // page), -(-budget // page)
+    n = B * (per + dst_per)
+    table = rng.permutation(n).reshape(B, per + dst_per).astype(np.int32)
+    table, dst = table[:, :per].copy(), table[:, per:].copy()
+    words = rng.integers(0, 1 << 32, (n, kv, 34 * page), dtype=np.uint32)
+    weight = weight_of(rng, (n, kv, page)).astype(np.float32)
+    cache = ops.KV4Cache(util.to_dev(words), util.to_dev(weight), n, kv, page)
+    new_lens, kept = i32(np.full(B, 77)), i32(np.full((B, kv, budget), stale))
+    ops.kv4_evict(cache, ops.KV4Batch.of(i32(table), i32(lens)), i32(dst), new_lens, kept, dst_per, budget, sink, recent)
+    got_words, got_weight, kept = words_of(cache), util.to_np(cache.key_weight), util.to_np(kept)
+    assert util.to_np(new_lens).tolist() == [min(L, budget) for L in lens]
+    for b, L in enumerate(lens):
+        for h in range(kv):
+            want = np.array(ref.evict(weight, table[b], L, h, page, n, budget, sink, recent))
+            assert np.array_equal(kept[b, h], np.append(want, np.full(budget - len(want), -1))), (b, h)
+            new = np.arange(len(want))
+            from_, to = (table[b, want // page], h, want % page), (dst[b, new // page], h, new % page)
+            for part in range(2):
+                codes = slice(part * 16 * page, (part + 1) * 16 * page)
+                view = lambda w: w[..., codes].reshape(n, kv, page, 16)  # noqa: E731
+                assert np.array_equal(view(got_words)[to], view(words)[from_])
+                params = slice((32 + part) * page, (33 + part) * page)
+                assert np.array_equal(got_words[..., params][to], words[..., params][from_])
+            assert np.array_equal(got_weight[to], weight[from_], equal_nan=True)
+
+
+@pytest.mark.parametrize("budget", [65, 700, 1500, 2200, 2990])
+@pytest.mark.parametrize("kind", ["low", "zeros", "high", "wide"])
+def test_eviction_of_weights_at_the_ends_of_the_searchs_first_range(ops, budget, kind):
+    """Weights densely around 2^-32 (what a peaked head leaves to most positions) and 2^32, where the first histogram's bins end."""
+    def weights(rng, shape):
+        if kind == "zeros":
+            return rng.uniform(1.0, 1.3, shape) * 2.0 ** -32 * rng.choice([0, 1, 1], shape)
+        if kind == "wide":
+            return np.exp(rng.uniform(-40, 0, shape))
+        return 2.0 ** rng.uniform(-1, 1, shape) * 2.0 ** (32 if kind == "high" else -32)
+    check_eviction(ops, [3000, 2500], 2, 16, budget, 4, 60, weights)
+
+
 # ---- as they are used ----------------------------------------------------------------------------------------------------
 
 

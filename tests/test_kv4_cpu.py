@@ -187,3 +187,73 @@ def test_the_bias_table_is_the_file_s(lib, version):
     assert [{n: getattr(b, n) for n, _ in b._fields_} for b in table] == want
     heads = qb.dims()["num_q_heads"] * 128
     assert all(b["q_bias"] is None or qb.host_base() <= b["q_bias"] <= qb.host_base() + qb.bytes.size - 2 * heads for b in want)
+
+
+SEARCH = r"""
+// The eviction's search on host arrays: per line of input a count `need` and keys; prints the key of rank `need` from the top as the
+// ranges of kv4_select.hpp lead to it, how many of that key are still to be taken, and how many keys lie above it.
+#include <cstdio>
+#include <iostream>
+#include <sstream>
+#include <string>
+#include <vector>
+#include "kv4_select.hpp"
+int main() {
+    for (std::string line; std::getline(std::cin, line);) {
+        std::istringstream in(line);
+        uint32_t need, k;
+        in >> need;
+        std::vector<uint32_t> keys;
+        while (in >> k) keys.push_back(k);
+        w4::KeyRange r;
+        int rounds = 0;
+        while (r.first != r.last && ++rounds < 8) {
+            std::vector<uint32_t> hist(w4::kEvictBins);
+            for (uint32_t key : keys) {
+                if (r.clamp) key = key < r.first ? r.first : key > r.last ? r.last : key;
+                if (key >= r.first && key <= r.last) ++hist.at((key - r.first) >> r.shift);
+            }
+            int bin = w4::kEvictBins - 1;
+            for (; bin > 0 && hist[bin] < need; --bin) need -= hist[bin];
+            r = w4::narrowed(r, bin);
+        }
+        uint32_t above = 0;
+        for (uint32_t key : keys) above += key > r.last;
+        std::printf("%u %u %u %d\n", r.last, need, above, rounds);
+    }
+}
+"""
+
+
+def test_the_evictions_search_finds_the_key_of_a_rank(lib, tmp_path):
+    """Weights around both ends of the first range (2^-32, 2^32), zeros, infinities and NaNs among them, and all over fp32: the key found is
+    the one of that rank, and what is still to be taken of it makes the count whole."""
+    import pathlib
+    import subprocess
+
+    import numpy as np
+    csrc = pathlib.Path(__file__).parents[1] / "qwen_engine_b200" / "csrc"
+    (tmp_path / "search.cpp").write_text(SEARCH)
+    subprocess.run(["g++", "-std=c++20", "-O1", f"-I{csrc}", "-o", str(tmp_path / "search"), str(tmp_path / "search.cpp")], check=True)
+    rng = np.random.default_rng(2)
+
+    def keys_of(w):
+        u = (w.astype(np.float32) + np.float32(0)).view(np.uint32)
+        k = np.where(u >> np.uint32(31), ~u, u | np.uint32(1 << 31))
+        return np.where(np.isnan(w), 0, k).astype(np.uint32)
+
+    sets = []
+    for i in range(300):
+        n = int(rng.integers(1, 400))
+        mid = 2.0 ** [-32, 32, 0][i % 3]
+        w = mid * [2.0 ** rng.uniform(-1, 1, n), rng.uniform(1.0, 1.3, n), np.exp(6 * rng.standard_normal(n))][i // 3 % 3]
+        w *= rng.choice([1, 1, 1, 0, -1], n)
+        if i % 5 == 0:
+            w[rng.random(n) < 0.2] = rng.choice([np.inf, np.nan, -np.inf, 1e38, 1e-40])
+        sets.append((keys_of(w), int(rng.integers(1, n + 1))))
+    sets.append((keys_of(np.array([1.01] * 300 + [1.1] * 200 + [5.0] * 100) * 2.0 ** -32), 400))
+    lines = "\n".join(" ".join(map(str, [need, *k.tolist()])) for k, need in sets)
+    out = subprocess.run([str(tmp_path / "search")], input=lines + "\n", capture_output=True, text=True, check=True, timeout=60).stdout.split("\n")
+    for (k, need), line in zip(sets, out):
+        key, left, above, rounds = map(int, line.split())
+        assert key == np.sort(k)[::-1][need - 1] and above == (k > key).sum() and above + left == need and rounds <= 4
