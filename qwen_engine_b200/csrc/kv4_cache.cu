@@ -479,7 +479,11 @@ __global__ void __launch_bounds__(kEvictThreads, 1) kv4_evict_kernel(const __gri
     for (int j0 = static_cast<int>(rank) * (kEvictThreads / 8) + (tid >> 3); j0 < keep; j0 += kMove * groups) {
         int i[kMove], from[kMove], to[kMove];
 #pragma unroll
-        for (int u = 0; u < kMove; ++u) i[u] = j0 + u * groups < keep ? __ldcg(kept + j0 + u * groups) : -1;
+        for (int u = 0; u < kMove; ++u) {
+            i[u] = j0 + u * groups < keep ? __ldcg(kept + j0 + u * groups) : -1;
+            // weights that change while they are read can leave the list short: what it held before is no position
+            if (static_cast<unsigned>(i[u]) >= static_cast<unsigned>(len)) i[u] = -1;
+        }
 #pragma unroll
         for (int u = 0; u < kMove; ++u) {
             from[u] = to[u] = -1;

@@ -384,6 +384,12 @@ def test_eviction_of_weights_at_the_ends_of_the_searchs_first_range(ops, budget,
     check_eviction(ops, [3000, 2500], 2, 16, budget, 4, 60, weights)
 
 
+@pytest.mark.parametrize("budget,sink,recent", [(300, 4, 64), (135000, 0, 1)])
+def test_eviction_of_more_positions_than_shared_memory_holds(ops, budget, sink, recent):
+    """From 131 072 positions on a CTA of the cluster reads its weights again in every pass."""
+    check_eviction(ops, [140001, 131500, 100], 1, 128, budget, sink, recent, lambda rng, shape: np.round(np.exp(9 * rng.standard_normal(shape)), 3))
+
+
 # ---- as they are used ----------------------------------------------------------------------------------------------------
 
 
