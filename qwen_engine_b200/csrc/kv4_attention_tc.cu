@@ -216,6 +216,10 @@ __device__ __forceinline__ void dequantise(uint32_t w, __half2 s, __half2 z, uin
     }
 }
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
+__device__ __forceinline__ uint32_t sixteenth(uint32_t x) {
+    const __half2 y = __hmul2(as_half2(x), __float2half2_rn(0.0625f));
+    return *reinterpret_cast<const uint32_t*>(&y);
+}
 
 // Row and 16-byte chunk (8 columns) of an operand in shared memory.
 __device__ __forceinline__ uint32_t operand_at(int row, int chunk) {
@@ -310,6 +314,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
         const bool mine = work && row < pl.rows;
         const size_t at_row = mine ? out_row(pl.w, c.kv_heads, a.group, pl.head, pl.row0 + row) : 0;
         const int limit = mine ? pl.w.past + (pl.row0 + row) / a.group + 1 : 0x7FFFFFFF;
+        float to_log2 = a.scale * kLog2e;
         if (steps > 0 && i < tiles) {
             uint4 w[16];
             float qsum = 0.0f;
@@ -324,6 +329,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
                                __byte_perm(w[k].z, w[k].w, 0x7632));
 #pragma unroll
             for (int k = 0; k < 16; ++k) qsum += sum_half8(w[k]);
+            if (fabsf(qsum) > 8.0f * 65504.0f) {
+                // an eighth of the sum is no fp16 number any more: the row a sixteenth of its size (128 * 65504 / 16 is in range again), its scores
+                // the other way.  Exact but for elements below 2^-10, where it is off by 2^-21, in a row whose mean is above 4094.
+#pragma unroll 1
+                for (int k = 0; k < 16; ++k) {
+                    uint4* at = reinterpret_cast<uint4*>(smem + i * kOperand + operand_at(r, k));
+                    *at = make_uint4(sixteenth(at->x), sixteenth(at->y), sixteenth(at->z), sixteenth(at->w));
+                }
+                qsum *= 0.0625f;
+                to_log2 *= 16.0f;
+            }
             const __half part = __float2half_rn(qsum * 0.125f), rest = __float2half_rn(fmaf(qsum, 0.125f, -__half2float(part)));
             const uint32_t pp = pack_half2(__half2float(part), __half2float(part)), rr = pack_half2(__half2float(rest), __half2float(rest));
             *reinterpret_cast<uint4*>(smem + kSmemQx + i * kExtra + extra_at(r, 0)) = make_uint4(pp, pp, pp, pp);
@@ -332,7 +348,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
-        const float to_log2 = a.scale * kLog2e;
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t t_s = lanes + static_cast<uint32_t>(i * 128), t_o = lanes + static_cast<uint32_t>(kTmemO + i * 128);
         // m: reference of the exponents, at most 15 below the row's largest so far and renewed where it is 8 below; grow: by how much, at

@@ -280,6 +280,21 @@ def test_attention_with_steep_scores(ops, tokens, f32):
     check_attention(got, lse, want, tokens, f32)
 
 
+@pytest.mark.parametrize("tokens,f32", [(100, False), (3, False), (3, True)])
+def test_attention_of_queries_as_large_as_fp16_goes(ops, tokens, f32):
+    """Rows whose sum passes 524 032 (eight times fp16's end), up to 128 times the end, beside ordinary ones; a scale that keeps scores small."""
+    lens, new, kv, heads, page, scale = [300], [tokens], 1, 4, 16, 1e-5
+    rng, pool, table, cache, batch = make(ops, 16, lens, new, kv, page)
+    q = rng.standard_normal((tokens, heads, 128))
+    q[:, 1] = 4500 + 100 * q[:, 1]
+    q[:, 2] = -30000 + 9000 * q[:, 2]
+    q[0, 3], q[1, 3] = 65504, -65504
+    q[2, 3, :64] = 60000                                  # and tiny elements beside large ones
+    q = np.clip(q, -65504, 65504).astype(BF)
+    got, lse = attend(ops, cache, batch, util.to_dev(q), heads, f32, scale)
+    check_attention(got, lse, ref.attention(pool, table, lens, new, q, scale, not few_rows(batch, heads, cache, f32)), tokens, f32)
+
+
 # ---- weights and eviction ----------------------------------------------------------------------------------------------
 
 
