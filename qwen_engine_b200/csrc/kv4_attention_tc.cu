@@ -498,8 +498,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
                 s_mask[j & 3][1][warp & 3] = bad;
             }
             {
-                // 8 * scale has to be finite: rows that span more than 122 820 lose up to 6 % of that
-                const __half2 s = __hmin2_nan(__half2half2(__ushort_as_half(static_cast<unsigned short>(kp))), __float2half2_rn(8188.0f));
+                const __half2 s = __half2half2(__ushort_as_half(static_cast<unsigned short>(kp)));
                 const uint32_t zero = __byte_perm(kp, kp, 0x3232);
                 *reinterpret_cast<uint4*>(smem + kSmemKx + t * 32 + 16 * part) = make_uint4(zero, zero, zero, zero);
 #pragma unroll
@@ -511,7 +510,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
                         kv4_centred_codes(words[e], o);         // pairs (0, 2), (4, 6), (1, 3), (5, 7)
 #pragma unroll
                         for (int n = 0; n < 4; ++n) {
-                            const __half2 h = __hmul2(as_half2(o[n]), s), l = __hfma2(as_half2(o[n]), s, __hneg2(h));
+                            // in a row that spans more than 15 * 8188 the product of the lowest code is below fp16's end: it is cut there, and
+                            // what is left, a multiple of 32 below 4400, is a second part like any other
+                            const __half2 h = __hmax2_nan(__hmul2(as_half2(o[n]), s), __float2half2_rn(-65504.0f)), l = __hfma2(as_half2(o[n]), s, __hneg2(h));
                             hi[n] = *reinterpret_cast<const uint32_t*>(&h);
                             lo[n] = *reinterpret_cast<const uint32_t*>(&l);
                         }

@@ -295,6 +295,22 @@ def test_attention_of_queries_as_large_as_fp16_goes(ops, tokens, f32):
     check_attention(got, lse, ref.attention(pool, table, lens, new, q, scale, not few_rows(batch, heads, cache, f32)), tokens, f32)
 
 
+@pytest.mark.parametrize("tokens,f32", [(100, False), (3, False), (3, True)])
+def test_attention_over_keys_that_span_the_whole_of_fp16(ops, tokens, f32):
+    """Key scales around 8188, eight times which is fp16's end, up to 8736; a softmax scale that keeps scores small."""
+    lens, new, kv, heads, page, scale = [300], [tokens], 1, 4, 16, 1e-6
+    rng, pool, table, cache, batch = make(ops, 17, lens, new, kv, page)
+    for j in range(300):
+        x = rng.uniform(-1, 1, 128) * [65504, 61440, 3.0][j % 3]
+        x[:2] = np.abs(x).max() * np.array([1, -1])
+        x[2] = rng.uniform(-65504, 65504) if j % 7 == 0 else x[2]
+        pool.put(table[0, j // page], 0, j % page, 0, *ref.quantise(x.astype(BF)))
+    cache.pages.copy_(util.to_dev(pool.words))
+    q = rng.standard_normal((tokens, heads, 128)).astype(BF)
+    got, lse = attend(ops, cache, batch, util.to_dev(q), heads, f32, scale)
+    check_attention(got, lse, ref.attention(pool, table, lens, new, q, scale, not few_rows(batch, heads, cache, f32)), tokens, f32)
+
+
 # ---- weights and eviction ----------------------------------------------------------------------------------------------
 
 
