@@ -491,7 +491,9 @@ W4A16_API int w4a16_kv4_read(const w4a16_kv4_cache* cache, const w4a16_kv4_batch
  * flight uses, two replayed graphs that may run at the same time included (nothing is kept in it between calls).  out must
  * not overlap q.
  * Two forms: fp16 results of at least 64 query rows a sequence and head (tokens x shared heads, on average) run on tcgen05 with
- * values and weights rounded to fp16; all others keep the values exact, and 32-bit results the weights too.  Keys never are.
+ * values and weights rounded to fp16, so that weights below 2^-24 of a row's largest are lost.  All others keep the values exact;
+ * a weight has 22 bits there for 32-bit results and 11 for fp16 ones, and is off by no less than 2^-31 of what the
+ * largest weight times value scale comes to.  Keys are never rounded.
  */
 W4A16_API int64_t w4a16_attention_kv4_workspace_bytes(int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads);
 W4A16_API int w4a16_attention_kv4(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, const void* q, void* out,

@@ -11,7 +11,10 @@
 //   out^T [128 x 8] += codes^T [128 x 16] . (p * value scale)^T: for a 32-bit result the weight enters as two fp16 numbers
 //       whose sum has 22 bits, for an fp16 result as one (2^-12 of a weight is less than the result's own rounding, and
 //       the weights' roundings average out); zeros enter as one 32-bit sum a query.
-//   running maximum: renewed only where a score exceeds it by 2^8, which a vote finds; p <= 2^8 fits.
+//   reference of the exponents: not the largest score but the largest log2(p * value scale), so that what fp16 holds best is what counts most
+//       in the result, whatever the value scales are (rows that get most of the attention often have the smallest values).  Renewed
+//       where an fp16 weight could pass 2^15, which a vote finds, and set so that the largest is 2^6: a weight is off by 2^-31 of the
+//       largest at most, or by 2^-22 of itself.  p itself is a 32-bit number that may be as large as 2^15 over the scale.
 #include "kv4.cuh"
 #include "kv4_attention.hpp"
 #include "kv4_work.cuh"
@@ -197,8 +200,6 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
     float o[NT][8][4] = {}, m[NT][2], l[NT][2] = {}, zacc[NT][2] = {};
 #pragma unroll
     for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY;
-    float pw = 0.0f;                                        // power of two on the value scales; 0: not chosen yet
-
     float mu[NT][2];                                        // m, or 0 where nothing has been seen
     for (int n = 0; n < NT; ++n) mu[n][0] = mu[n][1] = 0.0f;
     const int pos = key_position(g);                        // positions of rows g and g + 8 of A: pos and pos + 8
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
                 mma_16816(s[n], a1, b.z, b.w);
             }
         }
-        float ks[2], kz[2], vs[2], vz[2];
+        float ks[2], kz[2], vs[2], vz[2], lv[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             ks[i] = kv4_scale(r.kp[i]);
@@ -237,6 +238,9 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
             ks[i] *= to_log2;
             vs[i] = kv4_scale(r.vp[i]);
             vz[i] = fmaf(-0.5f, vs[i], kv4_zero(r.vp[i]));  // codes are taken around 7.5
+            // log2 of the scale less 15: exponent and seven bits of the mantissa as a number, at most 0.1 too small.  A scale of zero, or a
+            // NaN, counts as 2^-60.
+            lv[i] = fmaf(__uint_as_float(__byte_perm(__float_as_uint(fmaxf(vs[i], 0x1p-60f)), 0x4B000000u, 0x7632)), 0.0078125f, -(65536.0f + 127.0f + 15.0f));
         }
         bool above = false;
 #pragma unroll
@@ -256,22 +260,13 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) above = above || fmaxf(s[n][e], s[n][e + 2]) > m[n][e] + 8.0f;
-        if (__any_sync(0xFFFFFFFFu, above || pw == 0.0f || fmaxf(vs[0], vs[1]) * pw > 64.0f)) {
-            float big = fmaxf(vs[0], vs[1]);
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, d));
-            float ratio = 1.0f;
-            if (pw == 0.0f || big * pw > 64.0f) {           // the largest value scale times pw into [8, 16)
-                const float fresh = big > 0.0f ? __uint_as_float((130u + 127u - (__float_as_uint(big) >> 23)) << 23) : 1.0f;
-                ratio = pw == 0.0f ? 1.0f : fresh / pw;
-                pw = fresh;
-            }
+            for (int e = 0; e < 2; ++e) above = above || fmaxf(s[n][e] + lv[0], s[n][e + 2] + lv[1]) > m[n][e];
+        if (__any_sync(0xFFFFFFFFu, above)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float x = fmaxf(s[n][e], s[n][e + 2]);
+                    float x = fmaxf(s[n][e] + lv[0], s[n][e + 2] + lv[1]) + (15.0f - 6.0f);
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
                     const float fresh = fmaxf(m[n][e], x);
@@ -282,13 +277,11 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
                     zacc[n][e] *= f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        o[n][i][e] *= f * ratio;
-                        o[n][i][e + 2] *= f * ratio;
+                        o[n][i][e] *= f;
+                        o[n][i][e + 2] *= f;
                     }
                 }
         }
-        vs[0] *= pw;
-        vs[1] *= pw;
         uint32_t ph[NT][2];
         [[maybe_unused]] uint32_t pl[NT][2];                      // p * value scale in one or two fp16 parts, columns = positions
 #pragma unroll
@@ -366,7 +359,6 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
     __syncwarp();
 
     // the warps' parts into shared memory: a lane has dimensions 16 g .. 16 g + 15 of queries 2 t and 2 t + 1
-    const float undo = pw == 0.0f ? 1.0f : 1.0f / pw;
     constexpr int kElement[8] = {0, 4, 1, 5, 2, 6, 3, 7};
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -382,8 +374,8 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
             if (g == 0) s_ml[warp][r] = make_float2(m[n][e], ls);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                s_o(warp, r, 16 * g + kElement[i]) = fmaf(o[n][i][e], undo * kv4_value_undo(i), zs);
-                s_o(warp, r, 16 * g + 8 + kElement[i]) = fmaf(o[n][i][e + 2], undo * kv4_value_undo(i), zs);
+                s_o(warp, r, 16 * g + kElement[i]) = fmaf(o[n][i][e], kv4_value_undo(i), zs);
+                s_o(warp, r, 16 * g + 8 + kElement[i]) = fmaf(o[n][i][e + 2], kv4_value_undo(i), zs);
             }
         }
     __syncthreads();

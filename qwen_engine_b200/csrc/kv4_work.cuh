@@ -130,6 +130,12 @@ __device__ __forceinline__ void add_part(float4& x, float& sum, const float4& p,
     x.z = fmaf(p.z, f, x.z);
     x.w = fmaf(p.w, f, x.w);
 }
+// top + log2(sum).  The sum may be far from 1, and its exponent goes to top first, where the two cancel.
+__device__ __forceinline__ float log2_of_sum(float top, float sum) {
+    const uint32_t bits = __float_as_uint(sum);
+    const int e = static_cast<int>(bits >> 23) - 127;        // 128: an infinity or a NaN
+    return e == 128 ? top + sum : (top + static_cast<float>(e)) + log2f(__uint_as_float((bits & 0x007FFFFFu) | 0x3F800000u));
+}
 // A finished row: a warp, four dimensions a lane.
 template <bool F32>
 __device__ __forceinline__ void store_row(void* out, float* lse, size_t row, const float4& x, float top, float sum) {
@@ -142,7 +148,7 @@ __device__ __forceinline__ void store_row(void* out, float* lse, size_t row, con
         const uint2 h = make_uint2(pack_half2(y.x, y.y), pack_half2(y.z, y.w));
         reinterpret_cast<uint2*>(static_cast<__half*>(out) + row * kKvDim)[lane] = h;
     }
-    if (lane == 0 && lse != nullptr) lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+    if (lane == 0 && lse != nullptr) lse[row] = sum == 0.0f ? -INFINITY : log2_of_sum(top, sum) * kLn2;
 }
 
 }  // namespace

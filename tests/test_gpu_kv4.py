@@ -311,6 +311,53 @@ def test_attention_over_keys_that_span_the_whole_of_fp16(ops, tokens, f32):
     check_attention(got, lse, ref.attention(pool, table, lens, new, q, scale, not few_rows(batch, heads, cache, f32)), tokens, f32)
 
 
+@pytest.mark.parametrize("f32", [True, False])
+@pytest.mark.parametrize("tokens,heads", [(2, 4), (3, 4)])
+@pytest.mark.parametrize("gap", [2, 16, 20, 24, 40])
+@pytest.mark.parametrize("first", ["zero", "tiny", "large", "behind"])
+def test_attention_keeps_what_counts_in_the_result(ops, first, gap, tokens, heads, f32):
+    """A first position ahead by `gap` in the score (for one head as far behind) with values of none, of 1e-4 or of 1e4 of the size of the
+    others', or a few early ones as far behind with values 1e6 as large; and a last one, seen by the last token alone, with such values:
+    results are off relative to what the weights and values that make them up come to, not to the largest weight or value of the cache.
+
+    Queries have one element, so a score is one product: exact but for the scaling, the zero's part and their sum, 2^-24 each of their
+    sizes, and the exponent's argument, 2^-24 of it (the scores' range and up to 55 for the value scales'): d.  A weight is off by 2 d, so is their sum; the exponential adds 2^-22, two
+    fp16 parts 2^-21 (one: 2^-11), 32-bit sums of a row's L terms in groups of 16, truncated, L 2^-27, and the parts' joins 8 roundings."""
+    lens, new, kv, page = [700], [tokens], 1, 16
+    rng, pool, table, cache, batch = make(ops, 18, lens, new, kv, page)
+    size = {"zero": 0.0, "tiny": 1e-4, "large": 1e4, "behind": 0.01}[first]
+    others, behind = 0.01 if first == "behind" else 1.0, (3, 19, 35, 51) if first == "behind" else ()
+    for j in range(700):
+        k = 0.2 * rng.standard_normal(128) * (10 if behind else 1)       # there a few positions get most of the rest
+        k[0] = -8.0 if j in behind else 8.0 if j == 0 and not behind else k[0]
+        v = rng.standard_normal(128) * (size if j == 0 else 1e4 if j == 699 or j in behind else others) + (others / 2 if j % 50 == 1 else 0.0)
+        if j % 97 == 5:
+            v[:] = 0.25                                  # a scale of zero
+        for part, x in enumerate((k, v)):
+            pool.put(table[0, j // page], 0, j % page, part, *ref.quantise(x.astype(BF)))
+    cache.pages.copy_(util.to_dev(pool.words))
+    q = np.zeros((tokens, heads, 128), BF)
+    q[:, :, 0] = gap / 8 / SCALE * np.array([1, 0.9, -1, 0.8])
+    got, lse = attend(ops, cache, batch, util.to_dev(q), heads, f32)
+    k, v = (pool.rows(table[0], 0, 700, part)[0] for part in range(2))
+    params = [np.concatenate([pool.words[p, 0, (32 + part) * page:(33 + part) * page] for p in table[0]])[:700] for part in range(2)]
+    scale, zero = zip(*[((p & 0xFFFF).astype(np.uint16).view(BF).astype(np.float64), (p >> 16).astype(np.uint16).view(BF).astype(np.float64)) for p in params])
+    for i in range(tokens):
+        n = 700 - tokens + i + 1
+        for h in range(heads):
+            x = float(q[i, h, 0])
+            s = k[:n, 0] * x * SCALE
+            p = np.exp(s - s.max())
+            d = 3 * 2.0 ** -24 * (8 * scale[0][:n] + np.abs(zero[0][:n])).max() * abs(x) * SCALE + ((s.max() - s.min()) * 1.45 + 55 + 2 * np.abs(s).max()) * 2.0 ** -24
+            made_of = p @ (7.5 * scale[1][:n] + np.abs(zero[1][:n] - scale[1][:n] / 2)) / p.sum()
+            want = p @ v[:n] / p.sum()
+            room = made_of * (4 * d + 2.0 ** -22 + (2.0 ** -21 if f32 else 2.0 ** -11) + n * 2.0 ** -27 + 8 * 2.0 ** -24)
+            room = room + (0 if f32 else np.abs(want) * 2.0 ** -11 + 2.0 ** -25)
+            assert np.all(np.abs(got[i, h] - want) <= room), (i, h, np.abs(got[i, h] - want).max() / np.max(room))
+            wl = s.max() + np.log(p.sum())
+            assert abs(lse[i, h] - wl) <= 2 * d + 2.0 ** -21 + 2.0 ** -22 * abs(wl), (i, h, lse[i, h] - wl)
+
+
 # ---- weights and eviction ----------------------------------------------------------------------------------------------
 
 
