@@ -66,7 +66,7 @@ int ensure_device_ready(const DeviceInfo** out) {
             if (int st = gemv_set_attributes()) return st;
             if (int st = gemm_set_attributes()) return st;
             if (int st = kv4_set_attributes()) return st;
-            if (int st = kv4_chunk_set_attributes()) return st;
+            if ((info.chunk_status = kv4_chunk_set_attributes()) != 0) cudaGetLastError();
             info.ready = true;
             g_dev[dev] = info;
             g_dev_ready[dev].store(true, std::memory_order_release);
@@ -724,8 +724,10 @@ int w4a16_attention_kv4(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* bat
     if (misaligned(q, 16) || misaligned(out, 16) || misaligned(lse, 4) || misaligned(workspace, 16)) return W4A16_ERR_ALIGNMENT;
     const int64_t need = w4a16_attention_kv4_workspace_bytes(c.num_tokens, c.num_seqs, num_q_heads, c.kv_heads);
     if (need > 0 && (!workspace || workspace_bytes < need)) return W4A16_ERR_INVALID_ARG;
-    if (int st = ensure_device_ready(nullptr)) return st;
+    const DeviceInfo* device = nullptr;
+    if (int st = ensure_device_ready(&device)) return st;
     if (kv4_takes_chunk(c.num_tokens, c.num_seqs, num_q_heads, c.kv_heads, out_fp32 != 0)) {
+        if (device->chunk_status) return device->chunk_status;
         Kv4ChunkArgs a{};
         a.c = c; a.q = H(q); a.out = H(out); a.lse = lse; a.scale = softmax_scale; a.group = num_q_heads / c.kv_heads; a.q_stride = q_stride;
         return kv4_chunk_attention(a, num_q_heads, workspace, S(stream));

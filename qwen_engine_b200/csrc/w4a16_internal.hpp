@@ -18,6 +18,7 @@ namespace w4 {
 struct DeviceInfo {
     int sm_count = 0;
     int cc_major = 0;
+    int chunk_status = 0;     // of the chunk form's set-up (kv4_attention_tc.cu): calls that take it return it, others run
     bool ready = false;
 };
 int ensure_device_ready(const DeviceInfo** out);  // lazy per-device set-up; returns a status

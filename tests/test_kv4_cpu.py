@@ -257,3 +257,59 @@ def test_the_evictions_search_finds_the_key_of_a_rank(lib, tmp_path):
     for (k, need), line in zip(sets, out):
         key, left, above, rounds = map(int, line.split())
         assert key == np.sort(k)[::-1][need - 1] and above == (k > key).sum() and above + left == need and rounds <= 4
+
+
+FAKES = r"""
+// The entry points (c_abi.cu) over launchers and a device that are none: what they return where one kernel cannot run.
+#include <cstdio>
+#include <cstring>
+#include "kv4_attention.hpp"
+#include "w4a16_internal.hpp"
+namespace w4 {
+int quantize_set_attributes() { return 0; }
+int gemv_set_attributes() { return 0; }
+int gemm_set_attributes() { return 0; }
+int kv4_set_attributes() { return 0; }
+int kv4_chunk_set_attributes() { return 200; }
+int kv4_read(const Kv4View&, __half*, __half*, cudaStream_t) { return 0; }
+int kv4_attention(Kv4AttentionArgs, int, bool, void*, cudaStream_t) { return 0; }
+int kv4_chunk_attention(Kv4ChunkArgs, int, void*, cudaStream_t) { return 0; }
+Kv4AttentionPlan kv4_attention_plan(int, int, int, int) { return {1, 1, 1, 16, 32}; }
+Kv4ChunkPlan kv4_chunk_plan(int, int, int, int) { return {1, 1, 16, 32}; }
+}
+int main() {
+    alignas(16) static char m[64];
+    const w4a16_kv4_cache c{m, nullptr, 8, 1, 16};
+    const w4a16_kv4_batch b{reinterpret_cast<int32_t*>(m), reinterpret_cast<int32_t*>(m), reinterpret_cast<int32_t*>(m), 1, 8, 100};
+    for (int turn = 0; turn < 2; ++turn)
+        std::printf("%d %d %d ", w4a16_kv4_read(&c, &b, m, m, nullptr), w4a16_attention_kv4(&c, &b, m, m, nullptr, m, 1, 64, 1, 0.1f, 0, nullptr),
+                    w4a16_attention_kv4(&c, &b, m, m, nullptr, m, 1, 64, 0, 0.1f, 0, nullptr));
+}
+"""
+
+RUNTIME = r"""
+extern "C" {
+int cudaGetDevice(int* d) { *d = 0; return 0; }
+int cudaDeviceGetAttribute(int* v, int a, int) { *v = a == 75 ? 10 : 148; return 0; }      // 75: compute capability, major
+int cudaGetLastError() { return 0; }
+void** __cudaRegisterFatBinary(void*) { static void* p; return &p; }
+void __cudaRegisterFatBinaryEnd(void**) {}
+void __cudaUnregisterFatBinary(void**) {}
+}
+"""
+
+
+def test_a_kernel_that_cannot_run_takes_no_other_call_with_it(tmp_path):
+    """The chunk form's kernel wants a register count of its compiler.  Where it does not have it, calls that take it fail, no others."""
+    import pathlib
+    import subprocess
+
+    from qwen_engine_b200 import build
+    csrc = pathlib.Path(__file__).parents[1] / "qwen_engine_b200" / "csrc"
+    (tmp_path / "fakes.cu").write_text(FAKES)
+    (tmp_path / "runtime.cpp").write_text(RUNTIME)
+    subprocess.run([build.nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++20", "-O1", "--expt-relaxed-constexpr", f"-I{csrc}", "-cudart", "none",
+                    "-Xcompiler", "-fno-pie", "-Xlinker", "-no-pie,-z,lazy,--unresolved-symbols=ignore-all", "-o", str(tmp_path / "calls"),
+                    str(csrc / "c_abi.cu"), str(tmp_path / "fakes.cu"), str(tmp_path / "runtime.cpp")], check=True)
+    out = subprocess.run([str(tmp_path / "calls")], capture_output=True, text=True, check=True, timeout=60).stdout
+    assert out.split() == ["0", "0", "200"] * 2
