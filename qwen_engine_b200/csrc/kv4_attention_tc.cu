@@ -145,9 +145,9 @@ __device__ __forceinline__ void tmem_take32(float (&r)[32]) {
 // and conversion three behind.  (As loops that the compiler orders a row took 2200 cycles alone on its scheduler.)  The wait for
 // tensor-memory loads is one for all that are in flight, so 32 columns are asked for behind the wait for the 32 before them and
 // have all of their exponentials' time; asked for in eighths, later, each wait stalled (2200 cycles again, 1300 without loads).
-// SIMPLE: the row sees every position; else `sees` and, of those, `bad` (weight NaN).
+// SIMPLE: the row sees every position; else those of `sees`.
 template <bool SIMPLE>
-__device__ __forceinline__ float softmax_pass(uint32_t t_s, float2 scale2, float2 mu2, const uint32_t (&sees)[4], const uint32_t (&bad)[4], uint32_t (&p)[64], float* total) {
+__device__ __forceinline__ float softmax_pass(uint32_t t_s, float2 scale2, float2 mu2, const uint32_t (&sees)[4], uint32_t (&p)[64], float* total) {
     float s[2][32];
     float2 sum[2] = {};
     float top[2] = {-INFINITY, -INFINITY};
@@ -162,10 +162,6 @@ __device__ __forceinline__ float softmax_pass(uint32_t t_s, float2 scale2, float
     };
     auto finish = [&](int c, int k) {
         float &x = s[c & 1][2 * k], &y = s[c & 1][2 * k + 1];
-        if (!SIMPLE) {
-            if (bad[c] >> (2 * k) & 1u) x = __int_as_float(0x7FC00000);
-            if (bad[c] >> (2 * k) & 2u) y = __int_as_float(0x7FC00000);
-        }
         add2(sum[k & 1], x, y);
         p[16 * c + k] = pack_here(x, y);
     };
@@ -359,18 +355,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
             if (!ok) break;
             tc_fence_after();
             const int base = k0 + j * kChunkKeys;
-            uint32_t sees[4], bad[4];
-            bool simple;
+            uint32_t sees[4];
+            bool simple, poisoned;
             {
                 const uint4 there = *reinterpret_cast<const uint4*>(s_mask[j & 3][0]), poison = *reinterpret_cast<const uint4*>(s_mask[j & 3][1]);
                 const uint32_t all = there.x & there.y & there.z & there.w, any = poison.x | poison.y | poison.z | poison.w;
-                simple = __all_sync(0xFFFFFFFFu, base + kChunkKeys <= limit && all == ~0u && any == 0);
-                const uint32_t th[4] = {there.x, there.y, there.z, there.w}, po[4] = {poison.x, poison.y, poison.z, poison.w};
+                simple = __all_sync(0xFFFFFFFFu, base + kChunkKeys <= limit && all == ~0u);
+                poisoned = any != 0;
+                const uint32_t th[4] = {there.x, there.y, there.z, there.w};
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int n = limit - base - 32 * q;
                     sees[q] = th[q] & (n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u);
-                    bad[q] = sees[q] & po[q];
                 }
             }
             uint32_t p[64];
@@ -398,12 +394,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
                 }
                 const float mu = m == -INFINITY ? 0.0f : m;
                 const float2 scale2 = make_float2(to_log2, to_log2), mu2 = make_float2(-mu, -mu);
-                const float top = simple ? softmax_pass<true>(t_s, scale2, mu2, sees, bad, p, &sum) : softmax_pass<false>(t_s, scale2, mu2, sees, bad, p, &sum);
+                const float top = simple ? softmax_pass<true>(t_s, scale2, mu2, sees, p, &sum) : softmax_pass<false>(t_s, scale2, mu2, sees, p, &sum);
                 // too large for fp16, or the row's first positions: again with the maximum known
                 const bool fresh = m == -INFINITY && top > -INFINITY, again = fresh || top > 15.0f;
                 if (fresh) m = top;
                 else if (top > 8.0f) grow = top;
                 if (!__any_sync(0xFFFFFFFFu, again)) break;
+            }
+            if (poisoned) {                 // behind the sum, which the values have no part in
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t bad = sees[q] & s_mask[j & 3][1][q];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) p[16 * q + k] |= (bad >> (2 * k) & 1u ? 0x00007E00u : 0u) | (bad >> (2 * k) & 2u ? 0x7E000000u : 0u);
+                }
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q) {

@@ -248,6 +248,24 @@ def test_a_poisoned_row_reaches_the_tokens_that_see_it_only(ops, heads, f32):
         cache.pages.copy_(clean)
 
 
+@pytest.mark.parametrize("heads,f32", [(4, True), (4, False), (40, False)])
+def test_a_poisoned_value_leaves_lse_and_weights_alone(ops, heads, f32):
+    """The logarithm of the sum and the attention weights come from queries and keys: a value row of NaNs reaches the outputs only."""
+    lens, new, kv, page = [300], [20], 1, 16
+    rng, pool, table, cache, batch = make(ops, 19, lens, new, kv, page)
+    q = rng.standard_normal((20, heads, 128)).astype(BF)
+    for at in (5, 285):
+        cache.pages[int(table[0, at // page]), 0, 33 * page + at % page] = 0x7E007E00
+    want = ref.attention(pool, table, lens, new, q, SCALE, not few_rows(batch, heads, cache, f32))
+    got, lse = attend(ops, cache, batch, util.to_dev(q), heads, f32)
+    assert np.isnan(got[:20]).all()
+    assert np.all(np.abs(lse[:20] - want[1]) <= want[3])
+    add, rel = ref.key_weights(pool, table, lens, new, q, lse[:20].astype(np.float64), SCALE)
+    ops.kv4_add_key_weights(cache, batch, util.to_dev(q), util.to_dev(lse[:20]), heads, SCALE)
+    total = pool.weight + add
+    assert np.all(np.abs(util.to_np(cache.key_weight) - total) <= add * rel + total * 2.0 ** -22)
+
+
 @pytest.mark.parametrize("factor", [1e-3, 1.0, 3e3])
 @pytest.mark.parametrize("tokens,f32", [(1, True), (1, False), (40, False)])
 def test_attention_of_values_of_any_size(ops, factor, tokens, f32):
