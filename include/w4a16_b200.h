@@ -469,7 +469,7 @@ W4A16_API int64_t w4a16_kv4_page_bytes(int page_size, int num_kv_heads);
  *   q_out = fp16(rot(q + q_bias)), cached key = Q4(fp16(rot(k + k_bias))), cached value = Q4(fp16(v + v_bias)),
  * sums and rotation in fp32.  rot turns the pairs (d, d + 64) by positions[token] * rope_inv_freq[d], the angle taken in
  * 64 bits.  q: fp16 [num_tokens] rows of num_q_heads * 128 (q_stride elements apart, 0: packed), q_out the same, may be q;
- * both may be NULL.  k, v: rows of num_kv_heads * 128, kv_stride apart.  Biases may be NULL; positions NULL: the cached
+ * both may be NULL, and num_q_heads and q_stride are not looked at then.  k, v: rows of num_kv_heads * 128, kv_stride apart.  Biases may be NULL; positions NULL: the cached
  * position; rope_inv_freq fp32 [64], NULL: no rotation.  New positions start with key_weight 0.  Tensors 16-byte aligned,
  * strides multiples of 8.  No two tokens of a call may share a cached position.
  */

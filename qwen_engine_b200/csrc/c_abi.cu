@@ -684,8 +684,9 @@ int w4a16_kv4_append(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch,
     Kv4View c;
     if (int st = kv4_view(cache, batch, &c)) return st;
     if (!k || !v || (q == nullptr) != (q_out == nullptr) || (q_bias && !q)) return W4A16_ERR_INVALID_ARG;
-    if (int st = kv4_heads(c, num_q_heads, &q_stride, num_q_heads)) return st;
-    if (int st = kv4_heads(c, num_q_heads, &kv_stride, c.kv_heads)) return st;
+    if (q)
+        if (int st = kv4_heads(c, num_q_heads, &q_stride, num_q_heads)) return st;
+    if (int st = kv4_heads(c, q ? num_q_heads : c.kv_heads, &kv_stride, c.kv_heads)) return st;
     if (misaligned(q, 16) || misaligned(k, 16) || misaligned(v, 16) || misaligned(q_out, 16) || misaligned(q_bias, 16) || misaligned(k_bias, 16) ||
         misaligned(v_bias, 16) || misaligned(positions, 4) || misaligned(rope_inv_freq, 4))
         return W4A16_ERR_ALIGNMENT;

@@ -168,6 +168,22 @@ def test_append_leaves_alone_what_it_may_not_touch(ops):
     assert (kr[4:12][[i for i in range(8) if 40 - 8 + i >= 32]] == 0).all() and (kr[12:14] == 0).all()
 
 
+@pytest.mark.parametrize("kv", [5, 8])
+def test_append_of_keys_and_values_alone(ops, kv):
+    """No queries, and numbers of heads that are no divisors of the default number of query heads."""
+    lens, new, page = [20, 33], [20, 2], 16
+    rng, pool, table, cache, batch = make(ops, 22, lens, new, kv, page)
+    k, v = (rng.standard_normal((22, kv, 128)).astype(BF) for _ in range(2))
+    for b, first, L, n in ref.spans(lens, new):
+        for i in range(n):
+            at = L - n + i
+            for h in range(kv):
+                for part, x in enumerate((k, v)):
+                    pool.put(table[b, at // page], h, at % page, part, *ref.quantise(x[first + i, h]))
+    ops.kv4_append(cache, batch, None, util.to_dev(k), util.to_dev(v), None, None, None, None, None, None)
+    assert np.array_equal(words_of(cache), pool.words)
+
+
 # ---- attention -----------------------------------------------------------------------------------------------------------
 
 

@@ -72,6 +72,16 @@ def test_refusals(lib, changes, status, where):
         assert all(s > 0 or s == -4 for n, s in got.items() if n not in where), got
 
 
+@pytest.mark.parametrize("heads", [0, 11, 12])
+@pytest.mark.parametrize("kv", [5, 8])
+def test_an_append_without_queries_asks_nothing_of_query_heads(lib, heads, kv):
+    """Keys and values alone: 5 or 8 heads of them are no divisors of the default number of query heads, 12."""
+    if torch.cuda.is_available():
+        pytest.skip("the addresses would be followed")
+    status = calls(lib, q=None, q_out=None, num_kv_heads=kv, heads=heads, q_stride=4)["append"]
+    assert status > 0 or status == -4          # as far as asking for a device
+
+
 def test_null_views_are_refused(lib):
     c, b = views()
     assert lib.w4a16_kv4_read(None, b, P, P, None) == -1 and lib.w4a16_kv4_read(c, None, P, P, None) == -1
