@@ -13,6 +13,15 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (run with -m gpu on a B200)")
 
 
+def pytest_collection_modifyitems(items):
+    """The refusals of the 4-bit cache go through every entry point, also those that a change does not concern, with addresses that are none:
+    where there is a device these would launch."""
+    from tests import util
+    for item in items:
+        if item.path.name == "test_kv4_cpu.py" and item.originalname == "test_refusals" and util.cuda_available():
+            item.add_marker(pytest.mark.skip(reason="the addresses would be followed"))
+
+
 def pytest_collection_finish(session):
     gc.collect()
     gc.freeze()     # what is loaded by now stays: the collections below look at the tests' own objects only
