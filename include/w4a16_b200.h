@@ -515,7 +515,8 @@ W4A16_API int w4a16_kv4_add_key_weights(const w4a16_kv4_cache* cache, const w4a1
  * the rest those with the largest key_weight (the earlier of equal ones; a NaN is the smallest).  What stays keeps its
  * order and is copied, rows and weights, to the pages of dst_block_table [num_seqs][dst_max_pages_per_seq]: pages of their own, none
  * twice and none of the sequences being cut; the old pages are left as they are, so pages shared with other sequences are
- * safe.  Sequences that fit are copied whole.  new_seq_lens [num_seqs] = min(length, budget), another array than seq_lens;
+ * safe.  A kept position on a page number outside the pool moves nothing but counts: its fresh slot keeps what the page held, and calls on
+ * the new pages see it, so cut only sequences whose pages are all there.  Sequences that fit are copied whole.  new_seq_lens [num_seqs] = min(length, budget), another array than seq_lens;
  * kept int32 [num_seqs][num_kv_heads][budget]: the old positions in order, -1 behind the last.  num_tokens and query_start
  * of the batch are not used.
  */
