@@ -311,7 +311,7 @@ __device__ __forceinline__ uint32_t ld_cluster(const void* mine, uint32_t rank) 
 }
 
 __global__ void __launch_bounds__(kEvictThreads, 1) kv4_evict_kernel(const __grid_constant__ EvictArgs a) {
-    extern __shared__ uint32_t s_keys[];                         // [kEvictCached]
+    extern __shared__ __align__(16) uint32_t s_keys[];           // [kEvictCached], written four at a time
     __shared__ uint32_t s_hist[kEvictBins], s_coarse[kEvictCoarse];
     __shared__ uint32_t s_warp[2][kEvictWarps];
     __shared__ uint32_t s_found[2], s_total[2];
