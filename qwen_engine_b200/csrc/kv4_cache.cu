@@ -38,8 +38,9 @@ __device__ __forceinline__ uint4 float_to_half8(const float (&x)[8]) {
 
 // A row of 128 fp16 values in a half-warp: lane hl has 4 hl .. 4 hl + 3 and the same + 64, so that both values of a rotated pair are its
 // own.  Returns the code word that the lane stores, number kv4_word_of(hl), and the row's (scale, zero).  Both halves of a warp call it.
-// The codes are those of the formula in IEEE arithmetic: a product with the reciprocal is off by less than 1e-5 (|quotient| < 11), so
-// only where one lands nearer than that to a border between two codes are the divisions made.  A row with an infinity or a NaN gets
+// The codes are those of the formula in IEEE arithmetic: zero lies in the row's range, which is 15 scales and a half more where the scale is
+// subnormal, so |quotient| < 23, and a product with the reciprocal is off by less than 5e-6 (three roundings); only where one lands
+// nearer than 2e-5 to a border between two codes are the divisions made.  A row with an infinity or a NaN gets
 // a NaN scale: it reads back as NaN instead of as finite values that it does not hold.
 __device__ __forceinline__ int kv4_word_of(int hl) { return (hl & 1) * 8 + (hl >> 1); }
 __device__ __forceinline__ uint32_t kv4_quantise_lane(const __half2 (&h)[4], int hl, uint32_t* params) {

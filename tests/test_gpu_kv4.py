@@ -168,6 +168,35 @@ def test_append_leaves_alone_what_it_may_not_touch(ops):
     assert (kr[4:12][[i for i in range(8) if 40 - 8 + i >= 32]] == 0).all() and (kr[12:14] == 0).all()
 
 
+def test_append_of_rows_with_few_steps_or_subnormal_scales(ops):
+    """Rows of one to forty steps of fp16 far from zero, where zero's rounding is up to 7.5 scales, and rows whose scale is subnormal and up to
+    half a step off: quotients go to 15 and beyond, and the codes are the formula's all the same."""
+    kv, page, T = 4, 16, 64
+    rng, pool, table, cache, batch = make(ops, 23, [T], [T], kv, page)
+    x = np.empty((2, T, kv, 128), BF)
+    for part in range(2):
+        for t in range(T):
+            for h in range(kv):
+                steps = int(rng.integers(1, 41))
+                if (t + h) % 2:
+                    base = int(rng.integers(0x0400, 0x7800))                 # bits of a normal number and of those above it
+                    x[part, t, h] = (base + rng.integers(0, steps + 1, 128)).astype(np.uint16).view(BF) * BF(rng.choice([-1, 1]))
+                else:                                                        # multiples of 2^-24
+                    x[part, t, h] = (rng.integers(-4 * steps, 4 * steps + 1, 128) * 2.0 ** -24 + rng.choice([0, 2.0 ** -14])).astype(BF)
+    x[0, 0, 0] = 1.0 + 2.0 ** -10 * (np.arange(128) % 2)
+    most = 0.0
+    for t in range(T):
+        for h in range(kv):
+            for part in range(2):
+                w, s, z = ref.quantise(x[part, t, h])
+                pool.put(table[0, t // page], h, t % page, part, w, s, z)
+                if s > 0:
+                    most = max(most, np.abs((x[part, t, h].astype(np.float64) - float(z)) / float(s)).max())
+    assert 14 < most < 23
+    ops.kv4_append(cache, batch, None, util.to_dev(x[0]), util.to_dev(x[1]), None, None, None, None, None, None)
+    assert np.array_equal(words_of(cache), pool.words)
+
+
 @pytest.mark.parametrize("kv", [5, 8])
 def test_append_of_keys_and_values_alone(ops, kv):
     """No queries, and numbers of heads that are no divisors of the default number of query heads."""
