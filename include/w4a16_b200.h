@@ -484,7 +484,7 @@ W4A16_API int w4a16_kv4_read(const w4a16_kv4_cache* cache, const w4a16_kv4_batch
 
 /*
  * out[token][head] = sum over the positions j that the token sees of softmax_j(softmax_scale * q . key_j) * value_j;
- * query heads share key/value heads in consecutive groups.  out: fp16, or fp32 with out_fp32 (what
+ * query heads share key/value heads in consecutive groups.  out: fp16 (cut at +-65504), or fp32 with out_fp32 (what
  * w4a16_gemv_attn_heads_f32_w4a16 takes), [num_tokens][num_q_heads][128]; lse (may be NULL): fp32
  * [num_tokens][num_q_heads], the logarithm of the sum of exp(softmax_scale * q . key_j).  A token that sees nothing
  * gives zeros and -infinity.  workspace: w4a16_attention_kv4_workspace_bytes() of device memory that no other call in

@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
                     for (int k = 0; k < 4; ++k) {
                         uint32_t y[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) y[e] = l == 0.0f ? 0u : pack_half2(x[8 * k + 2 * e] * f, x[8 * k + 2 * e + 1] * f);
+                        for (int e = 0; e < 4; ++e) y[e] = l == 0.0f ? 0u : pack_result(x[8 * k + 2 * e] * f, x[8 * k + 2 * e + 1] * f);
                         reinterpret_cast<uint4*>(out)[k] = make_uint4(y[0], y[1], y[2], y[3]);
                     }
                 } else {

@@ -110,6 +110,11 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+// Results: an average of finite values can step over fp16's end by the roundings of scales, zeros and weights; it is cut there.
+__device__ __forceinline__ uint32_t pack_result(float a, float b) {
+    const __half2 end = __float2half2_rn(65504.0f), h = __hmax2_nan(__hmin2_nan(__floats2half2_rn(a, b), end), __hneg2(end));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
 __device__ __forceinline__ float sum_half8(const uint4& w) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
     float s = 0.0f;
@@ -145,7 +150,7 @@ __device__ __forceinline__ void store_row(void* out, float* lse, size_t row, con
     if constexpr (F32) {
         reinterpret_cast<float4*>(static_cast<float*>(out) + row * kKvDim)[lane] = y;
     } else {
-        const uint2 h = make_uint2(pack_half2(y.x, y.y), pack_half2(y.z, y.w));
+        const uint2 h = make_uint2(pack_result(y.x, y.y), pack_result(y.z, y.w));
         reinterpret_cast<uint2*>(static_cast<__half*>(out) + row * kKvDim)[lane] = h;
     }
     if (lane == 0 && lse != nullptr) lse[row] = sum == 0.0f ? -INFINITY : log2_of_sum(top, sum) * kLn2;

@@ -293,6 +293,29 @@ def test_a_poisoned_row_reaches_the_tokens_that_see_it_only(ops, heads, f32):
         cache.pages.copy_(clean)
 
 
+@pytest.mark.parametrize("tokens,heads,f32", [(2, 2, False), (70, 2, False), (300, 4, False), (2, 2, True)])
+def test_attention_over_the_largest_values_is_finite(ops, tokens, heads, f32):
+    """Rows from -65504 to 65504 come back as -65504 to 65536 (scale 8736, zero 4384: -8 * 8736 + 4384, 7 * 8736 + 4384), which is no fp16
+    number: fp16 results end at 65504, as rows that are read do.
+
+    Every position has the same values, so the average is theirs: for 32 bits but for sums; for fp16 results but for weights and result, 2^-11
+    each; in the chunk form the value besides, and its scale and zero, which are 65504 / 65536 as large (2^-11) and cut to fp16 (2^-10)."""
+    kv, page, n = 1, 16, 300
+    rng, pool, table, cache, batch = make(ops, 24, [n], [tokens], kv, page)
+    x = np.where(np.arange(128) % 2, 65504, -65504).astype(BF)
+    for j in range(n):
+        pool.put(table[0, j // page], 0, j % page, 1, *ref.quantise(x))
+    assert np.abs(pool.rows(table[0], 0, n, 1)[0]).max() == 65536
+    cache.pages.copy_(util.to_dev(pool.words))
+    q = (3 * rng.standard_normal((tokens, heads, 128))).astype(BF)
+    got, _ = attend(ops, cache, batch, util.to_dev(q), heads, f32)
+    got = got[:tokens].astype(np.float64)
+    assert np.isfinite(got).all() and np.all(np.sign(got) == np.sign(x.astype(np.float64)))
+    v = pool.row(table[0, 0], 0, 0, 1)
+    room = 2.0 ** -18 if f32 else 2.0 ** -10 if few_rows(batch, heads, cache, f32) else 3 * 2.0 ** -11 + 2.0 ** -11 + 2.0 ** -10
+    assert np.all(np.abs(got - (v if f32 else np.clip(v, -65504, 65504))) <= 65504 * room)
+
+
 @pytest.mark.parametrize("heads,f32", [(4, True), (4, False), (40, False)])
 def test_a_poisoned_value_leaves_lse_and_weights_alone(ops, heads, f32):
     """The logarithm of the sum and the attention weights come from queries and keys: a value row of NaNs reaches the outputs only."""
