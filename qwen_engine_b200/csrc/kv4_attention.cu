@@ -197,11 +197,16 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
     const int all_see = q.past + q.row0 / a.group + 1;      // positions that every row of the tile sees
     __syncthreads();
 
-    float o[NT][8][4] = {}, m[NT][2], l[NT][2] = {}, zacc[NT][2] = {};
+    // m: reference of the exponents, renewed where a weight's logarithm is above `above` (m, or -infinity: by every step)
+    constexpr float kNothingSeen = -3e38f;                  // finite: -infinity less it is -infinity
+    float o[NT][8][4] = {}, m[NT][2], above[NT][2], l[NT][2] = {}, zacc[NT][2] = {};
 #pragma unroll
-    for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY;
-    float mu[NT][2];                                        // m, or 0 where nothing has been seen
-    for (int n = 0; n < NT; ++n) mu[n][0] = mu[n][1] = 0.0f;
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            m[n][e] = kNothingSeen;
+            above[n][e] = -INFINITY;
+        }
     const int pos = key_position(g);                        // positions of rows g and g + 8 of A: pos and pos + 8
     const int value_from = kStageValues + 64 * t + ((8 * g) ^ (16 * (t & 2)));
     // CUT: some row does not see some of these positions
@@ -242,7 +247,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
             // NaN, counts as 2^-60.
             lv[i] = fmaf(__uint_as_float(__byte_perm(__float_as_uint(fmaxf(vs[i], 0x1p-60f)), 0x4B000000u, 0x7632)), 0.0078125f, -(65536.0f + 127.0f + 15.0f));
         }
-        bool above = false;
+        bool renew = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -260,19 +265,23 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) above = above || fmaxf(s[n][e] + lv[0], s[n][e + 2] + lv[1]) > m[n][e];
-        if (__any_sync(0xFFFFFFFFu, above)) {
+            for (int e = 0; e < 2; ++e) renew = renew || fmaxf(s[n][e] + lv[0], s[n][e + 2] + lv[1]) > above[n][e];
+        if (__any_sync(0xFFFFFFFFu, renew)) {
+            // From 2^23 on a score's neighbours are 1 and more away, and what is added to one is lost or rounded up: there the reference is the
+            // largest score itself, at every step, so that a weight is the scale at most.
+            constexpr float kFar = 8388608.0f;
+            auto reference = [&](float score, float l) { return fabsf(score) < kFar ? score + (l + (15.0f - 6.0f)) : score; };
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float x = fmaxf(s[n][e] + lv[0], s[n][e + 2] + lv[1]) + (15.0f - 6.0f);
+                    float x = fmaxf(reference(s[n][e], lv[0]), reference(s[n][e + 2], lv[1]));
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
                     const float fresh = fmaxf(m[n][e], x);
                     const float f = fresh == m[n][e] ? 1.0f : ex2(m[n][e] - fresh);
                     m[n][e] = fresh;
-                    mu[n][e] = fresh == -INFINITY ? 0.0f : fresh;
+                    above[n][e] = fabsf(fresh) < kFar ? fresh : -INFINITY;
                     l[n][e] *= f;
                     zacc[n][e] *= f;
 #pragma unroll
@@ -289,7 +298,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
             float x[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float p = ex2(s[n][e] - mu[n][e & 1]);
+                const float p = ex2(s[n][e] - m[n][e & 1]);
                 l[n][e & 1] += p;
                 x[e] = p * vs[e >> 1];
                 float z = p * vz[e >> 1];
@@ -371,7 +380,7 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : 2) kv4_attention_k
                 zs += __shfl_xor_sync(0xFFFFFFFFu, zs, d);
             }
             const int r = n * 8 + 2 * t + e;
-            if (g == 0) s_ml[warp][r] = make_float2(m[n][e], ls);
+            if (g == 0) s_ml[warp][r] = make_float2(m[n][e] == kNothingSeen ? -INFINITY : m[n][e], ls);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 s_o(warp, r, 16 * g + kElement[i]) = fmaf(o[n][i][e], kv4_value_undo(i), zs);

@@ -316,6 +316,48 @@ def test_attention_over_the_largest_values_is_finite(ops, tokens, heads, f32):
     assert np.all(np.abs(got - (v if f32 else np.clip(v, -65504, 65504))) <= 65504 * room)
 
 
+@pytest.mark.parametrize("tokens,f32", [(2, True), (9, True), (2, False)])
+@pytest.mark.parametrize("high", [10.2, 20.4, 22.7, 23.3, 23.8, 24.6, 25.3, 26.5, 27.4, 28.3, 28.9, 30.6, 33.1])
+def test_attention_with_scores_that_are_far_above_what_32_bits_count_in(ops, high, tokens, f32):
+    """Scores of about 2^high in the exponent's base: from 2^24 on neighbouring 32-bit numbers are more than 1 apart, so the reference of the exponents
+    cannot be chosen freely.  A few positions share the largest score bit for bit (their key rows are the same), with values of every
+    size, and all others are far below: the result is the average of those.
+
+    It is off by the weights' and values' roundings alone, relative to what makes it up: two fp16 parts 2^-21, with the sums 2^-18; one 2^-11, and
+    the value's 2^-11 in the chunk form.  lse: a score's sum, scaling and logarithm, at most 2^-21 of it."""
+    n, kv, heads, page = 300, 1, 2, 16
+    rng, pool, table, cache, batch = make(ops, 25, [n], [tokens], kv, page)
+    c, first = 60000.0, {0: [3, 17, 66, 140, 190], 1: [1, 40, 64, 65, 199]}
+    scale = 2.0 ** high * math.log(2) / (c * 50000.0)
+    top = rng.uniform(-0.9, 0.9, 128) * c
+    size = [1.0, 1e-3, 0.0, 30.0, 3e3]
+    for j in range(n):
+        k = rng.uniform(-0.8, 0.8, 128) * c
+        v = rng.standard_normal(128)
+        for h in range(2):
+            if j in first[h]:
+                k = np.concatenate([[c * (1, -1)[h]], top[1:]])
+                v = v * size[first[h].index(j)] + 0.125
+        for part, x in enumerate((k, v)):
+            pool.put(table[0, j // page], 0, j % page, part, *ref.quantise(x.astype(BF)))
+    cache.pages.copy_(util.to_dev(pool.words))
+    q = np.zeros((tokens, heads, 128), BF)
+    q[:, 0, 0], q[:, 1, 0] = 50000, -50000
+    got, lse = attend(ops, cache, batch, util.to_dev(q), heads, f32, scale)
+    k, v = (pool.rows(table[0], 0, n, part)[0] for part in range(2))
+    p = np.concatenate([pool.words[x, 0, 33 * page:34 * page] for x in table[0]])[:n]
+    vs, vz = ((p & 0xFFFF).astype(np.uint16).view(BF).astype(np.float64), (p >> 16).astype(np.uint16).view(BF).astype(np.float64))
+    few = few_rows(batch, heads, cache, f32)
+    for h in range(2):
+        D = first[h]
+        want, made_of = v[D].mean(0), (7.5 * vs + np.abs(vz - vs / 2))[D].mean()
+        room = made_of * (2.0 ** -18 if f32 else 2.0 ** -11 if few else 2.0 ** -10) + (0 if f32 else np.abs(want) * 2.0 ** -11 + 2.0 ** -25)
+        for i in range(tokens):
+            assert np.all(np.abs(got[i, h] - want) <= room), (i, h, np.abs(got[i, h] - want).max() / np.max(room))
+            wl = k[D[0], 0] * float(q[i, h, 0]) * scale + math.log(len(D))
+            assert abs(lse[i, h] - wl) <= 2.0 ** -21 * abs(wl), (i, h, lse[i, h] / wl - 1)
+
+
 @pytest.mark.parametrize("heads,f32", [(4, True), (4, False), (40, False)])
 def test_a_poisoned_value_leaves_lse_and_weights_alone(ops, heads, f32):
     """The logarithm of the sum and the attention weights come from queries and keys: a value row of NaNs reaches the outputs only."""
