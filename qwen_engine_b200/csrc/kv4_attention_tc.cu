@@ -121,6 +121,10 @@ __device__ __forceinline__ void fma2(float& x, float& y, float2 b, float2 c) {
     asm volatile("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tmov.b64 c, {%4, %5};\n\tfma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
                  : "+f"(x), "+f"(y) : "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
 }
+__device__ __forceinline__ void add_to2(float& x, float& y, float2 b) {
+    asm volatile("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+                 : "+f"(x), "+f"(y) : "f"(b.x), "f"(b.y));
+}
 __device__ __forceinline__ void add2(float2& s, float x, float y) {
     asm volatile("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
                  : "+f"(s.x), "+f"(s.y) : "f"(x), "f"(y));
@@ -145,9 +149,9 @@ __device__ __forceinline__ void tmem_take32(float (&r)[32]) {
 // and conversion three behind.  (As loops that the compiler orders a row took 2200 cycles alone on its scheduler.)  The wait for
 // tensor-memory loads is one for all that are in flight, so 32 columns are asked for behind the wait for the 32 before them and
 // have all of their exponentials' time; asked for in eighths, later, each wait stalled (2200 cycles again, 1300 without loads).
-// SIMPLE: the row sees every position; else those of `sees`.
+// SIMPLE: the row sees every position, and rest2 is not used; else those of `sees`, and rest2 is added.
 template <bool SIMPLE>
-__device__ __forceinline__ float softmax_pass(uint32_t t_s, float2 scale2, float2 mu2, const uint32_t (&sees)[4], uint32_t (&p)[64], float* total) {
+__device__ __forceinline__ float softmax_pass(uint32_t t_s, float2 scale2, float2 mu2, float2 rest2, const uint32_t (&sees)[4], uint32_t (&p)[64], float* total) {
     float s[2][32];
     float2 sum[2] = {};
     float top[2] = {-INFINITY, -INFINITY};
@@ -155,6 +159,7 @@ __device__ __forceinline__ float softmax_pass(uint32_t t_s, float2 scale2, float
         float &x = s[c & 1][2 * k], &y = s[c & 1][2 * k + 1];
         fma2(x, y, scale2, mu2);
         if (!SIMPLE) {
+            add_to2(x, y, rest2);
             if (!(sees[c] >> (2 * k) & 1u)) x = -INFINITY;
             if (!(sees[c] >> (2 * k) & 2u)) y = -INFINITY;
         }
@@ -348,7 +353,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
         const uint32_t t_s = lanes + static_cast<uint32_t>(i * 128), t_o = lanes + static_cast<uint32_t>(kTmemO + i * 128);
         // m: reference of the exponents, at most 15 below the row's largest so far and renewed where it is 8 below; grow: by how much, at
         // the next step.  Rows that have seen nothing have -infinity.
-        float m = -INFINITY, l = 0.0f, grow = 0.0f;
+        // From 2^23 on a 32-bit number's neighbours are 1 and more away.  The exponents are rounded once, behind the subtraction, so there the
+        // reference is m + rest, and m is taken from below, so that what is left to grow is above zero.
+        constexpr float kFar = 8388608.0f;
+        auto from_below = [&](float x) { return fabsf(x) < kFar ? x : __int_as_float(__float_as_int(x) + (x > 0.0f ? -1 : 1)); };
+        float m = -INFINITY, l = 0.0f, grow = 0.0f, rest = 0.0f;
         bool ok = true;
         for (int j = 0; j < (i < tiles ? steps : 0); ++j) {
             ok = park_warp(s_full(i), j & 1, s_abort);
@@ -371,10 +380,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
             }
             uint32_t p[64];
             float sum;
-            for (int turns = 0; turns < 2; ++turns) {
+            for (int turns = 0; turns < 3; ++turns) {       // the third one from 2^23 on
                 if (__any_sync(0xFFFFFFFFu, grow > 0.0f)) {
-                    const float f = ex2(-grow);
-                    m += grow;
+                    const float t = rest + grow, fresh = m + t, step = fresh - m;
+                    const float left = fabsf(fresh) < kFar ? 0.0f : (m - (fresh - step)) + (t - step);
+                    const float f = grow > 0.0f ? ex2(rest - left - step) : 1.0f;
+                    if (grow > 0.0f) {
+                        m = fresh;
+                        rest = left;
+                    }
                     l *= f;
                     grow = 0.0f;
                     if (j > 0) {
@@ -394,11 +408,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
                 }
                 const float mu = m == -INFINITY ? 0.0f : m;
                 const float2 scale2 = make_float2(to_log2, to_log2), mu2 = make_float2(-mu, -mu);
-                const float top = simple ? softmax_pass<true>(t_s, scale2, mu2, sees, p, &sum) : softmax_pass<false>(t_s, scale2, mu2, sees, p, &sum);
+                const float top = simple && __all_sync(0xFFFFFFFFu, fabsf(mu) < kFar) ? softmax_pass<true>(t_s, scale2, mu2, mu2, sees, p, &sum)
+                                                                                      : softmax_pass<false>(t_s, scale2, mu2, make_float2(-rest, -rest), sees, p, &sum);
                 // too large for fp16, or the row's first positions: again with the maximum known
                 const bool fresh = m == -INFINITY && top > -INFINITY, again = fresh || top > 15.0f;
-                if (fresh) m = top;
-                else if (top > 8.0f) grow = top;
+                if (fresh) m = from_below(top);
+                else if (top > 8.0f) grow = from_below(top);
                 if (!__any_sync(0xFFFFFFFFu, again)) break;
             }
             if (poisoned) {                 // behind the sum, which the values have no part in
@@ -451,8 +466,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) kv4_chunk_kernel(const __gri
                     for (int k = 0; k < 8; ++k) __stcg(out + k, make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]));
                 }
             }
-            if (mine && whole && a.lse != nullptr) a.lse[at_row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
-            if (mine && !whole) __stcg(a.part_ml + part, make_float2(m, l));
+            if (mine && whole && a.lse != nullptr) a.lse[at_row] = l == 0.0f ? -INFINITY : (m + (rest + log2f(l))) * kLn2;
+            if (mine && !whole) __stcg(a.part_ml + part, make_float2(m + rest, l));
         }
     } else if (warp < kMmaWarp) {
         // ================= operands: two threads a position =================

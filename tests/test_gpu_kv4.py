@@ -316,7 +316,7 @@ def test_attention_over_the_largest_values_is_finite(ops, tokens, heads, f32):
     assert np.all(np.abs(got - (v if f32 else np.clip(v, -65504, 65504))) <= 65504 * room)
 
 
-@pytest.mark.parametrize("tokens,f32", [(2, True), (9, True), (2, False)])
+@pytest.mark.parametrize("tokens,f32", [(2, True), (9, True), (2, False), (100, False)])
 @pytest.mark.parametrize("high", [10.2, 20.4, 22.7, 23.3, 23.8, 24.6, 25.3, 26.5, 27.4, 28.3, 28.9, 30.6, 33.1])
 def test_attention_with_scores_that_are_far_above_what_32_bits_count_in(ops, high, tokens, f32):
     """Scores of about 2^high in the exponent's base: from 2^24 on neighbouring 32-bit numbers are more than 1 apart, so the reference of the exponents
