@@ -469,9 +469,9 @@ W4A16_API int64_t w4a16_kv4_page_bytes(int page_size, int num_kv_heads);
  *   q_out = fp16(rot(q + q_bias)), cached key = Q4(fp16(rot(k + k_bias))), cached value = Q4(fp16(v + v_bias)),
  * sums and rotation in fp32.  rot turns the pairs (d, d + 64) by positions[token] * rope_inv_freq[d], the angle taken in
  * 64 bits.  q: fp16 [num_tokens] rows of num_q_heads * 128 (q_stride elements apart, 0: packed), q_out the same, may be q;
- * both may be NULL, and num_q_heads and q_stride are not looked at then.  k, v: rows of num_kv_heads * 128, kv_stride apart.  Biases may be NULL; positions NULL: the cached
- * position; rope_inv_freq fp32 [64], NULL: no rotation.  New positions start with key_weight 0.  Tensors 16-byte aligned,
- * strides multiples of 8.  No two tokens of a call may share a cached position.
+ * both may be NULL, and num_q_heads and q_stride are not looked at then.  k, v: rows of num_kv_heads * 128, kv_stride apart.  Biases may
+ * be NULL; positions NULL: the cached position; rope_inv_freq fp32 [64], NULL: no rotation.  New positions start with key_weight 0.
+ * Tensors 16-byte aligned, strides multiples of 8.  No two tokens of a call may share a cached position.
  */
 W4A16_API int w4a16_kv4_append(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, const void* q, const void* k,
                                const void* v, const void* q_bias, const void* k_bias, const void* v_bias,
@@ -492,8 +492,8 @@ W4A16_API int w4a16_kv4_read(const w4a16_kv4_cache* cache, const w4a16_kv4_batch
  * not overlap q.
  * Two forms: fp16 results of at least 64 query rows a sequence and head (tokens x shared heads, on average) run on tcgen05 with
  * values and weights rounded to fp16, so that weights below 2^-24 of a row's largest are lost.  All others keep the values exact;
- * a weight has 22 bits there for 32-bit results and 11 for fp16 ones, and is off by no less than 2^-31 of what the
- * largest weight times value scale comes to.  Keys are never rounded.
+ * a weight has 22 bits there for 32-bit results and 11 for fp16 ones, or is off by 2^-31 of the largest weight times value scale where that is
+ * more.  Keys are never rounded.  One form takes the whole call: prompts and single tokens of long sequences are faster as two calls.
  */
 W4A16_API int64_t w4a16_attention_kv4_workspace_bytes(int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads);
 W4A16_API int w4a16_attention_kv4(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, const void* q, void* out,
@@ -515,10 +515,10 @@ W4A16_API int w4a16_kv4_add_key_weights(const w4a16_kv4_cache* cache, const w4a1
  * the rest those with the largest key_weight (the earlier of equal ones; a NaN is the smallest).  What stays keeps its
  * order and is copied, rows and weights, to the pages of dst_block_table [num_seqs][dst_max_pages_per_seq]: pages of their own, none
  * twice and none of the sequences being cut; the old pages are left as they are, so pages shared with other sequences are
- * safe.  A kept position on a page number outside the pool moves nothing but counts: its fresh slot keeps what the page held, and calls on
- * the new pages see it, so cut only sequences whose pages are all there.  Sequences that fit are copied whole.  new_seq_lens [num_seqs] = min(length, budget), another array than seq_lens;
- * kept int32 [num_seqs][num_kv_heads][budget]: the old positions in order, -1 behind the last.  num_tokens and query_start
- * of the batch are not used.
+ * safe.  Sequences that fit are copied whole.  A kept position on a page number outside the pool moves nothing but counts: its fresh slot keeps
+ * what the page held, and calls on the new pages see it, so cut only sequences whose pages are all there.
+ * new_seq_lens [num_seqs] = min(length, budget), another array than seq_lens; kept int32 [num_seqs][num_kv_heads][budget]: the
+ * old positions in order, -1 behind the last.  num_tokens and query_start of the batch are not used.
  */
 W4A16_API int w4a16_kv4_evict(const w4a16_kv4_cache* cache, const w4a16_kv4_batch* batch, const int32_t* dst_block_table,
                               int32_t* new_seq_lens, int32_t* kept, int dst_max_pages_per_seq, int budget, int num_sink,
