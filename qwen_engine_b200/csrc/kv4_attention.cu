@@ -9,8 +9,8 @@
 //   scores^T [16 positions x 8 queries] = codes [16 x 128] . q^T;  then scale * score + zero * (sum of q), because a row is
 //       (code - 8) * scale + zero: the codes are exact in fp16 and no key is ever rounded.
 //   out^T [128 x 8] += codes^T [128 x 16] . (p * value scale)^T: for a 32-bit result the weight enters as two fp16 numbers
-//       whose sum has 22 bits, for an fp16 result as one (2^-12 of a weight is less than the result's own rounding, and
-//       the weights' roundings average out); zeros enter as one 32-bit sum a query.
+//       whose sum has 22 bits, for an fp16 result as one: its rounding and the result's own make 3.0e-4 where the
+//       latter is 2.1e-4 (64 sequences of up to 8190 positions: 100 us, with both parts 106); zeros enter as one 32-bit sum a query.
 //   reference of the exponents: not the largest score but the largest log2(p * value scale), so that what fp16 holds best is what counts most
 //       in the result, whatever the value scales are (rows that get most of the attention often have the smallest values).  Renewed
 //       where an fp16 weight could pass 2^15, which a vote finds, and set so that the largest is 2^6: a weight is off by 2^-31 of the

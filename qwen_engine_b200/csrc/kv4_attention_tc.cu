@@ -4,10 +4,11 @@
 // and walks over the positions 128 at a time:
 //   S_i [128 rows x 128 positions] = Q_i . K^T      both from shared memory
 //   P_i = 2^(S_i c - m), fp16, over S_i in tensor memory; m follows the running maximum, for the next step where it falls 8 behind, at
-//       once (the step's weights are worked out again) where 15, as fp16 ends at 2^16
+//       once (the step's weights are worked out again) where 15, as fp16 ends at 2^16.  Weights below 2^-24 of the largest are lost
 //   O_i [128 rows x 128 dims] += P_i . V            P from tensor memory, V (transposed: positions contiguous) from shared memory
 // While the softmax warps of one tile work the tensor core has the other one.  Keys and values become fp16 once for both tiles.  A
-// value is (code - 8) * scale + zero by one fma behind an exact conversion, so has one rounding.  A key has none: (code - 8) * scale
+// value is (code - 8) * scale + zero by one fma behind an exact conversion, so has one rounding (in two parts: 2.6e-4 instead of 3.3e-4 of a
+// result, but 970 us instead of 750 for a chunk of 1000 tokens at 32 100 positions and 32 heads on 8).  A key has none: (code - 8) * scale
 // has 15 bits at most and is the sum of two fp16 numbers, the product and what its rounding left (one fma), which are two operands;
 // its zero comes in as 16 more columns that all hold it, against the sum of q in two parts, an eighth in each of eight columns.
 // (Keys rounded to fp16 left 4e-4 in the lse of short sequences.  Exact codes as the operand and scale and zero in the softmax need two
