@@ -138,7 +138,7 @@ __device__ __forceinline__ void add_part(float4& x, float& sum, const float4& p,
 // top + log2(sum).  The sum may be far from 1, and its exponent goes to top first, where the two cancel.
 __device__ __forceinline__ float log2_of_sum(float top, float sum) {
     const uint32_t bits = __float_as_uint(sum);
-    const int e = static_cast<int>(bits >> 23) - 127;        // 128: an infinity or a NaN
+    const int e = static_cast<int>(bits >> 23 & 255u) - 127; // 128: an infinity or a NaN
     return e == 128 ? top + sum : (top + static_cast<float>(e)) + log2f(__uint_as_float((bits & 0x007FFFFFu) | 0x3F800000u));
 }
 // A finished row: a warp, four dimensions a lane.

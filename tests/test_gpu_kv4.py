@@ -358,6 +358,20 @@ def test_attention_with_scores_that_are_far_above_what_32_bits_count_in(ops, hig
             assert abs(lse[i, h] - wl) <= 2.0 ** -21 * abs(wl), (i, h, lse[i, h] / wl - 1)
 
 
+@pytest.mark.parametrize("sign", [0, 0x80008000])
+@pytest.mark.parametrize("heads,f32", [(4, True), (4, False), (40, False)])
+def test_a_poisoned_key_makes_lse_of_the_tokens_that_see_it_nan(ops, heads, f32, sign):
+    lens, new, kv, page = [300], [20], 1, 16
+    rng, pool, table, cache, batch = make(ops, 26, lens, new, kv, page)
+    q = rng.standard_normal((20, heads, 128)).astype(BF)
+    cache.pages[int(table[0, 290 // page]), 0, 32 * page + 290 % page] = int(np.uint32(0x7E007E00 | sign).view(np.int32))
+    got, lse = attend(ops, cache, batch, util.to_dev(q), heads, f32)
+    want = ref.attention(pool, table, lens, new, q, SCALE, not few_rows(batch, heads, cache, f32))
+    # token i is position 280 + i
+    assert np.isnan(lse[10:20]).all() and np.isnan(got[10:20]).all()
+    assert np.all(np.abs(lse[:10] - want[1][:10]) <= want[3][:10]) and np.isfinite(got[:10]).all()
+
+
 @pytest.mark.parametrize("heads,f32", [(4, True), (4, False), (40, False)])
 def test_a_poisoned_value_leaves_lse_and_weights_alone(ops, heads, f32):
     """The logarithm of the sum and the attention weights come from queries and keys: a value row of NaNs reaches the outputs only."""
