@@ -578,7 +578,7 @@ def check_eviction(ops, lens, kv, page, budget, sink, recent, weight_of, stale=0
     assert util.to_np(new_lens).tolist() == [min(L, budget) for L in lens]
     for b, L in enumerate(lens):
         for h in range(kv):
-            want = np.array(ref.evict(weight, table[b], L, h, page, n, budget, sink, recent))
+            want = np.array(ref.evict(weight, table[b], L, h, page, n, budget, sink, recent), dtype=np.int64)
             assert np.array_equal(kept[b, h], np.append(want, np.full(budget - len(want), -1))), (b, h)
             new = np.arange(len(want))
             from_, to = (table[b, want // page], h, want % page), (dst[b, new // page], h, new % page)
